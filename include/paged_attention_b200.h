@@ -264,6 +264,120 @@ typedef struct pa_gather_args {
  * unbounded. */
 PA_API int pa_decode_gather(const pa_decode_args* args, const pa_gather_args* gather, void* stream);
 
+/* ---- caches held in 8 bits ------------------------------------------------
+ * Codes are e4m3 bytes laid out like any cache view (strides in elements =
+ * bytes); value = code * scale[block, head].  Scales are fp32, >= 0. */
+typedef struct pa_cache_scales {
+  float* key_scales;             /* of key_cache: [num_blocks, num_kv_heads] */
+  int64_t key_stride_block, key_stride_head;
+  float* value_scales;           /* of value_cache */
+  int64_t value_stride_block, value_stride_head;
+} pa_cache_scales;
+
+/* Two runs of tokens of one pa_kv_append_8bit call lie in the same block, or a
+ * pa_pages_copy destination is another pair's source or an earlier pair's
+ * destination: the later run / the pair is left out. */
+#define PA_DEVERR_BLOCK_CONFLICT 0x40u
+
+/* pa_kv_append into an 8-bit cache.  args->dtype is the new rows' type (fp32,
+ * fp16 or bf16); the cache views hold e4m3 bytes, head_dim is a multiple of 16,
+ * block_size a power of two in [8, 256], cache rows 16-byte aligned.
+ * For each block and head: need = 2^e, the smallest e >= -100 with the new rows'
+ * largest finite magnitude <= 448 * 2^e.  A write at offset 0 starts the block anew
+ * (scale = need; what else it held is void); otherwise scale = max(held, need), and
+ * where that grows the block's other codes are rounded again to it.  Rounding is
+ * to nearest even, infinities saturate, NaN stays NaN.  All tokens of a call for
+ * one block must be one row's, without a token of another block between them
+ * (PA_DEVERR_BLOCK_CONFLICT else); of a slot given twice the last one counts. */
+PA_API int pa_kv_append_8bit(const pa_kv_append_args* args, const pa_cache_scales* scales, void* stream);
+
+/* ---- changed scores --------------------------------------------------------
+ * For the query token at position i = L_b - q_len + t and the key at j:
+ *   s = scale * (q . k_j);  s = softcap * tanh(s / softcap) when softcap > 0;
+ *   s -= alibi_slopes[hq] * |i - j|
+ * and the token sees j when key_starts[b, t] <= j, i - j < window (window > 0), and
+ * j <= i or j < prefix_lens[b].  A token that sees nothing gives a zero row.  What a
+ * token does not see does not reach its row, whatever the cache holds there;
+ * blocks before a row's first visible key are not read (their table entries may
+ * be anything). */
+typedef struct pa_score_modifiers {
+  float softcap;                 /* 0: none */
+  int32_t window;                /* 0: none */
+  const float* alibi_slopes;     /* [num_q_heads] or NULL */
+  const int32_t* key_starts;     /* first key of token (b, t) (a document's start), or NULL */
+  int64_t key_starts_stride_b, key_starts_stride_t;
+  const int32_t* prefix_lens;    /* [batch] or NULL */
+} pa_score_modifiers;
+
+/* pa_decode over an 8-bit cache (scales != NULL: args->dtype is the type of query
+ * and out, fp16 or bf16; head_dim a multiple of 16) and / or with changed scores
+ * (modifiers != NULL; any dtype).  Same workspace as pa_decode. */
+PA_API int pa_decode_ext(const pa_decode_args* args, const pa_cache_scales* scales,
+                         const pa_score_modifiers* modifiers, void* stream);
+
+/* ---- pages of a cache ------------------------------------------------------
+ * Caches whose pages move together, each [num_blocks, ...]: a page is `segments`
+ * runs of segment_bytes, stride_segment apart.  Strides in BYTES. */
+#define PA_MAX_PAGE_VIEWS 8
+typedef struct pa_page_view {
+  void* data;
+  int64_t stride_block;
+  int64_t segments;
+  int64_t stride_segment;
+  int64_t segment_bytes;
+} pa_page_view;
+
+/* Sequences over a pool of pages, all of it on the device.  Slot s holds
+ * seq_lens[s] tokens in pages block_tables[s, 0 .. ceil(len / block_size)), -1
+ * behind; ref_counts[page] is the number of table entries that hold the page. */
+typedef struct pa_page_tables {
+  int32_t* block_tables;         /* [num_seqs, >= max_blocks] */
+  int64_t block_table_stride;
+  int32_t num_seqs, max_blocks;
+  int32_t* seq_lens;             /* [num_seqs] */
+  int32_t* ref_counts;           /* [num_blocks] */
+  int32_t num_blocks, block_size;
+  int32_t* scratch;              /* pa_pages_scratch_words() words; one call at a time */
+  uint32_t* error_flags;         /* receives PA_DEVERR_* bits (may be NULL) */
+} pa_page_tables;
+
+/* A sequence slot outside the table or named twice, a child that is not empty, a
+ * negative count, or counts that disagree with the tables: that slot is left. */
+#define PA_DEVERR_SEQUENCE 0x80u
+/* Not enough free pages: the slots that did not get all of theirs are left. */
+#define PA_DEVERR_PAGES_EXHAUSTED 0x100u
+
+/* int32 words of pa_page_tables.scratch. */
+PA_API size_t pa_pages_scratch_words(int32_t num_seqs, int32_t num_blocks);
+
+/* Page src[i] of every view becomes page dst[i]; pairs with a negative id are
+ * padding.  Destinations must differ and be no pair's source.  The reference
+ * copies with torch indexing, once per tensor (GpuKVBlockPool.copy_blocks,
+ * runtime/phase2/paged_kv_kernel.py:233-250). */
+PA_API int pa_pages_copy(const pa_page_view* views, int32_t num_views, int32_t num_blocks, const int32_t* src,
+                         const int32_t* dst, int32_t n, uint32_t* error_flags, void* stream);
+
+/* Each slot's pages lose a holder and the slot becomes empty (negative: padding;
+ * a slot named twice is freed once).  n <= num_seqs here and below. */
+PA_API int pa_pages_free(const pa_page_tables* tables, const int32_t* slots, int32_t n, void* stream);
+
+/* Empty slot children[i] gets the tokens of parents[i]: full pages are shared, the
+ * page in use is copied (in every view) to the lowest free one, in the order of
+ * the pairs.  A negative parent or child: padding. */
+PA_API int pa_pages_fork(const pa_page_tables* tables, const int32_t* parents, const int32_t* children, int32_t n,
+                         const pa_page_view* views, int32_t num_views, void* stream);
+
+/* Slot slots[i] grows by tokens[i]: new pages, the lowest free ones in the order
+ * of the slots. */
+PA_API int pa_pages_reserve(const pa_page_tables* tables, const int32_t* slots, const int32_t* tokens, int32_t n,
+                            void* stream);
+
+/* Moves the live pages to ids [0, *live) (live: device word that receives their
+ * number): the k-th live page at or above it to the k-th free page below it, in
+ * ascending order.  Tables and counts follow. */
+PA_API int pa_pages_compact(const pa_page_tables* tables, const pa_page_view* views, int32_t num_views,
+                            int32_t* live, void* stream);
+
 /* Size of the scratch array behind pa_decode_static_workspace (16 MiB). */
 #define PA_STATIC_WORKSPACE_BYTES (16u << 20)
 

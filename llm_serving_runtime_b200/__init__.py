@@ -9,6 +9,13 @@ Public entry points
                                       (paged_attention_decode(..., prefix_groups=))
   shared_blocks.BlockRefAllocator     refcounted KV blocks: prefix-cache snapshots and
                                       hits share blocks instead of copying them
+  score_modifiers.ScoreModifiers      capped, biased and masked scores
+                                      (paged_attention_decode(..., score_modifiers=))
+  key_scales= / value_scales=         caches held in 8 bits (kv_append and
+                                      paged_attention_decode; kv_block_pool.Fp8KVBlockPool)
+  device_pages.DevicePages, copy_pages
+                                      pages copied, forked, freed, reserved and compacted
+                                      on the device
   reference_api                       drop-in for runtime/phase2/paged_attention_triton.py
   kv_block_pool.write_tokens_batch_into
                                       the reference pool's write_tokens_batch on the append kernel
@@ -18,6 +25,7 @@ Public entry points
 The kernels live in lib/libpa_b200.so (C ABI: include/paged_attention_b200.h).
 """
 
+from .device_pages import DevicePages, copy_pages  # noqa: F401
 from .paged_attention import (  # noqa: F401
     DeviceErrorFlags,
     decode_workspace,
@@ -27,5 +35,6 @@ from .paged_attention import (  # noqa: F401
     read_device_errors,
 )
 from .prefix_sharing import PrefixGroups, find_shared_prefixes  # noqa: F401
+from .score_modifiers import ScoreModifiers  # noqa: F401
 
 __version__ = "1.0.0"

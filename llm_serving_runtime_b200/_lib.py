@@ -29,12 +29,19 @@ PA_DEVERR_SLOT_RANGE = 0x4
 PA_DEVERR_WAIT_TIMEOUT = 0x8
 PA_DEVERR_PREFIX = 0x10
 PA_DEVERR_GATHER = 0x20
+PA_DEVERR_BLOCK_CONFLICT = 0x40
+PA_DEVERR_SEQUENCE = 0x80
+PA_DEVERR_PAGES_EXHAUSTED = 0x100
+
+PA_MAX_PAGE_VIEWS = 8
 
 PA_STATIC_WORKSPACE_BYTES = 16 << 20
 
 EXPORTED_SYMBOLS = (
     "pa_kv_append",
+    "pa_kv_append_8bit",
     "pa_decode",
+    "pa_decode_ext",
     "pa_decode_static_workspace",
     "pa_decode_cascade",
     "pa_cascade_workspace_bytes",
@@ -42,6 +49,12 @@ EXPORTED_SYMBOLS = (
     "pa_ipc_export",
     "pa_ipc_import",
     "pa_ipc_release",
+    "pa_pages_scratch_words",
+    "pa_pages_copy",
+    "pa_pages_free",
+    "pa_pages_fork",
+    "pa_pages_reserve",
+    "pa_pages_compact",
     "pa_decode_workspace_bytes",
     "pa_workspace_init",
     "pa_read_device_errors",
@@ -160,6 +173,49 @@ class GatherArgs(ctypes.Structure):
     ]
 
 
+class CacheScalesArgs(ctypes.Structure):
+    _fields_ = [
+        ("key_scales", _vp),
+        ("key_stride_block", _i64), ("key_stride_head", _i64),
+        ("value_scales", _vp),
+        ("value_stride_block", _i64), ("value_stride_head", _i64),
+    ]
+
+
+class ScoreModifiersArgs(ctypes.Structure):
+    _fields_ = [
+        ("softcap", ctypes.c_float),
+        ("window", _i32),
+        ("alibi_slopes", _vp),
+        ("key_starts", _vp),
+        ("key_starts_stride_b", _i64), ("key_starts_stride_t", _i64),
+        ("prefix_lens", _vp),
+    ]
+
+
+class PageViewArgs(ctypes.Structure):
+    _fields_ = [
+        ("data", _vp),
+        ("stride_block", _i64),
+        ("segments", _i64),
+        ("stride_segment", _i64),
+        ("segment_bytes", _i64),
+    ]
+
+
+class PageTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("block_tables", _vp),
+        ("block_table_stride", _i64),
+        ("num_seqs", _i32), ("max_blocks", _i32),
+        ("seq_lens", _vp),
+        ("ref_counts", _vp),
+        ("num_blocks", _i32), ("block_size", _i32),
+        ("scratch", _vp),
+        ("error_flags", _vp),
+    ]
+
+
 _lock = threading.Lock()
 _handle: ctypes.CDLL | None = None
 
@@ -194,6 +250,24 @@ def load() -> ctypes.CDLL:
         lib.pa_ipc_import.argtypes = [ctypes.POINTER(IpcHandle), ctypes.POINTER(_vp)]
         lib.pa_ipc_release.restype = ctypes.c_int
         lib.pa_ipc_release.argtypes = [_vp]
+        lib.pa_kv_append_8bit.restype = ctypes.c_int
+        lib.pa_kv_append_8bit.argtypes = [ctypes.POINTER(KvAppendArgs), ctypes.POINTER(CacheScalesArgs), _vp]
+        lib.pa_decode_ext.restype = ctypes.c_int
+        lib.pa_decode_ext.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(CacheScalesArgs),
+                                      ctypes.POINTER(ScoreModifiersArgs), _vp]
+        views, tables = ctypes.POINTER(PageViewArgs), ctypes.POINTER(PageTablesArgs)
+        lib.pa_pages_scratch_words.restype = _sz
+        lib.pa_pages_scratch_words.argtypes = [_i32, _i32]
+        lib.pa_pages_copy.restype = ctypes.c_int
+        lib.pa_pages_copy.argtypes = [views, _i32, _i32, _vp, _vp, _i32, _vp, _vp]
+        lib.pa_pages_free.restype = ctypes.c_int
+        lib.pa_pages_free.argtypes = [tables, _vp, _i32, _vp]
+        lib.pa_pages_fork.restype = ctypes.c_int
+        lib.pa_pages_fork.argtypes = [tables, _vp, _vp, _i32, views, _i32, _vp]
+        lib.pa_pages_reserve.restype = ctypes.c_int
+        lib.pa_pages_reserve.argtypes = [tables, _vp, _vp, _i32, _vp]
+        lib.pa_pages_compact.restype = ctypes.c_int
+        lib.pa_pages_compact.argtypes = [tables, views, _i32, _vp, _vp]
         lib.pa_decode_workspace_bytes.restype = _sz
         lib.pa_decode_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32, _i32]
         lib.pa_workspace_init.restype = ctypes.c_int

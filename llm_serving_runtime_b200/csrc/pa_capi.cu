@@ -122,13 +122,14 @@ int check_cache_view(const pa_cache_view& v, const char* name) {
 }
 
 // 4-D tensor map (head_dim, token, kv head, block) with 128-byte swizzle and a
-// box of (64 elements, min(bs, 16) tokens, 1, 1).
+// box of (64 elements, min(bs, 16) tokens, 1, 1).  tile8: an 8-bit cache and its
+// tile's columns: a box of (tile8 bytes, ...), swizzled over its own row.
 int encode_cache_map(CUtensorMap* map, const pa_cache_view& v, int dtype, int D, int bs, int Hkv,
-                     const char* name) {
+                     const char* name, int tile8 = 0) {
   PFN_cuTensorMapEncodeTiled_v12000 enc;
   int st = get_encode(&enc);
   if (st != PA_OK) return st;
-  const int e = elem_bytes(dtype);
+  const int e = tile8 ? 1 : elem_bytes(dtype);
   if (!aligned_ptr(v.data, 16))
     return fail(PA_ERR_UNSUPPORTED, "%s: base address must be 16-byte aligned", name);
   const int64_t sb[3] = {v.stride_token * e, v.stride_head * e, v.stride_block * e};
@@ -137,14 +138,30 @@ int encode_cache_map(CUtensorMap* map, const pa_cache_view& v, int dtype, int D,
       return fail(PA_ERR_UNSUPPORTED, "%s: strides must be multiples of 16 bytes", name);
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)bs, (cuuint64_t)Hkv, (cuuint64_t)v.num_blocks};
   cuuint64_t strides[3] = {(cuuint64_t)sb[0], (cuuint64_t)sb[1], (cuuint64_t)sb[2]};
-  cuuint32_t box[4] = {64u, (cuuint32_t)(bs < 16 ? bs : 16), 1u, 1u};
+  cuuint32_t box[4] = {tile8 ? (cuuint32_t)tile8 : 64u, (cuuint32_t)(bs < 16 ? bs : 16), 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  CUresult r = enc(map, dtype == PA_DTYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+  CUresult r = enc(map, tile8                        ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                        : dtype == PA_DTYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                    4, v.data, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   tile8 == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PA_ERR_UNSUPPORTED, "%s: cuTensorMapEncodeTiled failed (%d)", name, (int)r);
+  return PA_OK;
+}
+
+// What the 8-bit kernels need of a cache beyond check_cache_view (A: the append's
+// or the decode's arguments).
+template <typename A>
+int check_cache_8bit(const A& a, int bs, int head_dim) {
+  if (head_dim % 16 != 0)
+    return fail(PA_ERR_UNSUPPORTED, "an 8-bit cache needs a head_dim that is a multiple of 16, got %d", head_dim);
+  if (bs < 8 || bs > 256 || (bs & (bs - 1)) != 0)
+    return fail(PA_ERR_UNSUPPORTED, "an 8-bit cache needs a power-of-two block_size in [8, 256], got %d", bs);
+  for (const pa_cache_view* v : {&a.key_cache, &a.value_cache})
+    if (!aligned_ptr(v->data, 16) || ((v->stride_block | v->stride_head | v->stride_token) & 15) != 0)
+      return fail(PA_ERR_UNSUPPORTED, "an 8-bit cache needs 16-byte aligned rows");
   return PA_OK;
 }
 
@@ -315,7 +332,7 @@ int pa_read_device_errors(void* device_word, uint32_t* host_flags, int32_t clear
   return PA_OK;
 }
 
-int pa_kv_append(const pa_kv_append_args* a, void* stream) {
+static int append_impl(const pa_kv_append_args* a, const pa_cache_scales* sc, void* stream) {
   g_last_error[0] = 0;
   if (a == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null args");
   if (a->dtype < PA_DTYPE_FLOAT32 || a->dtype > PA_DTYPE_BFLOAT16)
@@ -335,6 +352,17 @@ int pa_kv_append(const pa_kv_append_args* a, void* stream) {
     if (a->block_tables == nullptr || a->positions == nullptr)
       return fail(PA_ERR_INVALID_ARGUMENT, "without slot_mapping, block_tables and positions are required");
     if (a->max_blocks <= 0) return fail(PA_ERR_INVALID_ARGUMENT, "max_blocks must be positive");
+  }
+  if (sc != nullptr) {
+    if (sc->key_scales == nullptr || sc->value_scales == nullptr)
+      return fail(PA_ERR_INVALID_ARGUMENT, "key_scales and value_scales must be given");
+    st = check_cache_8bit(*a, a->block_size, a->head_dim);
+    if (st != PA_OK) return st;
+    // one CTA for each block a row can touch, or each slot
+    const long long runs = a->slot_mapping != nullptr ? a->q_len
+                                                      : ((long long)a->q_len + a->block_size - 2) / a->block_size + 1;
+    if (runs * a->batch > (1LL << 30))
+      return fail(PA_ERR_UNSUPPORTED, "batch * q_len too large");
   }
   pa::AppendParams p;
   p.key = a->key;
@@ -368,9 +396,24 @@ int pa_kv_append(const pa_kv_append_args* a, void* stream) {
   p.bs = a->block_size;
   p.elem_bytes = elem_bytes(a->dtype);
   p.error_flags = a->error_flags;
+  if (sc != nullptr) {
+    const pa::ScaleParams s8 = {sc->key_scales,       sc->value_scales,       sc->key_stride_block,
+                                sc->key_stride_head, sc->value_stride_block, sc->value_stride_head};
+    cudaError_t e8 = pa::launch_kv_append8(p, s8, a->dtype, static_cast<cudaStream_t>(stream));
+    if (e8 != cudaSuccess) return cuda_fail(e8, "kv_append_8bit launch");
+    return PA_OK;
+  }
   cudaError_t e = pa::launch_kv_append(p, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "kv_append launch");
   return PA_OK;
+}
+
+int pa_kv_append(const pa_kv_append_args* a, void* stream) { return append_impl(a, nullptr, stream); }
+
+int pa_kv_append_8bit(const pa_kv_append_args* a, const pa_cache_scales* scales, void* stream) {
+  g_last_error[0] = 0;
+  if (scales == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null scales");
+  return append_impl(a, scales, stream);
 }
 
 size_t pa_cascade_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t q_len,
@@ -388,7 +431,7 @@ size_t pa_cascade_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t nu
 }
 
 static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, const pa_gather_args* gat,
-                       void* stream);
+                       void* stream, const pa_cache_scales* sc = nullptr, const pa_score_modifiers* sm = nullptr);
 
 int pa_decode(const pa_decode_args* a, void* stream) { return decode_impl(a, nullptr, nullptr, stream); }
 
@@ -457,8 +500,26 @@ int pa_decode_cascade(const pa_decode_args* a, const pa_prefix_groups* grp, void
   return decode_impl(a, grp->num_groups > 0 ? grp : nullptr, nullptr, stream);
 }
 
+int pa_decode_ext(const pa_decode_args* a, const pa_cache_scales* scales, const pa_score_modifiers* modifiers,
+                  void* stream) {
+  g_last_error[0] = 0;
+  if (a == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null args");
+  if (scales != nullptr) {
+    if (scales->key_scales == nullptr || scales->value_scales == nullptr)
+      return fail(PA_ERR_INVALID_ARGUMENT, "key_scales and value_scales must be given");
+    if (a->dtype == PA_DTYPE_FLOAT32)
+      return fail(PA_ERR_UNSUPPORTED, "8-bit caches are attended by fp16/bf16 queries");
+  }
+  if (modifiers != nullptr) {
+    if (!(modifiers->softcap >= 0.f) || !(modifiers->softcap < 1e30f))
+      return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be 0 (none) or positive and finite");
+    if (modifiers->window < 0) return fail(PA_ERR_INVALID_ARGUMENT, "window must be 0 (none) or positive");
+  }
+  return decode_impl(a, nullptr, nullptr, stream, scales, modifiers);
+}
+
 static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, const pa_gather_args* gat,
-                       void* stream) {
+                       void* stream, const pa_cache_scales* sc, const pa_score_modifiers* sm) {
   g_last_error[0] = 0;
   if (a == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null args");
   const int dtype = a->dtype;
@@ -540,6 +601,29 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.status = static_cast<uint32_t*>(a->workspace);
   p.slot_rows = s.slot_rows;
+  if (sc != nullptr) {
+    st = check_cache_8bit(*a, bs, Dv);
+    if (st != PA_OK) return st;
+    p.k_scales = sc->key_scales;
+    p.ks_sblk = sc->key_stride_block;
+    p.ks_sh = sc->key_stride_head;
+    p.v_scales = sc->value_scales;
+    p.vs_sblk = sc->value_stride_block;
+    p.vs_sh = sc->value_stride_head;
+  }
+  if (sm != nullptr) {
+    p.scored = 1;
+    p.window = sm->window;
+    p.softcap = sm->softcap;
+    p.softcap_log2 = sm->softcap * 1.4426950408889634f;
+    p.inv_softcap_log2 = sm->softcap > 0.f ? 1.f / p.softcap_log2 : 0.f;
+    p.alibi_slopes = sm->alibi_slopes;
+    p.key_starts = sm->key_starts;
+    p.kst_sb = sm->key_starts_stride_b;
+    p.kst_st = sm->key_starts_stride_t;
+    p.prefix_lens = sm->prefix_lens;
+  }
+  const bool ext = sc != nullptr || sm != nullptr;
   const bool pdl = a->allow_overlap_with_previous != 0;
   cudaStream_t strm = static_cast<cudaStream_t>(stream);
 
@@ -613,19 +697,37 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
 
   // Ring depth: as many 16-token stages per warp as shared memory allows (2..8).
   const size_t budget = (size_t)info->max_smem_optin - 128;  // static shared memory of the kernel (96 B)
+  auto smem_bytes = [&](int n) {
+    return ext ? pa::decode_ext_smem_bytes(D, p.B, n, sc != nullptr, sm != nullptr)
+               : pa::decode_mma_smem_bytes(D, p.B, n, cascade);
+  };
   int stages = 8;
-  while (stages >= 2 && pa::decode_mma_smem_bytes(D, p.B, stages, cascade) > budget) --stages;
+  while (stages >= 2 && smem_bytes(stages) > budget) --stages;
   if (stages < 2)
     return fail(PA_ERR_UNSUPPORTED, "batch %d too large for the decode kernel's shared memory", p.B);
   p.stages = stages;
-  const size_t smem = pa::decode_mma_smem_bytes(D, p.B, stages, cascade);
+  const size_t smem = smem_bytes(stages);
 
   CUtensorMap tmk, tmv;
   // the maps' rows are the real head_dim: TMA fills the columns past it with zeros
-  st = encode_cache_map(&tmk, a->key_cache, dtype, Dv, bs, p.Hkv, "key_cache");
+  st = encode_cache_map(&tmk, a->key_cache, dtype, Dv, bs, p.Hkv, "key_cache", sc != nullptr ? D : 0);
   if (st != PA_OK) return st;
-  st = encode_cache_map(&tmv, a->value_cache, dtype, Dv, bs, p.Hkv, "value_cache");
+  st = encode_cache_map(&tmv, a->value_cache, dtype, Dv, bs, p.Hkv, "value_cache", sc != nullptr ? D : 0);
   if (st != PA_OK) return st;
+
+  if (ext) {
+    // as below: many query rows per KV head share K/V tiles, few split the work
+    if (p.GQ >= 64 && (long long)p.B * p.Hkv * ((p.GQ + 127) / 128) >= info->num_sms) {
+      g_last_kernel = "pa::prefill_mma_kernel<ext>";
+      e = pa::launch_prefill_ext(p, tmk, tmv, dtype, pdl, strm);
+      if (e != cudaSuccess) return cuda_fail(e, "multi-query launch");
+      return PA_OK;
+    }
+    g_last_kernel = "pa::decode_mma_kernel<ext>";
+    e = pa::launch_decode_ext(p, tmk, tmv, dtype, grid, smem, pdl, strm);
+    if (e != cudaSuccess) return cuda_fail(e, "decode launch");
+    return PA_OK;
+  }
 
   {
     const int di = dtype, dj = D == 128 ? 1 : 0;
@@ -689,6 +791,136 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   g_last_kernel = "pa::decode_mma_kernel";
   e = pa::launch_decode_mma(p, tmk, tmv, dtype, grid, smem, pdl, strm);
   if (e != cudaSuccess) return cuda_fail(e, "decode launch");
+  return PA_OK;
+}
+
+// ---- pages ----------------------------------------------------------------------
+
+static int page_views(const pa_page_view* views, int32_t num_views, pa::PageViews* out) {
+  if (num_views < 0 || num_views > PA_MAX_PAGE_VIEWS)
+    return fail(PA_ERR_INVALID_ARGUMENT, "0 to %d caches, got %d", PA_MAX_PAGE_VIEWS, num_views);
+  if (num_views > 0 && views == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null page views");
+  memset(out, 0, sizeof(*out));
+  int64_t total = 0;
+  for (int i = 0; i < num_views; ++i) {
+    const pa_page_view& v = views[i];
+    if (v.segments < 0 || v.segment_bytes < 0 || v.stride_block < 0 || v.stride_segment < 0)
+      return fail(PA_ERR_INVALID_ARGUMENT, "page view %d: negative size or stride", i);
+    if (v.segments == 0 || v.segment_bytes == 0) continue;  // pages without bytes
+    if (v.data == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "page view %d: null data pointer", i);
+    if (v.segments > (int64_t(1) << 40) / v.segment_bytes || v.segments * v.segment_bytes > (int64_t(1) << 29))
+      return fail(PA_ERR_UNSUPPORTED, "page view %d: a page of more than 2^29 bytes", i);
+    out->v[out->n++] = {v.data, v.stride_block, v.segments, v.segments > 1 ? v.stride_segment : 0, v.segment_bytes};
+    total += v.segments * v.segment_bytes;
+  }
+  if (total > (int64_t(1) << 30) - (1 << 15)) return fail(PA_ERR_UNSUPPORTED, "pages of more than 2^30 bytes");
+  return PA_OK;
+}
+
+static int page_tables(const pa_page_tables* t, int32_t n, pa::PageTables* out) {
+  if (t == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null tables");
+  if (t->num_seqs <= 0 || t->max_blocks <= 0 || t->num_blocks <= 0 || t->block_size <= 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "num_seqs, max_blocks, num_blocks and block_size must be positive");
+  if ((int64_t)t->max_blocks * t->block_size > (int64_t(1) << 30) || t->max_blocks > (1 << 20) ||
+      t->num_blocks > (1 << 28) || t->num_seqs > (1 << 24))
+    return fail(PA_ERR_UNSUPPORTED, "tables too large");
+  if (t->block_table_stride < t->max_blocks)
+    return fail(PA_ERR_INVALID_ARGUMENT, "block_table_stride must be at least max_blocks");
+  if (t->block_tables == nullptr || t->seq_lens == nullptr || t->ref_counts == nullptr || t->scratch == nullptr)
+    return fail(PA_ERR_INVALID_ARGUMENT, "block_tables, seq_lens, ref_counts and scratch must be given");
+  if (n < 0 || n > t->num_seqs)
+    return fail(PA_ERR_INVALID_ARGUMENT, "0 to num_seqs (%d) slots, got %d", t->num_seqs, n);
+  *out = {t->block_tables, t->block_table_stride, t->num_seqs, t->max_blocks, t->seq_lens, t->ref_counts,
+          t->num_blocks, t->block_size, t->scratch, t->error_flags};
+  return PA_OK;
+}
+
+static int current_device(DeviceInfo** info) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  return device_info(dev, info);
+}
+
+size_t pa_pages_scratch_words(int32_t num_seqs, int32_t num_blocks) {
+  if (num_seqs <= 0 || num_blocks <= 0) return 0;
+  return 3 * (size_t)num_seqs + 2 * (size_t)num_blocks + 8;
+}
+
+int pa_pages_copy(const pa_page_view* views, int32_t num_views, int32_t num_blocks, const int32_t* src,
+                  const int32_t* dst, int32_t n, uint32_t* error_flags, void* stream) {
+  g_last_error[0] = 0;
+  pa::PageViews pv;
+  int st = page_views(views, num_views, &pv);
+  if (st != PA_OK) return st;
+  if (num_blocks <= 0 || n < 0) return fail(PA_ERR_INVALID_ARGUMENT, "num_blocks must be positive, n not negative");
+  if (n == 0 || pv.n == 0) return PA_OK;
+  if (src == nullptr || dst == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "src and dst must be given");
+  DeviceInfo* info = nullptr;
+  st = current_device(&info);
+  if (st != PA_OK) return st;
+  cudaError_t e =
+      pa::launch_pages_copy(pv, src, dst, n, num_blocks, info->num_sms, error_flags, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pages_copy launch");
+  return PA_OK;
+}
+
+int pa_pages_free(const pa_page_tables* t, const int32_t* slots, int32_t n, void* stream) {
+  g_last_error[0] = 0;
+  pa::PageTables pt;
+  int st = page_tables(t, n, &pt);
+  if (st != PA_OK) return st;
+  if (n == 0) return PA_OK;
+  if (slots == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "slots must be given");
+  cudaError_t e = pa::launch_pages_free(pt, slots, n, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pages_free launch");
+  return PA_OK;
+}
+
+int pa_pages_fork(const pa_page_tables* t, const int32_t* parents, const int32_t* children, int32_t n,
+                  const pa_page_view* views, int32_t num_views, void* stream) {
+  g_last_error[0] = 0;
+  pa::PageTables pt;
+  pa::PageViews pv;
+  int st = page_tables(t, n, &pt);
+  if (st != PA_OK) return st;
+  st = page_views(views, num_views, &pv);
+  if (st != PA_OK) return st;
+  if (n == 0) return PA_OK;
+  if (parents == nullptr || children == nullptr)
+    return fail(PA_ERR_INVALID_ARGUMENT, "parents and children must be given");
+  cudaError_t e = pa::launch_pages_fork(pt, parents, children, n, pv, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pages_fork launch");
+  return PA_OK;
+}
+
+int pa_pages_reserve(const pa_page_tables* t, const int32_t* slots, const int32_t* tokens, int32_t n, void* stream) {
+  g_last_error[0] = 0;
+  pa::PageTables pt;
+  int st = page_tables(t, n, &pt);
+  if (st != PA_OK) return st;
+  if (n == 0) return PA_OK;
+  if (slots == nullptr || tokens == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "slots and tokens must be given");
+  cudaError_t e = pa::launch_pages_reserve(pt, slots, tokens, n, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pages_reserve launch");
+  return PA_OK;
+}
+
+int pa_pages_compact(const pa_page_tables* t, const pa_page_view* views, int32_t num_views, int32_t* live,
+                     void* stream) {
+  g_last_error[0] = 0;
+  pa::PageTables pt;
+  pa::PageViews pv;
+  int st = page_tables(t, 0, &pt);
+  if (st != PA_OK) return st;
+  st = page_views(views, num_views, &pv);
+  if (st != PA_OK) return st;
+  if (live == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "live must be given");
+  DeviceInfo* info = nullptr;
+  st = current_device(&info);
+  if (st != PA_OK) return st;
+  cudaError_t e = pa::launch_pages_compact(pt, pv, live, info->num_sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "pages_compact launch");
   return PA_OK;
 }
 

@@ -110,7 +110,45 @@ struct DecodeParams {
   uint32_t* done_warps;         // warps finished in this call (zero between calls)
   int32_t n_ranks, rank, head_offset;
   int64_t wait_ns;
+  // 8-bit caches (pa_decode_ext with scales): one fp32 scale per block and KV
+  // head; k_scales is null otherwise.  Strides in elements.
+  const float* k_scales;
+  const float* v_scales;
+  int64_t ks_sblk, ks_sh, vs_sblk, vs_sh;
+  // Changed scores (pa_decode_ext with modifiers), scored != 0.
+  int32_t scored;
+  int32_t window;               // keys at distance >= window are hidden; 0: none
+  float softcap;                // 0: none; c * tanh(s / c)
+  float softcap_log2, inv_softcap_log2;  // the cap and its inverse in the log2 domain
+  const float* alibi_slopes;    // [Hq] or null
+  const int32_t* key_starts;    // first key of query token (b, t), or null
+  int64_t kst_sb, kst_st;
+  const int32_t* prefix_lens;   // [B] keys every token of the row sees, or null
 };
+
+// Keys query token t of a row of attended length L sees: [first, end), empty
+// when first >= end.  start: the token's key_starts entry (0 without), prefix:
+// the row's prefix_lens entry (0 without).
+struct KeyRange {
+  int first, end;
+};
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline KeyRange key_range(int L, int q_len, int t, int window, int start, int prefix) {
+  const int pos = L - q_len + t;
+  KeyRange r;
+  r.end = pos + 1;
+  const int shared = prefix < L ? prefix : L;
+  if (shared > r.end) r.end = shared;
+  if (pos < 0) r.end = 0;  // a token before the sequence's start
+  r.first = start > 0 ? start : 0;
+  if (window > 0 && pos - window + 1 > r.first) r.first = pos - window + 1;
+  return r;
+}
+
+// Arrays of the decode kernel's per-sequence shared-memory tables (ints).
+constexpr int decode_seq_tables(bool cascade, bool scored) { return scored ? 5 : cascade ? 4 : 3; }
 
 struct AppendParams {
   const void* key;
@@ -133,6 +171,45 @@ struct AppendParams {
   uint32_t* error_flags;
 };
 
+// Scales of an 8-bit cache that an append writes (strides in elements).
+struct ScaleParams {
+  float* k_scales;
+  float* v_scales;
+  int64_t ks_sblk, ks_sh, vs_sblk, vs_sh;
+};
+
+// Caches whose pages move together: byte strides; a page is `segments` runs of
+// segment_bytes, stride_segment apart.
+constexpr int kMaxPageViews = PA_MAX_PAGE_VIEWS;
+struct PageView {
+  void* data;
+  int64_t stride_block, segments, stride_segment, segment_bytes;
+};
+struct PageViews {
+  int32_t n;
+  PageView v[kMaxPageViews];
+};
+// A table of sequences (pa_page_tables).
+struct PageTables {
+  int32_t* tables;
+  int64_t stride;
+  int32_t num_seqs, max_blocks;
+  int32_t* lens;
+  int32_t* refs;
+  int32_t num_blocks, bs;
+  int32_t* scratch;
+  uint32_t* flags;
+};
+cudaError_t launch_pages_copy(const PageViews& pv, const int32_t* src, const int32_t* dst, int n, int num_blocks,
+                              int num_sms, uint32_t* flags, cudaStream_t stream);
+cudaError_t launch_pages_free(const PageTables& t, const int32_t* slots, int n, cudaStream_t stream);
+cudaError_t launch_pages_fork(const PageTables& t, const int32_t* parents, const int32_t* children, int n,
+                              const PageViews& pv, cudaStream_t stream);
+cudaError_t launch_pages_reserve(const PageTables& t, const int32_t* slots, const int32_t* tokens, int n,
+                                 cudaStream_t stream);
+cudaError_t launch_pages_compact(const PageTables& t, const PageViews& pv, int32_t* live, int num_sms,
+                                 cudaStream_t stream);
+
 // Record the message pa_last_error() returns on this host thread; returns status.
 int set_last_error(int status, const char* msg);
 
@@ -142,12 +219,19 @@ size_t ws_partial_bytes(int nw_total, int slot_rows, int D);
 
 // Launchers (return cudaError_t of the launch).
 cudaError_t launch_kv_append(const AppendParams& p, cudaStream_t stream);
+// The append into an 8-bit cache; dtype: of the new rows (p.elem_bytes: theirs).
+// Blocks of a power of two of tokens up to 256, head_dim a multiple of 16, cache
+// rows 16-byte aligned.
+cudaError_t launch_kv_append8(const AppendParams& p, const ScaleParams& sc, int dtype, cudaStream_t stream);
 // Mode follows the params: cascade when seq_group is set, fused gather when
 // out_ranks is set, plain otherwise.
 cudaError_t launch_decode_mma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv,
                               int dtype, int grid, size_t smem, bool pdl, cudaStream_t stream);
 cudaError_t launch_decode_f32(const DecodeParams& p, bool pdl, cudaStream_t stream);
 cudaError_t launch_prefill_mma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
+                               bool pdl, cudaStream_t stream);
+// pa_decode_ext's form of the same kernel (8-bit cache and / or changed scores).
+cudaError_t launch_prefill_ext(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                bool pdl, cudaStream_t stream);
 cudaError_t launch_prefill_umma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                 bool pdl, cudaStream_t stream);
@@ -169,5 +253,9 @@ constexpr int kUmmaTileRows = 256;
 size_t decode_mma_smem_bytes(int D, int B, int stages, bool cascade);
 // Opt a kernel instantiation into large dynamic shared memory (once per device).
 cudaError_t decode_mma_prepare(int dtype, int D, size_t smem);
+// The same for pa_decode_ext's instantiations (8-bit cache and / or changed scores).
+size_t decode_ext_smem_bytes(int D, int B, int stages, bool eight, bool scored);
+cudaError_t launch_decode_ext(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
+                              int grid, size_t smem, bool pdl, cudaStream_t stream);
 
 }  // namespace pa

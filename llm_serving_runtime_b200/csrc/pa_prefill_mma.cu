@@ -10,20 +10,27 @@
 // 128 query rows instead of once per 16, and the tile stops at its latest
 // row's causal limit.  Tiles of the latest query tokens (the most work) are
 // scheduled first.  No split, so no partials: every warp stores its own rows.
+// KV and kScored: 8-bit caches and changed scores (pa_decode_ext, arithmetic in
+// pa_tile_ext.cuh); a tile then starts at its earliest row's first key.
+#include <limits.h>
 #include <math.h>
 
 #include "pa_common.cuh"
 #include "pa_internal.h"
+#include "pa_tile_ext.cuh"
 #include "pa_tile_math.cuh"
 
 namespace pa {
 
-template <typename T, int D>
+template <typename T, int D, typename KV = T, bool kScored = false>
 __global__ void __launch_bounds__(kPrefillThreads, 1)
     prefill_mma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                        const DecodeParams p) {
-  constexpr int HALVES = D / 64;
-  constexpr uint32_t TILE_BYTES = 16 * D * 2;
+  constexpr bool k8 = kIs8<KV>::value;
+  constexpr bool kExt = k8 || kScored;
+  using TL = TileLayout<KV, D>;
+  constexpr int HALVES = TL::kHalves;
+  constexpr uint32_t TILE_BYTES = TL::kTileBytes;
   constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
   constexpr int S = kPrefillStages;
 
@@ -33,6 +40,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const uint32_t ring = smem_addr(smem);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * STAGE_BYTES);
   uint64_t* empty = full + S;
+  __shared__ float4 s_scales[k8 ? S : 1];  // 8-bit: a slot's scales, K of tokens 0-7 and 8-15, V of the same
+  __shared__ int s_lo, s_hi;               // changed scores: keys that some row of the tile sees
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -57,11 +66,29 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int rows_tile = min(128, p.GQ - row0);
   const int active = (rows_tile + 15) / 16;  // consumer warps that own rows
   const int lim_tile = L - p.q_len + (row0 + rows_tile - 1) / p.G;
-  const int n_units = lim_tile < 0 ? 0 : (lim_tile + kUnitTokens) / kUnitTokens;
+  int u_first = 0;  // the tile's first unit
+  int n_units = lim_tile < 0 ? 0 : (lim_tile + kUnitTokens) / kUnitTokens;
+  if constexpr (kScored) {
+    if (tid == 0) {
+      s_lo = INT_MAX;
+      s_hi = 0;
+    }
+    __syncthreads();
+    if (tid < rows_tile) {
+      const KeyRange kr = row_keys<kScored>(p, b, L, (row0 + tid) / p.G);
+      if (kr.first < kr.end) {
+        atomicMin(&s_lo, kr.first);
+        atomicMax(&s_hi, kr.end);
+      }
+    }
+    __syncthreads();
+    u_first = min(s_lo, s_hi) / kUnitTokens;
+    n_units = s_lo < s_hi ? (s_hi + kUnitTokens - 1) / kUnitTokens - u_first : 0;
+  }
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(smem_addr(&full[s]), 1);
+      mbar_init(smem_addr(&full[s]), k8 ? 2 : 1);
       mbar_init(smem_addr(&empty[s]), active);
     }
     prefetch_tensormap(&tmk);
@@ -87,7 +114,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           return;
         }
       }
-      const int tok0 = u * kUnitTokens;
+      const int tok0 = (u_first + u) * kUnitTokens;
       const int lb0 = tok0 / bs;
       const int need = bs >= kUnitTokens ? 1 : kUnitTokens / bs;
       if (win_base < 0 || lb0 < win_base || lb0 + need > win_base + 32) {
@@ -102,18 +129,33 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const uint32_t stage = ring + (uint32_t)slot * STAGE_BYTES;
       const uint32_t bar = smem_addr(&full[slot]);
       const bool need1 = bs < kUnitTokens && (lb0 + 1) * bs < L;
-      const uint32_t box_bytes = bs >= kUnitTokens ? 2048u : (uint32_t)bs * 128u;
-      const int nbox = (need1 ? 2 : 1) * HALVES * 2;
+      // changed scores: nor is a first block that ends before the tile's first key
+      bool need0 = true;
+      if constexpr (kScored) need0 = bs >= kUnitTokens || (lb0 + 1) * bs > s_lo;
+      const uint32_t box_bytes = bs >= kUnitTokens ? TL::kHalfBytes : (uint32_t)bs * TL::kRowBytes;
+      const int nbox = ((need0 ? 1 : 0) + (need1 ? 1 : 0)) * HALVES * 2;
       if (lane == 0) {
-        if (phys0 < 0 || phys0 >= p.num_blocks || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
+        if ((need0 && (phys0 < 0 || phys0 >= p.num_blocks)) || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
           raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
         mbar_arrive_expect_tx(bar, (uint32_t)nbox * box_bytes);
+        if constexpr (k8) {
+          const uint32_t dst = smem_addr(&s_scales[slot]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int phys = bs >= kUnitTokens ? phys0 : j ? (need1 ? phys1 : -1) : (need0 ? phys0 : -1);
+            const bool ok = phys >= 0 && phys < p.num_blocks;
+            const long long blk = ok ? phys : 0;
+            cp_async_4_zfill(dst + 4u * j, p.k_scales + blk * p.ks_sblk + h * p.ks_sh, ok ? 4u : 0u);
+            cp_async_4_zfill(dst + 8u + 4u * j, p.v_scales + blk * p.vs_sblk + h * p.vs_sh, ok ? 4u : 0u);
+          }
+          cp_async_mbar_arrive_noinc(bar);
+        }
       }
       __syncwarp();
       if (lane < nbox) {  // lane -> (block j, K or V, half)
-        const int j = lane / (2 * HALVES), kv = (lane / HALVES) & 1, hf = lane % HALVES;
+        const int j = lane / (2 * HALVES) + (need0 ? 0 : 1), kv = (lane / HALVES) & 1, hf = lane % HALVES;
         const int y = bs >= kUnitTokens ? tok0 - lb0 * bs : 0;
-        tma_load_4d(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * 2048u + (uint32_t)j * box_bytes,
+        tma_load_4d(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * TL::kHalfBytes + (uint32_t)j * box_bytes,
                     kv ? &tmv : &tmk, bar, hf * 64, y, h, j ? phys1 : phys0);
       }
       __syncwarp();
@@ -152,7 +194,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int mask_from = L - p.q_len + (row0 + warp * 16) / p.G;
 
   uint32_t qa[D / 16][4];
-  load_query_frags<T, D>(qa, qp0, qp1, quad, p.Dv);
+  [[maybe_unused]] RowState st;
+  [[maybe_unused]] int tok_lo = INT_MAX, tok_hi = 0, full_lo = 0, full_hi = INT_MAX;
+  if constexpr (k8) {
+    float qinv[2];
+    load_query_frags_8<T, D>(qa, qp0, qp1, quad, p.Dv, qinv);
+    st.c[0] = p.scale_log2 * qinv[0];
+    st.c[1] = p.scale_log2 * qinv[1];
+  } else {
+    load_query_frags<T, D>(qa, qp0, qp1, quad, p.Dv);
+    st.c[0] = st.c[1] = p.scale_log2;
+  }
+  if constexpr (kExt) init_rows<kScored>(st, p, b, h, L, qr0, tok_lo, tok_hi, full_lo, full_hi);
   float o_acc[D / 8][4];
 #pragma unroll
   for (int nd = 0; nd < D / 8; ++nd) o_acc[nd][0] = o_acc[nd][1] = o_acc[nd][2] = o_acc[nd][3] = 0.f;
@@ -165,8 +218,19 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       if (lane == 0) raise_flag(p.status, PA_DEVERR_WAIT_TIMEOUT);
       return;  // the producer's own bounded waits end it
     }
-    if (u < n_w) {
-      const uint32_t kbase = ring + (uint32_t)slot * STAGE_BYTES;
+    const uint32_t kbase = ring + (uint32_t)slot * STAGE_BYTES;
+    if constexpr (kExt) {
+      const int tok0 = (u_first + u) * kUnitTokens;
+      if (tok0 < tok_hi && tok0 + kUnitTokens > tok_lo) {  // some row of the warp sees some key of the unit
+        float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+        if constexpr (k8) {
+          const float4 sc = s_scales[slot];
+          ks[0] = sc.x, ks[1] = sc.y, vs[0] = sc.z, vs[1] = sc.w;
+        }
+        attend_unit_ext<T, KV, D, kScored>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo,
+                                           full_hi, ks, vs, p, lane);
+      }
+    } else if (u < n_w) {
       attend_unit<T, D>(kbase, kbase + TILE_BYTES, qa, o_acc, m0, m1, l0, l1, u * kUnitTokens, L, lim0, lim1,
                         mask_from, p.scale_log2, lane);
     }
@@ -174,18 +238,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     if (lane == 0) mbar_arrive(smem_addr(&empty[slot]));
   }
 
+  if constexpr (kExt) l0 = st.l[0], l1 = st.l[1];
+  if constexpr (k8) end_piece_columns<D>(o_acc, st);
   float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
   float lt1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
   lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
   lt1 += __shfl_xor_sync(0xffffffffu, lt1, 2);
-  store_rows<T, D>(op0, op1, o_acc, lt0, lt1, quad, p.Dv);
+  if constexpr (kExt)
+    store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm(lt0, st.first[0] < st.end[0]),
+                             row_norm(lt1, st.first[1] < st.end[1]), quad, p.Dv);
+  else
+    store_rows<T, D>(op0, op1, o_acc, lt0, lt1, quad, p.Dv);
 }
 
 size_t prefill_smem_bytes(int D) {
   return 1024 + (size_t)kPrefillStages * (2u * 16u * (size_t)D * 2u) + 2 * kPrefillStages * 8;
 }
 
-template <typename T, int D>
+template <typename T, int D, typename KV = T, bool kScored = false>
 static cudaError_t launch_prefill_impl(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv,
                                        bool pdl, cudaStream_t stream) {
   const size_t smem = prefill_smem_bytes(D);
@@ -193,7 +263,7 @@ static cudaError_t launch_prefill_impl(const DecodeParams& p, const CUtensorMap&
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !prepared[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_mma_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(prefill_mma_kernel<T, D, KV, kScored>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
     prepared[dev] = true;
@@ -208,7 +278,7 @@ static cudaError_t launch_prefill_impl(const DecodeParams& p, const CUtensorMap&
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl ? attr : nullptr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, prefill_mma_kernel<T, D>, tmk, tmv, p);
+  return cudaLaunchKernelEx(&cfg, prefill_mma_kernel<T, D, KV, kScored>, tmk, tmv, p);
 }
 
 cudaError_t launch_prefill_mma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
@@ -221,6 +291,23 @@ cudaError_t launch_prefill_mma(const DecodeParams& p, const CUtensorMap& tmk, co
     if (p.D == 64) return launch_prefill_impl<__half, 64>(p, tmk, tmv, pdl, stream);
   }
   return cudaErrorInvalidValue;
+}
+
+template <typename T, int D>
+static cudaError_t pick_prefill_ext(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, bool pdl,
+                                    cudaStream_t stream) {
+  if (p.k_scales == nullptr) return launch_prefill_impl<T, D, T, true>(p, tmk, tmv, pdl, stream);
+  if (p.scored) return launch_prefill_impl<T, D, e4m3_t, true>(p, tmk, tmv, pdl, stream);
+  return launch_prefill_impl<T, D, e4m3_t, false>(p, tmk, tmv, pdl, stream);
+}
+
+cudaError_t launch_prefill_ext(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
+                               bool pdl, cudaStream_t stream) {
+  if (dtype == PA_DTYPE_BFLOAT16)
+    return p.D == 128 ? pick_prefill_ext<__nv_bfloat16, 128>(p, tmk, tmv, pdl, stream)
+                      : pick_prefill_ext<__nv_bfloat16, 64>(p, tmk, tmv, pdl, stream);
+  return p.D == 128 ? pick_prefill_ext<__half, 128>(p, tmk, tmv, pdl, stream)
+                    : pick_prefill_ext<__half, 64>(p, tmk, tmv, pdl, stream);
 }
 
 }  // namespace pa

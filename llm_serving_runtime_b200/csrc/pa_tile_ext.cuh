@@ -1,0 +1,504 @@
+// pa_tile_ext.cuh — one warp's attention over one 16-token unit for the two
+// extensions of the plain tile (pa_tile_math.cuh): caches held in 8 bits (e4m3
+// with one scale per block of tokens and KV head) and changed scores (tanh cap,
+// distance bias, sliding window, document starts, prefix mask).
+//
+// With x = log2(e) * s the score of a query at position i and a key at j, and
+// first <= j < end the keys the row sees:
+//   s = scale * (q . k_j),  capped c * tanh(s / c),  minus slope * |i - j|
+//   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m)
+//
+// 8-bit caches.  k_j = ks * c_j and v_j = vs * d_j with codes c, d and the
+// block's scales ks, vs.  Codes widen to fp16 without rounding, so both products
+// run as fp16 MMAs whatever the query's type; ks multiplies the finished dot
+// product.  A bf16 query row is brought to fp16 by a power of two of its own
+// that puts its largest element into [2^14, 2^15): 8-bit significands fit
+// fp16's 11, and only elements 2^29 below the row's largest lose bits.
+// vs goes into the weights: the accumulator's reference is
+//   mo = max_j (x_j + log2 vs_j),  weights w_j = 2^(x_j + log2 vs_j - mo + 14)
+// apart from the sum's reference m = max_j x_j, so a block of large scale and no
+// weight cannot push the others' weights out of fp16's range.  w is rounded to
+// fp16 (11 bits, at most 2^-11 of each weight), normal down to 2^-28 of the
+// largest.  At the end of a piece the accumulator returns to the reference m.
+//
+// What a mask hides never reaches a row: hidden scores are -inf whatever K
+// holds, and where rows of one tile see different keys, tokens whose V row is
+// not finite are taken out of the MMA (0 * inf) and added row by row.
+#pragma once
+
+#include <limits.h>
+
+#include "pa_common.cuh"
+#include "pa_internal.h"
+#include "pa_tile_math.cuh"
+
+namespace pa {
+
+// Cache element of 8-bit caches (an e4m3 code).
+struct e4m3_t {
+  uint8_t bits;
+};
+
+template <typename C>
+struct kIs8 {
+  static constexpr bool value = sizeof(C) == 1;
+};
+
+// Element type of the P V product.
+template <typename T, typename C>
+struct PvType {
+  using type = T;
+};
+template <typename T>
+struct PvType<T, e4m3_t> {
+  using type = __half;
+};
+
+// Two e4m3 codes (bits 0-7, 8-15) to two fp16 values, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+  uint32_t d;
+  const unsigned short h = (unsigned short)two;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(h));
+  return d;
+}
+
+// log2 (approximate instruction; exact powers of two come out as integers).
+__device__ __forceinline__ float lg2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Element layout of a unit's tile in shared memory.  16-bit: 64-element column
+// halves of 16 rows x 128 bytes, 128-byte swizzle.  8-bit: 16 rows of D bytes,
+// swizzled over 128 bytes (D = 128) or 64 bytes (D = 64).
+template <typename C, int D>
+struct TileLayout {
+  static constexpr bool k8 = kIs8<C>::value;
+  static constexpr int kHalves = k8 ? 1 : D / 64;           // TMA boxes across a row
+  static constexpr int kBoxElems = k8 ? D : 64;             // elements of a box row
+  static constexpr uint32_t kRowBytes = k8 ? D : 128;       // bytes of a box row
+  static constexpr uint32_t kHalfBytes = 16 * kRowBytes;    // one box of 16 tokens
+  static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
+};
+
+// Byte address of 16-byte chunk `chunk` of row `tok` in a tile at `base`.
+template <typename C, int D>
+__device__ __forceinline__ uint32_t tile_chunk_addr(uint32_t base, int tok, int chunk) {
+  using L = TileLayout<C, D>;
+  if constexpr (L::kRowBytes == 128)
+    return base + (uint32_t)(chunk >> 3) * L::kHalfBytes + (uint32_t)tok * 128u +
+           ((uint32_t)((chunk & 7) ^ (tok & 7)) << 4);
+  else
+    return base + (uint32_t)tok * 64u + ((uint32_t)(chunk ^ ((tok >> 1) & 3)) << 4);
+}
+
+// Output column of accumulator element (nd, 0) of a lane (element 1 is the next
+// column) once a piece has ended.  8-bit tiles come out of the byte transpose
+// with even and odd columns in separate n-tiles; end_piece_columns() pairs them.
+template <typename C>
+__device__ __forceinline__ int frag_col(int nd, int quad) {
+  if constexpr (kIs8<C>::value)
+    return (nd >> 1) * 16 + 4 * quad + 2 * (nd & 1);
+  else
+    return nd * 8 + 2 * quad;
+}
+
+// Running state of a warp's rows lane/4 (index 0) and lane/4 + 8 (index 1).
+struct RowState {
+  float m[2], l[2];    // max and sum of 2^(x - m)
+  float mo[2];         // 8-bit: max of x + log2 vs
+  float c[2];          // dot product -> x (scale * log2 e, and the query row's power of two)
+  int first[2], end[2];  // keys the row sees
+  float slope[2];      // distance bias, log2 domain
+  int pos[2];          // the row's own position
+};
+
+// Keys that query token t of sequence b (attended length L) sees.
+template <bool kScored>
+__device__ __forceinline__ KeyRange row_keys(const DecodeParams& p, int b, int L, int t) {
+  if constexpr (kScored) {
+    const int start = p.key_starts != nullptr ? __ldg(&p.key_starts[b * p.kst_sb + t * p.kst_st]) : 0;
+    const int prefix = p.prefix_lens != nullptr ? __ldg(&p.prefix_lens[b]) : 0;
+    return key_range(L, p.q_len, t, p.window, start, prefix);
+  }
+  return key_range(L, p.q_len, t, 0, 0, 0);
+}
+
+// Fresh state of rows qr0 and qr0 + 8 of KV head h (st.c is the caller's), and of
+// the tile's 16 rows: keys that some row sees lie in [tok_lo, tok_hi), keys in
+// [full_lo, full_hi) are seen by every row.
+template <bool kScored>
+__device__ __forceinline__ void init_rows(RowState& st, const DecodeParams& p, int b, int h, int L, int qr0,
+                                          int& tok_lo, int& tok_hi, int& full_lo, int& full_hi) {
+  tok_lo = full_hi = INT_MAX;
+  tok_hi = full_lo = 0;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    const int qr = qr0 + 8 * r;
+    st.m[r] = st.mo[r] = -INFINITY;
+    st.l[r] = 0.f;
+    st.first[r] = 0;  // rows past the group's last see everything and are not stored
+    st.end[r] = INT_MAX;
+    st.slope[r] = 0.f;
+    st.pos[r] = 0;
+    if (qr < p.GQ) {
+      const int t = qr / p.G, g = qr - t * p.G;
+      const KeyRange kr = row_keys<kScored>(p, b, L, t);
+      if (kScored && p.alibi_slopes != nullptr)
+        st.slope[r] = __ldg(&p.alibi_slopes[h * p.G + g]) * 1.4426950408889634f;
+      st.first[r] = kr.first;
+      st.end[r] = kr.end;
+      st.pos[r] = L - p.q_len + t;
+      tok_lo = min(tok_lo, kr.first);
+      tok_hi = max(tok_hi, kr.end);
+      full_lo = max(full_lo, kr.first);
+      full_hi = min(full_hi, kr.end);
+    }
+  }
+  tok_lo = __reduce_min_sync(0xffffffffu, tok_lo);
+  tok_hi = __reduce_max_sync(0xffffffffu, tok_hi);
+  full_lo = __reduce_max_sync(0xffffffffu, full_lo);
+  full_hi = __reduce_min_sync(0xffffffffu, full_hi);
+}
+
+// Query fragments of an 8-bit tile: k-step ks holds columns 16 ks + 4 quad, +1
+// (registers 0, 1) and +2, +3 (registers 2, 3), the order in which ldmatrix
+// hands out four neighbouring codes.  qinv: what takes the rows' own powers of
+// two back out of their dot products.
+template <typename T, int D>
+__device__ __forceinline__ void load_query_frags_8(uint32_t (&qa)[D / 16][4], const T* qp0, const T* qp1, int quad,
+                                                   int Dv, float (&qinv)[2]) {
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const int d = ks * 16 + 4 * quad;
+    const bool in = d < Dv;  // Dv is a multiple of 16
+    qa[ks][0] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d)) : 0u;
+    qa[ks][1] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d)) : 0u;
+    qa[ks][2] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d + 2)) : 0u;
+    qa[ks][3] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d + 2)) : 0u;
+  }
+  qinv[0] = qinv[1] = 1.f;
+  if constexpr (sizeof(T) == 2 && !kSplitProbabilities<T>::value) return;  // fp16 already
+  float mx[2] = {0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      mx[i & 1] = fmaxf(mx[i & 1], fmaxf(fabsf(lo_half<T>(qa[ks][i])), fabsf(hi_half<T>(qa[ks][i]))));
+  float mul[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+    const int e = (int)(__float_as_uint(mx[r]) >> 23);  // biased exponent: mx in [2^(e-127), 2^(e-126))
+    // 2^(14 + 127 - e), within what fp32 holds; rows of 0 or with an infinity stay as they are
+    const int k = (e == 0 || e == 255) ? 0 : min(max(14 + 127 - e, -120), 100);
+    mul[r] = __uint_as_float((uint32_t)(127 + k) << 23);
+    qinv[r] = __uint_as_float((uint32_t)(127 - k) << 23);
+  }
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      qa[ks][i] = pack2<__half>(lo_half<T>(qa[ks][i]) * mul[i & 1], hi_half<T>(qa[ks][i]) * mul[i & 1]);
+}
+
+// c * tanh(x / c) in the log2 domain (cap, inv_cap = 1 / cap, both of it).
+// tanh y = 1 - 2 / (1 + e^2y) loses its low bits near 0, where the odd Taylor
+// series y - y^3/3 + 2y^5/15 - 17y^7/315 takes over (at |y| <= 0.25 its first
+// left-out term, 62y^9/2835, is 3.4e-7 of y).
+__device__ __forceinline__ float softcap_log2(float x, float cap, float inv_cap) {
+  const float y = x * inv_cap;
+  const float e = ex2(y * 2.8853900817779268f);
+  const float big = 1.f - __fdividef(2.f, 1.f + fminf(e, 1e30f));
+  const float y2 = y * y;
+  const float p = fmaf(y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
+  // NaN fails the comparison and comes out of the series' argument
+  return fabsf(y) > 0.25f ? cap * big : x * p;
+}
+
+// One unit.  ks / vs: the scales of tokens 0-7 and 8-15 (8-bit caches).
+// tok_base: position of the unit's first token; tokens before tok_lo or at or
+// past tok_hi are seen by no row of the tile (their V may be anything); units
+// outside [full_lo, full_hi) hold keys that some row does not see.
+template <typename T, typename C, int D, bool kScored>
+__device__ __forceinline__ void attend_unit_ext(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
+                                                float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
+                                                int tok_hi, int full_lo, int full_hi, const float (&ks)[2],
+                                                const float (&vs)[2], const DecodeParams& p, int lane) {
+  constexpr bool k8 = kIs8<C>::value;
+  constexpr int NDT = D / 8;
+  const int quad = lane & 3;
+
+  // ---- S = Q K^T ----
+  float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+  if constexpr (k8) {
+    const int tok = ((lane >> 4) << 3) | (lane & 7);
+#pragma unroll
+    for (int kp = 0; kp < D / 32; ++kp) {
+      uint32_t r0, r1, r2, r3;  // tokens 0-7: k-steps 2kp, 2kp+1; tokens 8-15: the same
+      ldsm_x4(tile_chunk_addr<C, D>(kbase, tok, 2 * kp + ((lane >> 3) & 1)), r0, r1, r2, r3);
+      Mma16816<__half>::run(x[0], qa[2 * kp], e4m3x2_to_f16x2(r0), e4m3x2_to_f16x2(r0 >> 16));
+      Mma16816<__half>::run(x[1], qa[2 * kp], e4m3x2_to_f16x2(r2), e4m3x2_to_f16x2(r2 >> 16));
+      Mma16816<__half>::run(x[0], qa[2 * kp + 1], e4m3x2_to_f16x2(r1), e4m3x2_to_f16x2(r1 >> 16));
+      Mma16816<__half>::run(x[1], qa[2 * kp + 1], e4m3x2_to_f16x2(r3), e4m3x2_to_f16x2(r3 >> 16));
+    }
+  } else {
+    const int tok = ((lane >> 4) << 3) | (lane & 7);
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t r0, r1, r2, r3;
+      ldsm_x4(tile_chunk_addr<C, D>(kbase, tok, 2 * kk + ((lane >> 3) & 1)), r0, r1, r2, r3);
+      Mma16816<T>::run(x[0], qa[kk], r0, r1);
+      Mma16816<T>::run(x[1], qa[kk], r2, r3);
+    }
+  }
+
+  // ---- scores in the log2 domain ----
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const float c0 = k8 ? st.c[0] * ks[n] : st.c[0], c1 = k8 ? st.c[1] * ks[n] : st.c[1];
+    x[n][0] *= c0;
+    x[n][1] *= c0;
+    x[n][2] *= c1;
+    x[n][3] *= c1;
+  }
+  if constexpr (kScored) {
+    if (p.softcap_log2 > 0.f) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = softcap_log2(x[n][i], p.softcap_log2, p.inv_softcap_log2);
+    }
+    if (p.alibi_slopes != nullptr) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+          x[n][i] = fmaf(-st.slope[i >> 1], fabsf((float)(st.pos[i >> 1] - tok)), x[n][i]);
+        }
+    }
+  }
+  const bool boundary = tok_base < full_lo || tok_base + kUnitTokens > full_hi;
+  uint32_t odd_tokens = 0;  // tokens of a boundary unit whose V row is not finite
+  if (boundary) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+        if (tok < st.first[i >> 1] || tok >= st.end[i >> 1]) x[n][i] = -INFINITY;
+      }
+    // lane pair 2t, 2t+1 looks over V row t
+    const int t = lane >> 1;
+    bool odd = false;
+    constexpr int CH = D * (int)sizeof(C) / 16;  // 16-byte chunks of a row
+#pragma unroll
+    for (int ch = 0; ch < CH / 2; ++ch) {
+      uint32_t w0, w1, w2, w3;
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3)
+                   : "r"(tile_chunk_addr<C, D>(vbase, t, 2 * ch + (lane & 1))));
+      const uint32_t w[4] = {w0, w1, w2, w3};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (k8) {
+          odd |= __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
+        } else {
+          const uint32_t em = kSplitProbabilities<T>::value ? 0x7f80u : 0x7c00u;
+          odd |= (w[j] & em) == em || (w[j] & (em << 16)) == (em << 16);
+        }
+      }
+    }
+    const uint32_t pairs = __ballot_sync(0xffffffffu, odd && tok_base + t >= tok_lo && tok_base + t < tok_hi);
+    const uint32_t either = pairs | (pairs >> 1);  // bit 2t: token t
+    if (either & 0x55555555u) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) odd_tokens |= ((either >> (2 * j)) & 1u) << j;
+    }
+  }
+
+  // ---- online softmax ----
+  float alpha[2], w[2][4];
+  const float lvs[2] = {k8 ? lg2(vs[0]) : 0.f, k8 ? lg2(vs[1]) : 0.f};
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float mx[2];  // of tokens 0-7 and 8-15
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      mx[n] = fmaxf(x[n][2 * r], x[n][2 * r + 1]);
+      mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 1));
+      mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 2));
+    }
+    const float mn = fmaxf(st.m[r], fmaxf(mx[0], mx[1]));
+    const float base = mn == -INFINITY ? 0.f : mn;
+    const float a = ex2(st.m[r] - base);
+    float pr[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pr[i] = ex2(x[i >> 1][2 * r + (i & 1)] - base);
+    st.l[r] = st.l[r] * a + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
+    st.m[r] = mn;
+    if constexpr (k8) {
+      const float on = fmaxf(st.mo[r], fmaxf(mx[0] + lvs[0], mx[1] + lvs[1]));
+      const float obase = (on == -INFINITY ? 0.f : on) - 14.f;
+      alpha[r] = ex2(st.mo[r] - 14.f - obase);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float xi = x[i >> 1][2 * r + (i & 1)];
+        // a hidden score stays without weight even beside a scale that is not finite
+        w[r][i] = xi == -INFINITY ? 0.f : ex2(xi + (lvs[i >> 1] - obase));
+      }
+      st.mo[r] = on;
+    } else {
+      alpha[r] = a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[r][i] = pr[i];
+    }
+  }
+  if (__any_sync(0xffffffffu, (alpha[0] != 1.f) | (alpha[1] != 1.f))) {
+#pragma unroll
+    for (int nd = 0; nd < NDT; ++nd) {
+      o_acc[nd][0] *= alpha[0];
+      o_acc[nd][1] *= alpha[0];
+      o_acc[nd][2] *= alpha[1];
+      o_acc[nd][3] *= alpha[1];
+    }
+  }
+
+  // ---- O += P V ----
+  using P = typename PvType<T, C>::type;
+  uint32_t pa[4] = {pack2<P>(w[0][0], w[0][1]), pack2<P>(w[1][0], w[1][1]), pack2<P>(w[0][2], w[0][3]),
+                    pack2<P>(w[1][2], w[1][3])};
+  constexpr bool kSplitP = !k8 && kSplitProbabilities<T>::value;
+  uint32_t plo[4] = {0u, 0u, 0u, 0u};
+  if constexpr (kSplitP) {
+    plo[0] = pack2<P>(w[0][0] - lo_half<P>(pa[0]), w[0][1] - hi_half<P>(pa[0]));
+    plo[1] = pack2<P>(w[1][0] - lo_half<P>(pa[1]), w[1][1] - hi_half<P>(pa[1]));
+    plo[2] = pack2<P>(w[0][2] - lo_half<P>(pa[2]), w[0][3] - hi_half<P>(pa[2]));
+    plo[3] = pack2<P>(w[1][2] - lo_half<P>(pa[3]), w[1][3] - hi_half<P>(pa[3]));
+  }
+  uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
+  if (boundary) {
+    uint32_t keep = 0;  // this lane's tokens 2 quad, +1, +8, +9
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = 2 * quad + (j & 1) + 8 * (j >> 1);
+      const bool k = tok_base + t >= tok_lo && tok_base + t < tok_hi && !((odd_tokens >> t) & 1u);
+      keep |= (uint32_t)k << j;
+    }
+    vm0 = ((keep & 1u) ? 0x0000ffffu : 0u) | ((keep & 2u) ? 0xffff0000u : 0u);
+    vm1 = ((keep & 4u) ? 0x0000ffffu : 0u) | ((keep & 8u) ? 0xffff0000u : 0u);
+  }
+  const int tok = (((lane >> 3) & 1) << 3) | (lane & 7);
+  if constexpr (k8) {
+#pragma unroll
+    for (int c = 0; c < D / 16; c += 2) {
+      uint32_t r0, r1, r2, r3;  // chunk c: tokens 0-7, 8-15; chunk c + 1: the same
+      ldsm_x4_trans(tile_chunk_addr<C, D>(vbase, tok, c + (lane >> 4)), r0, r1, r2, r3);
+      const uint32_t r[4] = {r0, r1, r2, r3};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // bytes (token 2q: even, odd column; token 2q+1: even, odd) -> (even, even, odd, odd)
+        const uint32_t a = __byte_perm(r[2 * j], 0u, 0x3120), b = __byte_perm(r[2 * j + 1], 0u, 0x3120);
+        Mma16816<__half>::run(o_acc[2 * (c + j)], pa, e4m3x2_to_f16x2(a) & vm0, e4m3x2_to_f16x2(b) & vm1);
+        Mma16816<__half>::run(o_acc[2 * (c + j) + 1], pa, e4m3x2_to_f16x2(a >> 16) & vm0,
+                              e4m3x2_to_f16x2(b >> 16) & vm1);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int nd = 0; nd < NDT; nd += 2) {
+      uint32_t v0, v1, v2, v3;
+      ldsm_x4_trans(tile_chunk_addr<C, D>(vbase, tok, nd + (lane >> 4)), v0, v1, v2, v3);
+      v0 &= vm0;
+      v1 &= vm1;
+      v2 &= vm0;
+      v3 &= vm1;
+      Mma16816<T>::run(o_acc[nd], pa, v0, v1);
+      Mma16816<T>::run(o_acc[nd + 1], pa, v2, v3);
+      if constexpr (kSplitP) {
+        Mma16816<T>::run(o_acc[nd], plo, v0, v1);
+        Mma16816<T>::run(o_acc[nd + 1], plo, v2, v3);
+      }
+    }
+  }
+  // Tokens taken out above, for the rows that see them (rare: one is not finite).
+  while (odd_tokens) {
+    const int t = __ffs(odd_tokens) - 1;
+    odd_tokens &= odd_tokens - 1;
+    const int src = (lane & ~3) | ((t & 7) >> 1);  // the quad lane that holds column t
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float lo = (t >> 3) ? w[r][2] : w[r][0], hi = (t >> 3) ? w[r][3] : w[r][1];
+      const float wt = __shfl_sync(0xffffffffu, (t & 1) ? hi : lo, src);
+      if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
+#pragma unroll
+      for (int nd = 0; nd < NDT; ++nd)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // column of element (nd, j) before end_piece_columns()
+          const int col = k8 ? (nd >> 1) * 16 + 4 * quad + 2 * j + (nd & 1) : nd * 8 + 2 * quad + j;
+          const uint32_t addr = tile_chunk_addr<C, D>(vbase, t, col * (int)sizeof(C) / 16) +
+                                (uint32_t)(col * (int)sizeof(C) % 16);
+          float v;
+          if constexpr (k8) {
+            uint32_t code;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(addr));
+            v = lo_half<__half>(e4m3x2_to_f16x2(code));
+          } else {
+            unsigned short h;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr));
+            v = lo_half<T>((uint32_t)h);
+          }
+          o_acc[nd][2 * r + j] = fmaf(wt, v, o_acc[nd][2 * r + j]);
+        }
+    }
+  }
+}
+
+// End of a piece of an 8-bit row: the accumulator back to the reference m, and
+// its columns in the order of frag_col().
+template <int D>
+__device__ __forceinline__ void end_piece_columns(float (&o_acc)[D / 8][4], const RowState& st) {
+  float f[2];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) f[r] = st.mo[r] == -INFINITY ? 0.f : ex2(st.mo[r] - 14.f - st.m[r]);
+#pragma unroll
+  for (int nd = 0; nd < D / 8; ++nd) {
+    o_acc[nd][0] *= f[0];
+    o_acc[nd][1] *= f[0];
+    o_acc[nd][2] *= f[1];
+    o_acc[nd][3] *= f[1];
+  }
+#pragma unroll
+  for (int nd = 0; nd < D / 8; nd += 2)
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      const float t = o_acc[nd][r + 1];  // column 4q + 2; the odd tile holds 4q + 1, 4q + 3
+      o_acc[nd][r + 1] = o_acc[nd + 1][r];
+      o_acc[nd + 1][r] = t;
+    }
+}
+
+// 1 / l of a finished row.  A row without weight is zero when it sees no key, and
+// NaN (0 / 0) when all its scores are -inf; so is one whose sum is NaN.
+__device__ __forceinline__ float row_norm(float l, bool sees_a_key) {
+  return l > 0.f ? 1.f / l : (l == 0.f && !sees_a_key) ? 0.f : __int_as_float(0x7fffffff);
+}
+
+// store_rows with the norms inv0 / inv1 and the columns of frag_col<KV>().
+template <typename T, typename KV, int D>
+__device__ __forceinline__ void store_rows_ext(T* op0, T* op1, const float (&o_acc)[D / 8][4], float inv0, float inv1,
+                                               int quad, int Dv) {
+#pragma unroll
+  for (int nd = 0; nd < D / 8; ++nd) {
+    const int d = frag_col<KV>(nd, quad);
+    if (d >= Dv) break;
+    if (op0) *reinterpret_cast<uint32_t*>(op0 + d) = pack2<T>(o_acc[nd][0] * inv0, o_acc[nd][1] * inv0);
+    if (op1) *reinterpret_cast<uint32_t*>(op1 + d) = pack2<T>(o_acc[nd][2] * inv1, o_acc[nd][3] * inv1);
+  }
+}
+
+}  // namespace pa

@@ -19,7 +19,7 @@ from __future__ import annotations
 
 import torch
 
-from .paged_attention import paged_attention_decode
+from .paged_attention import CACHE_8BIT, paged_attention_decode
 
 __all__ = ["DecodeStepGraph", "bucket_max_blocks"]
 
@@ -34,7 +34,12 @@ def bucket_max_blocks(max_blocks: int) -> int:
 
 class DecodeStepGraph:
     def __init__(self, key_caches, value_caches, *, batch: int, max_blocks: int, num_q_heads: int,
-                 q_len: int = 1, scale: float, warmup: int = 1, prefix_groups=None):
+                 q_len: int = 1, scale: float, warmup: int = 1, prefix_groups=None, key_scales=None,
+                 value_scales=None, score_modifiers=None, dtype: torch.dtype | None = None):
+        """``key_scales`` / ``value_scales``: one tensor per layer, for 8-bit caches, whose
+        ``dtype`` (of query, new rows and output) has to be given (fp16 or bf16).
+        ``score_modifiers``: a ScoreModifiers for every layer, or one per layer; their
+        tensors are read at replay."""
         if len(key_caches) != len(value_caches) or not key_caches:
             raise ValueError("one key and one value cache view per layer")
         kc0 = key_caches[0]
@@ -42,8 +47,23 @@ class DecodeStepGraph:
         self.key_caches = list(key_caches)
         self.value_caches = list(value_caches)
         _, Hkv, _, D = kc0.shape
-        dt = kc0.dtype
         L = len(key_caches)
+        if kc0.dtype == CACHE_8BIT:
+            if key_scales is None or value_scales is None or len(key_scales) != L or len(value_scales) != L:
+                raise ValueError("8-bit caches need one key_scales and one value_scales tensor per layer")
+            if dtype is None:
+                raise ValueError("8-bit caches need the dtype of query and output (fp16 or bf16)")
+        elif dtype is not None and dtype != kc0.dtype:
+            raise ValueError(f"dtype {dtype} differs from the caches' {kc0.dtype}")
+        elif key_scales is not None or value_scales is not None:
+            raise ValueError("key_scales and value_scales belong to 8-bit caches")
+        dt = dtype or kc0.dtype
+        self.key_scales = list(key_scales) if key_scales is not None else [None] * L
+        self.value_scales = list(value_scales) if value_scales is not None else [None] * L
+        self.score_modifiers = (list(score_modifiers) if isinstance(score_modifiers, (list, tuple))
+                                else [score_modifiers] * L)
+        if len(self.score_modifiers) != L:
+            raise ValueError("one score_modifiers for all layers, or one per layer")
         self.scale = float(scale)
         # shared-prefix groups (cascade); their tensors are read at replay, so
         # they may be rewritten in place between steps (same host bounds)
@@ -70,7 +90,8 @@ class DecodeStepGraph:
             paged_attention_decode(
                 self.query[layer], self.key_caches[layer], self.value_caches[layer], self.block_tables,
                 self.context_lens, self.scale, self.slot_mapping, self.new_key[layer], self.new_value[layer],
-                out=self.out[layer], prefix_groups=self.prefix_groups,
+                out=self.out[layer], prefix_groups=self.prefix_groups, key_scales=self.key_scales[layer],
+                value_scales=self.value_scales[layer], score_modifiers=self.score_modifiers[layer],
             )
 
     def replay(self) -> list[torch.Tensor]:

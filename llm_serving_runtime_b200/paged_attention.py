@@ -52,7 +52,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import CacheView, DecodeArgs, KvAppendArgs
+from ._lib import CacheScalesArgs, CacheView, DecodeArgs, KvAppendArgs
 
 __all__ = [
     "paged_attention_decode",
@@ -71,6 +71,8 @@ _DTYPE_CODE = {
     torch.float16: _lib.PA_DTYPE_FLOAT16,
     torch.bfloat16: _lib.PA_DTYPE_BFLOAT16,
 }
+# element type of caches held in 8 bits, with a scale for each block and KV head
+CACHE_8BIT = torch.float8_e4m3fn
 
 
 class DeviceErrorFlags:
@@ -80,16 +82,20 @@ class DeviceErrorFlags:
     WAIT_TIMEOUT = _lib.PA_DEVERR_WAIT_TIMEOUT
     PREFIX = _lib.PA_DEVERR_PREFIX
     GATHER = _lib.PA_DEVERR_GATHER
+    BLOCK_CONFLICT = _lib.PA_DEVERR_BLOCK_CONFLICT
+    SEQUENCE = _lib.PA_DEVERR_SEQUENCE
+    PAGES_EXHAUSTED = _lib.PA_DEVERR_PAGES_EXHAUSTED
 
 
 def device_error(flags: int) -> Exception:
     """The exception for a non-zero device error word: IndexError for invalid
     block ids, slots, underruns and prefix groups (the reference's error for
-    them); RuntimeError when only a bounded wait ran out or a fused gather fell
-    out of step."""
+    them), for blocks written twice in one call and bad sequence slots;
+    RuntimeError when only a bounded wait ran out, a fused gather fell out of
+    step or the free pages ran out."""
     text = describe_device_errors(flags)
     index_bits = (DeviceErrorFlags.BLOCK_ID_RANGE | DeviceErrorFlags.TABLE_UNDERRUN | DeviceErrorFlags.SLOT_RANGE
-                  | DeviceErrorFlags.PREFIX)
+                  | DeviceErrorFlags.PREFIX | DeviceErrorFlags.BLOCK_CONFLICT | DeviceErrorFlags.SEQUENCE)
     return IndexError(text) if flags & index_bits else RuntimeError(text)
 
 
@@ -107,6 +113,12 @@ def describe_device_errors(flags: int) -> str:
         parts.append("prefix group does not match its members' block tables or bounds")
     if flags & DeviceErrorFlags.GATHER:
         parts.append("fused gather ranks out of step (close() on every rank, then start again)")
+    if flags & DeviceErrorFlags.BLOCK_CONFLICT:
+        parts.append("one call writes a block from two places")
+    if flags & DeviceErrorFlags.SEQUENCE:
+        parts.append("sequence slot out of range, named twice, not empty, or in disagreement with the page counts")
+    if flags & DeviceErrorFlags.PAGES_EXHAUSTED:
+        parts.append("not enough free pages")
     return "; ".join(parts)
 
 
@@ -385,6 +397,29 @@ def _cache_view(t: torch.Tensor) -> CacheView:
     return CacheView(t.data_ptr(), t.shape[0], st[0], st[1], st[2])
 
 
+def _check_scales(scales: torch.Tensor, name: str, cache: torch.Tensor) -> None:
+    if tuple(scales.shape) != tuple(cache.shape[:2]):
+        raise ValueError(f"{name} must be [num_blocks={cache.shape[0]}, num_kv_heads={cache.shape[1]}], "
+                         f"got {tuple(scales.shape)}")
+    if scales.dtype != torch.float32 or scales.device != cache.device:
+        raise ValueError(f"{name} must be float32 on the cache's device")
+
+
+def _scales_args(key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor | None,
+                 value_scales: torch.Tensor | None) -> "CacheScalesArgs | None":
+    """The scales of an 8-bit cache, checked; None for a cache of another type."""
+    if key_cache.dtype != CACHE_8BIT:
+        if key_scales is not None or value_scales is not None:
+            raise ValueError(f"key_scales and value_scales belong to {CACHE_8BIT} caches, not {key_cache.dtype}")
+        return None
+    if key_scales is None or value_scales is None:
+        raise ValueError(f"a {CACHE_8BIT} cache needs key_scales and value_scales")
+    _check_scales(key_scales, "key_scales", key_cache)
+    _check_scales(value_scales, "value_scales", value_cache)
+    return CacheScalesArgs(key_scales.data_ptr(), *key_scales.stride(), value_scales.data_ptr(),
+                           *value_scales.stride())
+
+
 def _check_cache_pair(key_cache: torch.Tensor, value_cache: torch.Tensor) -> None:
     if key_cache.dim() != 4 or value_cache.dim() != 4:
         raise ValueError("key_cache/value_cache must be [num_blocks, num_kv_heads, block_size, head_dim]")
@@ -396,16 +431,19 @@ def _check_cache_pair(key_cache: torch.Tensor, value_cache: torch.Tensor) -> Non
         raise ValueError("cache head_dim must be contiguous")
     if not key_cache.is_cuda or key_cache.device != value_cache.device:
         raise ValueError("caches must be CUDA tensors on one device")
-    if key_cache.dtype not in _DTYPE_CODE:
+    if key_cache.dtype not in _DTYPE_CODE and key_cache.dtype != CACHE_8BIT:
         raise ValueError(f"unsupported cache dtype {key_cache.dtype}")
 
 
 def _check_new_rows(t: torch.Tensor, name: str, B: int, Hkv: int, q_len: int, D: int,
-                    dtype: torch.dtype, device: torch.device) -> None:
+                    dtype: torch.dtype | None, device: torch.device) -> None:
     if t.dim() != 4 or tuple(t.shape) != (B, Hkv, q_len, D):
         raise ValueError(f"{name} must be [batch={B}, num_kv_heads={Hkv}, q_len={q_len}, head_dim={D}], "
                          f"got {tuple(t.shape)}")
-    if t.dtype != dtype or t.device != device:
+    if dtype is None:  # an 8-bit cache: rows of any kernel type are rounded to it
+        if t.dtype not in _DTYPE_CODE or t.device != device:
+            raise ValueError(f"{name} must be fp32, fp16 or bf16 on the cache's device")
+    elif t.dtype != dtype or t.device != device:
         raise ValueError(f"{name} must match the cache dtype and device")
     if t.stride(3) != 1:
         raise ValueError(f"{name} head_dim must be contiguous")
@@ -467,6 +505,8 @@ def kv_append(
     position_offset: int = 0,
     error_word: torch.Tensor | None = None,
     validate: bool | None = None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
 ) -> None:
     """Scatter new rows ``key``/``value`` [B, Hkv, q_len, D] into the caches.
 
@@ -475,6 +515,15 @@ def kv_append(
     p = positions[b] + position_offset + t.  Bit-exact.  Invalid slots or block
     ids are skipped and flagged; the next call on the same error word raises
     IndexError (``validate=True``: this call, synchronously).
+
+    A cache of ``torch.float8_e4m3fn`` takes ``key_scales`` / ``value_scales``
+    (float32 [num_blocks, Hkv], any strides) and rows of fp32, fp16 or bf16: the
+    value of a code is code * scale[block, head].  A block's scale is the least
+    2^e (e >= -100) with its largest finite magnitude at most 448 * 2^e; writing
+    offset 0 starts the block anew, any other write only raises the scale, and the
+    block's other codes are then rounded again.  The tokens of a block must come
+    from one row of the call (another row's are left out and flagged).
+    head_dim is a multiple of 16, block_size a power of two in [8, 256].
     """
     _check_cache_pair(key_cache, value_cache)
     device = key_cache.device
@@ -482,8 +531,12 @@ def kv_append(
         raise ValueError("key must be [batch, num_kv_heads, q_len, head_dim]")
     B, _, q_len, _ = key.shape
     _, Hkv, bs, Dc = key_cache.shape
-    _check_new_rows(key, "key", B, Hkv, q_len, Dc, key_cache.dtype, device)
-    _check_new_rows(value, "value", B, Hkv, q_len, Dc, key_cache.dtype, device)
+    scales = _scales_args(key_cache, value_cache, key_scales, value_scales)
+    row_dtype = None if scales is not None else key_cache.dtype
+    _check_new_rows(key, "key", B, Hkv, q_len, Dc, row_dtype, device)
+    _check_new_rows(value, "value", B, Hkv, q_len, Dc, row_dtype, device)
+    if key.dtype != value.dtype:
+        raise ValueError("key and value must have the same dtype")
     args = KvAppendArgs()
     args.key = key.data_ptr()
     args.key_stride_b, args.key_stride_h, args.key_stride_t = key.stride()[:3]
@@ -523,7 +576,7 @@ def kv_append(
         args.positions_is_int64 = 1 if positions.dtype == torch.int64 else 0
         args.position_offset = int(position_offset)
     args.batch, args.q_len, args.num_kv_heads, args.head_dim, args.block_size = B, q_len, Hkv, Dc, bs
-    args.dtype = _DTYPE_CODE[key_cache.dtype]
+    args.dtype = _DTYPE_CODE[key.dtype]
     if error_word is None:
         error_word = decode_workspace(device)
     args.error_flags = error_word.data_ptr()
@@ -531,7 +584,11 @@ def kv_append(
     if deferred:
         _raise_landed_errors(error_word)
     with _with_device(device):
-        _lib.check(_lib.load().pa_kv_append(ctypes.byref(args), _stream_ptr(device)), "pa_kv_append")
+        if scales is not None:
+            _lib.check(_lib.load().pa_kv_append_8bit(ctypes.byref(args), ctypes.byref(scales), _stream_ptr(device)),
+                       "pa_kv_append_8bit")
+        else:
+            _lib.check(_lib.load().pa_kv_append(ctypes.byref(args), _stream_ptr(device)), "pa_kv_append")
     if deferred:
         _copy_after_call(error_word, _stream_ptr(device))
     elif validate if validate is not None else _VALIDATE_DEFAULT:
@@ -570,8 +627,18 @@ def paged_attention_decode(
     validate: bool | None = None,
     prefix_groups=None,
     gather=None,
+    key_scales: torch.Tensor | None = None,
+    value_scales: torch.Tensor | None = None,
+    score_modifiers=None,
 ) -> torch.Tensor:
     """Append this step's K/V (optional) and attend; returns [B, Hq, q_len, D].
+
+    ``key_scales`` / ``value_scales`` (float32 [num_blocks, Hkv]) go with caches
+    of ``torch.float8_e4m3fn``, whose values are code * scale[block, head]; the
+    query is fp16 or bf16, and new rows are rounded as ``kv_append`` says.
+
+    ``score_modifiers`` (a ``score_modifiers.ScoreModifiers``) caps, biases and
+    masks the scores.  Neither goes with ``prefix_groups`` or ``gather``.
 
     ``prefix_groups`` (a ``prefix_sharing.PrefixGroups``) marks rows whose
     tables share leading physical blocks: the call then attends each shared
@@ -589,8 +656,15 @@ def paged_attention_decode(
     _, Hkv, bs, Dc = key_cache.shape
     if D != Dc:
         raise ValueError(f"query head_dim {D} does not match cache head_dim {Dc}")
-    if query.dtype != key_cache.dtype or query.device != device:
+    scales = _scales_args(key_cache, value_cache, key_scales, value_scales)
+    if scales is not None:
+        if query.dtype not in (torch.float16, torch.bfloat16) or query.device != device:
+            raise ValueError("an 8-bit cache is attended by fp16 or bf16 queries on its device")
+    elif query.dtype != key_cache.dtype or query.device != device:
         raise ValueError("query must match the cache dtype and device")
+    shared = prefix_groups is not None and prefix_groups.num_groups > 0
+    if (scales is not None or score_modifiers is not None) and (shared or gather is not None):
+        raise ValueError("8-bit caches and score_modifiers go with neither prefix_groups nor gather")
     if query.stride(3) != 1:
         raise ValueError("query head_dim must be contiguous")
     if Hq % Hkv != 0:
@@ -621,7 +695,8 @@ def paged_attention_decode(
 
     lib = _lib.load()
     dcode = _DTYPE_CODE[query.dtype]
-    cascade = prefix_groups is not None and prefix_groups.num_groups > 0
+    modifiers = None if score_modifiers is None else score_modifiers.to_args(B, Hq, q_len, device)
+    cascade = shared
     if cascade:
         if prefix_groups.seq_group.numel() != B or prefix_groups.seq_group.device != device:
             raise ValueError("prefix_groups must describe this batch on the cache's device")
@@ -641,7 +716,7 @@ def paged_attention_decode(
             key, value, key_cache, value_cache, slot_mapping,
             block_tables=block_tables, positions=context_lens,
             position_offset=-q_len if context_lens_include_new else 0,
-            error_word=workspace, validate=False,
+            error_word=workspace, validate=False, key_scales=key_scales, value_scales=value_scales,
         )
         appended = True
 
@@ -682,7 +757,11 @@ def paged_attention_decode(
             _lib.check(lib.pa_decode_cascade(ctypes.byref(args), ctypes.byref(groups), stream_ptr),
                        "pa_decode_cascade")
         else:
-            rc = lib.pa_decode(ctypes.byref(args), stream_ptr)
+            if scales is None and modifiers is None:
+                rc = lib.pa_decode(ctypes.byref(args), stream_ptr)
+            else:
+                rc = lib.pa_decode_ext(ctypes.byref(args), ctypes.byref(scales) if scales is not None else None,
+                                       ctypes.byref(modifiers) if modifiers is not None else None, stream_ptr)
             if rc == _lib.PA_ERR_UNSUPPORTED and B > 1 and _BATCH_LIMIT_TEXT in _lib.last_error():
                 # More sequences than the kernel's shared-memory tables hold:
                 # the rows are independent, so attend the two halves one after
@@ -692,7 +771,10 @@ def paged_attention_decode(
                     paged_attention_decode(query[lo:hi], key_cache, value_cache, block_tables[lo:hi],
                                            context_lens[lo:hi], scale, out=out[lo:hi],
                                            context_lens_include_new=context_lens_include_new,
-                                           workspace=workspace, validate=False)
+                                           workspace=workspace, validate=False, key_scales=key_scales,
+                                           value_scales=value_scales,
+                                           score_modifiers=None if score_modifiers is None
+                                           else score_modifiers.rows(lo, hi))
             else:
                 _lib.check(rc, "pa_decode")
     if deferred:
