@@ -123,7 +123,8 @@ int check_cache_view(const pa_cache_view& v, const char* name) {
 
 // 4-D tensor map (head_dim, token, kv head, block) with 128-byte swizzle and a
 // box of (64 elements, min(bs, 16) tokens, 1, 1).  tile8: an 8-bit cache and its
-// tile's columns: a box of (tile8 bytes, ...), swizzled over its own row.
+// tile's columns: a box of (tile8 bytes, min(bs, 32) tokens, 1, 1), swizzled over
+// its own row.
 int encode_cache_map(CUtensorMap* map, const pa_cache_view& v, int dtype, int D, int bs, int Hkv,
                      const char* name, int tile8 = 0) {
   PFN_cuTensorMapEncodeTiled_v12000 enc;
@@ -138,7 +139,8 @@ int encode_cache_map(CUtensorMap* map, const pa_cache_view& v, int dtype, int D,
       return fail(PA_ERR_UNSUPPORTED, "%s: strides must be multiples of 16 bytes", name);
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)bs, (cuuint64_t)Hkv, (cuuint64_t)v.num_blocks};
   cuuint64_t strides[3] = {(cuuint64_t)sb[0], (cuuint64_t)sb[1], (cuuint64_t)sb[2]};
-  cuuint32_t box[4] = {tile8 ? (cuuint32_t)tile8 : 64u, (cuuint32_t)(bs < 16 ? bs : 16), 1u, 1u};
+  const int unit = tile8 ? 32 : 16;  // tokens
+  cuuint32_t box[4] = {tile8 ? (cuuint32_t)tile8 : 64u, (cuuint32_t)(bs < unit ? bs : unit), 1u, 1u};
   cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
   CUresult r = enc(map, tile8                        ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                         : dtype == PA_DTYPE_BFLOAT16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
@@ -721,6 +723,17 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
       g_last_kernel = "pa::prefill_mma_kernel<ext>";
       e = pa::launch_prefill_ext(p, tmk, tmv, dtype, pdl, strm);
       if (e != cudaSuccess) return cuda_fail(e, "multi-query launch");
+      return PA_OK;
+    }
+    static const long long direct_rows = getenv("DIRECT_ROWS") ? atoll(getenv("DIRECT_ROWS")) : info->num_sms;
+    if ((long long)p.B * p.Hkv * p.NMG <= direct_rows) {
+      int n = 8;
+      while (n > 2 && pa::decode_direct_smem_bytes(D, n, sc != nullptr) > budget - 6144) --n;
+      p.stages = n;
+      g_last_kernel = "pa::decode_direct_kernel";
+      e = pa::launch_decode_direct(p, tmk, tmv, dtype, info->num_sms,
+                                   pa::decode_direct_smem_bytes(D, n, sc != nullptr), pdl, strm);
+      if (e != cudaSuccess) return cuda_fail(e, "decode launch");
       return PA_OK;
     }
     g_last_kernel = "pa::decode_mma_kernel<ext>";

@@ -5,8 +5,8 @@
 namespace pa {
 
 size_t decode_ext_smem_bytes(int D, int B, int stages, bool eight, bool scored) {
-  const size_t stage_bytes = 2u * 16u * (size_t)D * (eight ? 1u : 2u);
-  return 1024 + (size_t)kDecodeWarps * stages * (stage_bytes + 8 + (eight ? 16 : 0)) +
+  const size_t stage_bytes = 2u * 16u * (size_t)D * 2u;  // 16 tokens of 2 bytes, or 32 of 1
+  return 1024 + (size_t)kDecodeWarps * stages * (stage_bytes + 8 + (eight ? 32 : 0)) +
          ((size_t)decode_seq_tables(false, scored) * B + 2) * 4;
 }
 

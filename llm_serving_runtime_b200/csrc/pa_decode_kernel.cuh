@@ -56,22 +56,24 @@ struct Cursor {
 // Query rows of one kv head are ordered token-major: row qr is query token
 // qr / G of query head h*G + qr % G, so a 16-row group holds consecutive tokens
 // of every head that reads this kv head.  A group whose latest token is t_max
-// attends positions 0 .. L - q_len + t_max: it scans that many 16-token units.
+// attends positions 0 .. L - q_len + t_max: it scans that many units of UT tokens.
+template <int UT>
 __device__ __forceinline__ int group_units(int L, int mg, const DecodeParams& p) {
   const int last_row = min(16 * mg + 15, p.GQ - 1);
   const int lim = L - p.q_len + last_row / p.G;  // last attendable position
-  return lim < 0 ? 0 : (lim + kUnitTokens) / kUnitTokens;
+  return lim < 0 ? 0 : (lim + UT) / UT;
 }
 
 // Changed scores: the units a group scans, from its earliest token's first key
 // (start: the least key_starts entry of the sequence) to its latest token's last.
+template <int UT>
 __device__ __forceinline__ void group_range(int L, int start, int prefix, int mg, const DecodeParams& p, int& u0,
                                             int& n) {
   const int last_row = min(16 * mg + 15, p.GQ - 1);
   const int lo = key_range(L, p.q_len, (16 * mg) / p.G, p.window, start, prefix).first;
   const int hi = key_range(L, p.q_len, last_row / p.G, 0, 0, prefix).end;
-  u0 = lo / kUnitTokens;
-  n = hi <= lo ? 0 : (hi + kUnitTokens - 1) / kUnitTokens - u0;
+  u0 = lo / UT;
+  n = hi <= lo ? 0 : (hi + UT - 1) / UT - u0;
 }
 
 // The fused all-gather's end of a call, run by the grid's last warp: raise
@@ -147,10 +149,11 @@ inline __device__ __noinline__ void gather_barrier(uint32_t* const* flags_ranks,
 // rows.  kMode 2 (gather): output rows go to every rank's gathered output
 // (pa_decode_gather).  kMode 0: plain decode.  KV: the cache's element (T, or
 // e4m3_t with scales), kScored: changed scores; both with kMode 0 only, and
-// pa_tile_ext.cuh has their arithmetic.  8 bits halve a unit's bytes at the
-// same ring size, so the ring holds twice the units.  Their two scales come with
-// the unit: lane 0 copies them next to the tiles (cp.async) and the copies
-// arrive on the unit's own mbarrier.
+// pa_tile_ext.cuh has their arithmetic.  An 8-bit
+// unit has 32 tokens, the bytes of a 16-bit unit's 16.  Its scales come with it:
+// eight lanes copy one each next to the tiles (cp.async), and their copies arrive
+// on the unit's own mbarrier.  With either, several lanes issue a unit's copies in
+// one instruction.
 template <typename T, int D, int kMode, typename KV = T, bool kScored = false>
 __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
     decode_mma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
@@ -161,8 +164,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   constexpr bool kExt = k8 || kScored;
   static_assert(!kExt || kMode == 0, "8-bit caches and changed scores: plain decode only");
   using TL = TileLayout<KV, D>;
+  constexpr int UT = TL::kTokens;            // tokens of a unit
   constexpr int HALVES = TL::kHalves;        // TMA boxes across a tile row
-  constexpr uint32_t TILE_BYTES = TL::kTileBytes;  // one 16-token K (or V) tile
+  constexpr uint32_t TILE_BYTES = TL::kTileBytes;  // a unit's K (or V) tile
   constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
   constexpr int DPL = D / 32;                // dims per lane in the merge
 
@@ -173,9 +177,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   const int stages = p.stages;
   const uint32_t ring_addr = smem_addr(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)kDecodeWarps * stages * STAGE_BYTES);
-  // 8-bit: each ring slot's scales (K of tokens 0-7 and 8-15, V of the same)
+  // 8-bit: each ring slot's scales (K of its four groups of 8 tokens, V of the same)
   float4* s_scales = reinterpret_cast<float4*>(bars + kDecodeWarps * stages);
-  int* s_lens = reinterpret_cast<int*>(s_scales + (k8 ? kDecodeWarps * stages : 0));
+  int* s_lens = reinterpret_cast<int*>(s_scales + (k8 ? 2 * kDecodeWarps * stages : 0));
   int* s_pref = s_lens + p.B;
   int* s_rpref = s_pref + p.B + 1;  // exclusive prefix of rows with units, per sequence
   // Cascade (shared prefixes): the prefix kernel has attended each member's
@@ -195,7 +199,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   const int B = p.B;
 
   if (lane == 0) {
-    for (int s = 0; s < stages; ++s) mbar_init(smem_addr(&bars[warp * stages + s]), k8 ? 2 : 1);
+    for (int s = 0; s < stages; ++s) mbar_init(smem_addr(&bars[warp * stages + s]), k8 ? 9 : 1);
   }
   if (tid == 0) {
     prefetch_tensormap(&tmk);
@@ -237,9 +241,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
       for (int mg = 0; mg < p.NMG; ++mg) {
         int n;
         if constexpr (kScored)
-          group_range(L, s_start[b], s_prefix[b], mg, p, u0, n);
+          group_range<UT>(L, s_start[b], s_prefix[b], mg, p, u0, n);
         else
-          n = max(0, group_units(L, mg, p) - u0);
+          n = max(0, group_units<UT>(L, mg, p) - u0);
         units += n;
         rows += n > 0;
       }
@@ -273,9 +277,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
       for (int mg = 0; mg < p.NMG; ++mg) {
         int n, u0;
         if constexpr (kScored)
-          group_range(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
+          group_range<UT>(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
         else
-          n = max(0, group_units(s_lens[b], mg, p) - (cascade ? s_u0[b] : 0));
+          n = max(0, group_units<UT>(s_lens[b], mg, p) - (cascade ? s_u0[b] : 0));
         units += n;
         rows += n > 0;
       }
@@ -314,10 +318,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   auto units_of = [&](int b, int mg) -> int {
     if constexpr (kScored) {
       int u0, n;
-      group_range(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
+      group_range<UT>(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
       return n;
     }
-    const int n = group_units(s_lens[b], mg, p);
+    const int n = group_units<UT>(s_lens[b], mg, p);
     return cascade ? max(0, n - s_u0[b]) : n;
   };
 
@@ -325,7 +329,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   auto first_unit = [&](int b, int mg) -> int {
     if constexpr (kScored) {
       int u0, n;
-      group_range(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
+      group_range<UT>(s_lens[b], s_start[b], s_prefix[b], mg, p, u0, n);
       return u0;
     }
     return cascade ? s_u0[b] : 0;
@@ -375,7 +379,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   // in its equal share of the total cost C.
   constexpr int kRowCostUnits = cascade ? kRowCostUnitsCascade : kRowCostUnitsPlain;
   const long long C = W + (long long)kRowCostUnits * s_rpref[B];
-  long long nw_eff = (C + kMinUnitsPerWarp - 1) / kMinUnitsPerWarp;
+#ifndef EXT_MIN_UNITS
+#define EXT_MIN_UNITS 8
+#endif
+  constexpr int kMinUnits = kExt ? EXT_MIN_UNITS : kMinUnitsPerWarp;
+  long long nw_eff = (C + kMinUnits - 1) / kMinUnits;
   if (nw_eff > p.nw_total) nw_eff = p.nw_total;
   if (nw_eff < 1) nw_eff = 1;
   // Per-SM shares.  SMs stream at different speeds (up to ~10 % apart, in a
@@ -545,14 +553,14 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
         }
       }
       if constexpr (kScored)
-        group_range(s_lens[c.b], s_start[c.b], s_prefix[c.b], c.mg, p, c.u0, c.n);
+        group_range<UT>(s_lens[c.b], s_start[c.b], s_prefix[c.b], c.mg, p, c.u0, c.n);
       else
         c.n = units_of(c.b, c.mg);
     } while (c.n == 0);
   };
   // Position of the first token of the cursor's unit.
   auto unit_token = [&](const Cursor& c) -> int {
-    return (c.u + (kScored ? c.u0 : cascade ? s_u0[c.b] : 0)) * kUnitTokens;
+    return (c.u + (kScored ? c.u0 : cascade ? s_u0[c.b] : 0)) * UT;
   };
 
   const uint32_t my_ring = ring_addr + (uint32_t)(warp * stages) * STAGE_BYTES;
@@ -563,6 +571,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   long long pf = ws;
   int win_b = -1, win_base = 0, win_val = -1;
   const int bs = p.bs;
+  [[maybe_unused]] const int bs_log2 = 31 - __clz(bs);
 
   // Keeps block-table entries [win_base, win_base + 32) of sequence win_b in
   // the warp's lanes; reloads (one coalesced load) when lb .. lb+need-1 leave it.
@@ -602,20 +611,47 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
     const uint32_t stage = my_ring + (uint32_t)slot * STAGE_BYTES;
     const uint32_t bar = my_bars + (uint32_t)slot * 8u;
     const int tok0 = unit_token(pc);
-    // 8-bit: the scales of the unit's one or two blocks, copied by lane 0 next to
-    // the tiles (a bad block id, whose tiles are zeros, gets zeros).
-    [[maybe_unused]] auto copy_scales = [&](int phys0, int phys1) {
-      const uint32_t dst = smem_addr(&s_scales[warp * stages + slot]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int phys = j ? phys1 : phys0;
-        const bool ok = phys >= 0 && phys < p.num_blocks;
-        const long long blk = ok ? phys : 0;
-        cp_async_4_zfill(dst + 4u * j, p.k_scales + blk * p.ks_sblk + h * p.ks_sh, ok ? 4u : 0u);
-        cp_async_4_zfill(dst + 8u + 4u * j, p.v_scales + blk * p.vs_sblk + h * p.vs_sh, ok ? 4u : 0u);
+    if constexpr (kExt) {
+      // Lane roles: 8-bit, lane = 4 * (K or V) + group of 8 tokens, each copying
+      // its group's scale and the first group of a block its box as well; 16-bit,
+      // lane = (block, K or V, column half).
+      const int L = s_lens[pc.b];
+      int lo = 0;  // a block that ends before the row's first key is not loaded, nor one past L
+      if constexpr (kScored)
+        lo = key_range(L, p.q_len, (16 * pc.mg) / p.G, p.window, s_start[pc.b], s_prefix[pc.b]).first;
+      const int lb0 = tok0 >> bs_log2;
+      ensure_window(pc.b, lb0, max(1, UT >> bs_log2));
+      const int g = k8 ? 8 * (lane & 3) : (lane / (2 * HALVES)) * bs;  // this lane's first token of the unit
+      const int kv = k8 ? (lane >> 2) & 1 : (lane / HALVES) & 1;
+      const int hf = k8 ? 0 : lane % HALVES;
+      const int lb = (tok0 + g) >> bs_log2;
+      const int y = (tok0 + g) & (bs - 1);
+      const int phys = __shfl_sync(0xffffffffu, win_val, (lb - win_base) & 31);
+      const bool mine = k8 ? lane < 8 : lane < 2 * HALVES * (bs < UT ? UT >> bs_log2 : 1);
+      const bool want = mine && (lb << bs_log2) < L && ((lb + 1) << bs_log2) > lo;
+      const bool ok = phys >= 0 && phys < p.num_blocks;
+      const bool box = want && (!k8 || (lane & 3) == 0 || y == 0);
+      const uint32_t boxes = __ballot_sync(0xffffffffu, box);
+      const uint32_t box_bytes = (uint32_t)min(bs, UT) * TL::kRowBytes;
+      if (want && !ok) raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
+      if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * box_bytes);
+      __syncwarp();
+      if (box)  // a bad id is out of the map's range: TMA fills zeros
+        tma_load_4d_policy(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * TL::kHalfBytes +
+                               (uint32_t)g * TL::kRowBytes,
+                           kv ? &tmv : &tmk, bar, hf * 64, y, h, phys, kv_policy);
+      if constexpr (k8) {
+        if (lane < 8) {
+          const bool use = want && ok;
+          const long long blk = use ? phys : 0;
+          const float* from = kv ? p.v_scales + blk * p.vs_sblk + h * p.vs_sh : p.k_scales + blk * p.ks_sblk + h * p.ks_sh;
+          cp_async_4_zfill(smem_addr(&s_scales[2 * (warp * stages + slot)]) + 4u * lane, from, use ? 4u : 0u);
+          cp_async_mbar_arrive_noinc(bar);
+        }
       }
-      cp_async_mbar_arrive_noinc(bar);
-    };
+      __syncwarp();
+      return;
+    }
     if (bs >= kUnitTokens) {
       const int lb = tok0 / bs;
       const int y = tok0 - lb * bs;
@@ -624,7 +660,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
       if (lane == 0) {
         if (phys < 0 || phys >= p.num_blocks) raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
         mbar_arrive_expect_tx(bar, STAGE_BYTES);
-        if constexpr (k8) copy_scales(phys, phys);
 #pragma unroll
         for (int hf = 0; hf < HALVES; ++hf)
           tma_load_4d_policy(stage + hf * 2048u, &tmk, bar, hf * 64, y, h, phys, kv_policy);
@@ -641,18 +676,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
       const int phys1 = __shfl_sync(0xffffffffu, win_val, lb0 + 1 - win_base);
       if (lane == 0) {
         const bool need1 = (lb0 + 1) * bs < L;
-        // changed scores: nor is a first block that ends before the row's first key
-        bool need0 = true;
-        if constexpr (kScored)
-          need0 = (lb0 + 1) * bs >
-                  key_range(L, p.q_len, (16 * pc.mg) / p.G, p.window, s_start[pc.b], s_prefix[pc.b]).first;
-        const uint32_t box_bytes = (uint32_t)bs * TL::kRowBytes;
-        const uint32_t nbox = ((need0 ? 1u : 0u) + (need1 ? 1u : 0u)) * HALVES * 2u;
-        if ((need0 && (phys0 < 0 || phys0 >= p.num_blocks)) || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
+        const uint32_t box_bytes = (uint32_t)bs * 128u;
+        const uint32_t nbox = (need1 ? 2u : 1u) * HALVES * 2u;
+        if (phys0 < 0 || phys0 >= p.num_blocks || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
           raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
         mbar_arrive_expect_tx(bar, nbox * box_bytes);
-        if constexpr (k8) copy_scales(need0 ? phys0 : -1, need1 ? phys1 : -1);
-        for (int j = need0 ? 0 : 1; j < (need1 ? 2 : 1); ++j) {
+        for (int j = 0; j < (need1 ? 2 : 1); ++j) {
           const int phys = j ? phys1 : phys0;
 #pragma unroll
           for (int hf = 0; hf < HALVES; ++hf) {
@@ -667,7 +696,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
 
   if (has_work) {
     const int tok0 = unit_token(start);
-    ensure_window(start.b, tok0 / bs, bs >= kUnitTokens ? 1 : 2);
+    ensure_window(start.b, tok0 / bs, bs >= UT ? 1 : UT / bs);
   }
 
   // Everything below reads the K/V cache, which the previous kernel may write
@@ -780,13 +809,13 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
 
     // ---- QK^T, masked online softmax, PV on tensor cores ----
     if constexpr (kExt) {
-      float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
-      if constexpr (k8) {
-        const float4 sc = s_scales[warp * stages + slot];
-        ks[0] = sc.x, ks[1] = sc.y, vs[0] = sc.z, vs[1] = sc.w;
-      }
-      attend_unit_ext<T, KV, D, kScored>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo,
-                                        full_hi, ks, vs, p, lane);
+      if constexpr (k8)
+        attend_unit_8<T, D, kScored>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi,
+                                     s_scales[2 * (warp * stages + slot)], s_scales[2 * (warp * stages + slot) + 1],
+                                     p, lane);
+      else
+        attend_unit_scored<T, D>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi, p,
+                                 lane);
     } else {
       attend_unit<T, D>(kbase, vbase, qa, o_acc, m0, m1, l0, l1, unit_token(cc), L, lim0, lim1, mask_from,
                         p.scale_log2, lane);
@@ -806,7 +835,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
     if (row_end || cf + 1 == we) {
       if constexpr (kExt) {
         m0 = st.m[0], m1 = st.m[1], l0 = st.l[0], l1 = st.l[1];
-        if constexpr (k8) end_piece_columns<D>(o_acc, st);
+        if constexpr (k8) end_piece_columns<D>(o_acc);
       }
       float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
       float lt1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -834,8 +863,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
           const long long ridx1 = (rb + qa1 % p.G) * p.q_len + qa1 / p.G;
           store_rows_folded<T, D>(op0, op1, o_acc, mm0, mm1, ll0, ll1, ridx0, ridx1, p, quad);
         } else if constexpr (kExt) {
-          store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm(ll0, st.first[0] < st.end[0]),
-                                   row_norm(ll1, st.first[1] < st.end[1]), quad, p.Dv);
+          store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm<KV>(ll0, st.first[0] < st.end[0]),
+                                   row_norm<KV>(ll1, st.first[1] < st.end[1]), quad, p.Dv);
         } else {
           store_rows<T, D>(op0, op1, o_acc, ll0, ll1, quad, p.Dv);
         }
@@ -1024,7 +1053,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
                 float inv = lsum[r] > 0.f ? 1.f / lsum[r] : 0.f;
                 if constexpr (kExt) {
                   const KeyRange kr = row_keys<kScored>(p, b, L, t);
-                  inv = row_norm(lsum[r], kr.first < kr.end);
+                  inv = row_norm<KV>(lsum[r], kr.first < kr.end);
                 }
                 for (int dst = 0; dst < n_dst; ++dst) {
                   T* op = out_row(dst, b, h * p.G + g, t);

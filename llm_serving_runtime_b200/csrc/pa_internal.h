@@ -178,6 +178,12 @@ struct ScaleParams {
   int64_t ks_sblk, ks_sh, vs_sblk, vs_sh;
 };
 
+// pa_decode_ext for at most num_sms rows (B * Hkv * NMG): CTAs of their own for
+// each row (pa_decode_direct.cu).
+size_t decode_direct_smem_bytes(int D, int stages, bool eight);
+cudaError_t launch_decode_direct(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
+                                 int num_sms, size_t smem, bool pdl, cudaStream_t stream);
+
 // Caches whose pages move together: byte strides; a page is `segments` runs of
 // segment_bytes, stride_segment apart.
 constexpr int kMaxPageViews = PA_MAX_PAGE_VIEWS;

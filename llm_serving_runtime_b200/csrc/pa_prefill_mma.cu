@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   constexpr bool k8 = kIs8<KV>::value;
   constexpr bool kExt = k8 || kScored;
   using TL = TileLayout<KV, D>;
+  constexpr int UT = TL::kTokens;  // tokens of a unit
   constexpr int HALVES = TL::kHalves;
   constexpr uint32_t TILE_BYTES = TL::kTileBytes;
   constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
@@ -40,7 +41,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const uint32_t ring = smem_addr(smem);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + (size_t)S * STAGE_BYTES);
   uint64_t* empty = full + S;
-  __shared__ float4 s_scales[k8 ? S : 1];  // 8-bit: a slot's scales, K of tokens 0-7 and 8-15, V of the same
+  __shared__ float4 s_scales[k8 ? 2 * S : 1];  // 8-bit: a slot's scales, K of its groups of 8 tokens, V of the same
   __shared__ int s_lo, s_hi;               // changed scores: keys that some row of the tile sees
 
   const int tid = threadIdx.x;
@@ -67,7 +68,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   const int active = (rows_tile + 15) / 16;  // consumer warps that own rows
   const int lim_tile = L - p.q_len + (row0 + rows_tile - 1) / p.G;
   int u_first = 0;  // the tile's first unit
-  int n_units = lim_tile < 0 ? 0 : (lim_tile + kUnitTokens) / kUnitTokens;
+  int n_units = lim_tile < 0 ? 0 : (lim_tile + UT) / UT;
   if constexpr (kScored) {
     if (tid == 0) {
       s_lo = INT_MAX;
@@ -82,13 +83,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       }
     }
     __syncthreads();
-    u_first = min(s_lo, s_hi) / kUnitTokens;
-    n_units = s_lo < s_hi ? (s_hi + kUnitTokens - 1) / kUnitTokens - u_first : 0;
+    u_first = min(s_lo, s_hi) / UT;
+    n_units = s_lo < s_hi ? (s_hi + UT - 1) / UT - u_first : 0;
   }
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(smem_addr(&full[s]), k8 ? 2 : 1);
+      mbar_init(smem_addr(&full[s]), k8 ? 9 : 1);
       mbar_init(smem_addr(&empty[s]), active);
     }
     prefetch_tensormap(&tmk);
@@ -114,48 +115,67 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
           return;
         }
       }
-      const int tok0 = (u_first + u) * kUnitTokens;
+      const int tok0 = (u_first + u) * UT;
       const int lb0 = tok0 / bs;
-      const int need = bs >= kUnitTokens ? 1 : kUnitTokens / bs;
+      const int need = bs >= UT ? 1 : UT / bs;
       if (win_base < 0 || lb0 < win_base || lb0 + need > win_base + 32) {
         win_base = lb0;
         const int e = lb0 + lane;
         win_val = (e < p.max_blocks) ? __ldg(&p.block_tables[(long long)b * p.bt_stride + e]) : -1;
       }
+      const uint32_t stage = ring + (uint32_t)slot * STAGE_BYTES;
+      const uint32_t bar = smem_addr(&full[slot]);
+      if constexpr (kExt) {
+        // lane roles as in the decode kernel: 8-bit, 4 * (K or V) + group of 8 tokens;
+        // 16-bit, (block, K or V, column half)
+        const int lo = kScored ? s_lo : 0;
+        const int g = k8 ? 8 * (lane & 3) : (lane / (2 * HALVES)) * bs;
+        const int kv = k8 ? (lane >> 2) & 1 : (lane / HALVES) & 1;
+        const int hf = k8 ? 0 : lane % HALVES;
+        const int lb = (tok0 + g) / bs;
+        const int y = tok0 + g - lb * bs;
+        const int phys = __shfl_sync(0xffffffffu, win_val, (lb - win_base) & 31);
+        const bool mine = k8 ? lane < 8 : lane < 2 * HALVES * need;
+        const bool want = mine && lb * bs < L && (lb + 1) * bs > lo;
+        const bool ok = phys >= 0 && phys < p.num_blocks;
+        const bool box = want && (!k8 || (lane & 3) == 0 || y == 0);
+        const uint32_t boxes = __ballot_sync(0xffffffffu, box);
+        if (want && !ok) raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
+        if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)__popc(boxes) * (uint32_t)min(bs, UT) * TL::kRowBytes);
+        __syncwarp();
+        if (box)
+          tma_load_4d(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * TL::kHalfBytes + (uint32_t)g * TL::kRowBytes,
+                      kv ? &tmv : &tmk, bar, hf * 64, y, h, phys);
+        if constexpr (k8) {
+          if (lane < 8) {
+            const bool use = want && ok;
+            const long long blk = use ? phys : 0;
+            const float* from =
+                kv ? p.v_scales + blk * p.vs_sblk + h * p.vs_sh : p.k_scales + blk * p.ks_sblk + h * p.ks_sh;
+            cp_async_4_zfill(smem_addr(&s_scales[2 * slot]) + 4u * lane, from, use ? 4u : 0u);
+            cp_async_mbar_arrive_noinc(bar);
+          }
+        }
+        __syncwarp();
+        continue;
+      }
       const int phys0 = __shfl_sync(0xffffffffu, win_val, lb0 - win_base);
       const int phys1 = __shfl_sync(0xffffffffu, win_val, (lb0 + 1 - win_base) & 31);
       // One box per lane (K or V x 64-column half, x block for size 8), in one
       // instruction: a thread's bulk-tensor copies issue one after another.
-      const uint32_t stage = ring + (uint32_t)slot * STAGE_BYTES;
-      const uint32_t bar = smem_addr(&full[slot]);
       const bool need1 = bs < kUnitTokens && (lb0 + 1) * bs < L;
-      // changed scores: nor is a first block that ends before the tile's first key
-      bool need0 = true;
-      if constexpr (kScored) need0 = bs >= kUnitTokens || (lb0 + 1) * bs > s_lo;
-      const uint32_t box_bytes = bs >= kUnitTokens ? TL::kHalfBytes : (uint32_t)bs * TL::kRowBytes;
-      const int nbox = ((need0 ? 1 : 0) + (need1 ? 1 : 0)) * HALVES * 2;
+      const uint32_t box_bytes = bs >= kUnitTokens ? 2048u : (uint32_t)bs * 128u;
+      const int nbox = (need1 ? 2 : 1) * HALVES * 2;
       if (lane == 0) {
-        if ((need0 && (phys0 < 0 || phys0 >= p.num_blocks)) || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
+        if (phys0 < 0 || phys0 >= p.num_blocks || (need1 && (phys1 < 0 || phys1 >= p.num_blocks)))
           raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
         mbar_arrive_expect_tx(bar, (uint32_t)nbox * box_bytes);
-        if constexpr (k8) {
-          const uint32_t dst = smem_addr(&s_scales[slot]);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int phys = bs >= kUnitTokens ? phys0 : j ? (need1 ? phys1 : -1) : (need0 ? phys0 : -1);
-            const bool ok = phys >= 0 && phys < p.num_blocks;
-            const long long blk = ok ? phys : 0;
-            cp_async_4_zfill(dst + 4u * j, p.k_scales + blk * p.ks_sblk + h * p.ks_sh, ok ? 4u : 0u);
-            cp_async_4_zfill(dst + 8u + 4u * j, p.v_scales + blk * p.vs_sblk + h * p.vs_sh, ok ? 4u : 0u);
-          }
-          cp_async_mbar_arrive_noinc(bar);
-        }
       }
       __syncwarp();
       if (lane < nbox) {  // lane -> (block j, K or V, half)
-        const int j = lane / (2 * HALVES) + (need0 ? 0 : 1), kv = (lane / HALVES) & 1, hf = lane % HALVES;
+        const int j = lane / (2 * HALVES), kv = (lane / HALVES) & 1, hf = lane % HALVES;
         const int y = bs >= kUnitTokens ? tok0 - lb0 * bs : 0;
-        tma_load_4d(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * TL::kHalfBytes + (uint32_t)j * box_bytes,
+        tma_load_4d(stage + (uint32_t)kv * TILE_BYTES + (uint32_t)hf * 2048u + (uint32_t)j * box_bytes,
                     kv ? &tmv : &tmk, bar, hf * 64, y, h, j ? phys1 : phys0);
       }
       __syncwarp();
@@ -220,15 +240,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
     }
     const uint32_t kbase = ring + (uint32_t)slot * STAGE_BYTES;
     if constexpr (kExt) {
-      const int tok0 = (u_first + u) * kUnitTokens;
-      if (tok0 < tok_hi && tok0 + kUnitTokens > tok_lo) {  // some row of the warp sees some key of the unit
-        float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
-        if constexpr (k8) {
-          const float4 sc = s_scales[slot];
-          ks[0] = sc.x, ks[1] = sc.y, vs[0] = sc.z, vs[1] = sc.w;
-        }
-        attend_unit_ext<T, KV, D, kScored>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo,
-                                           full_hi, ks, vs, p, lane);
+      const int tok0 = (u_first + u) * UT;
+      if (tok0 < tok_hi && tok0 + UT > tok_lo) {  // some row of the warp sees some key of the unit
+        if constexpr (k8)
+          attend_unit_8<T, D, kScored>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo,
+                                       full_hi, s_scales[2 * slot], s_scales[2 * slot + 1], p, lane);
+        else
+          attend_unit_scored<T, D>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo, full_hi,
+                                   p, lane);
       }
     } else if (u < n_w) {
       attend_unit<T, D>(kbase, kbase + TILE_BYTES, qa, o_acc, m0, m1, l0, l1, u * kUnitTokens, L, lim0, lim1,
@@ -239,14 +258,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
 
   if constexpr (kExt) l0 = st.l[0], l1 = st.l[1];
-  if constexpr (k8) end_piece_columns<D>(o_acc, st);
+  if constexpr (k8) end_piece_columns<D>(o_acc);
   float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
   float lt1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
   lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
   lt1 += __shfl_xor_sync(0xffffffffu, lt1, 2);
   if constexpr (kExt)
-    store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm(lt0, st.first[0] < st.end[0]),
-                             row_norm(lt1, st.first[1] < st.end[1]), quad, p.Dv);
+    store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm<KV>(lt0, st.first[0] < st.end[0]),
+                             row_norm<KV>(lt1, st.first[1] < st.end[1]), quad, p.Dv);
   else
     store_rows<T, D>(op0, op1, o_acc, lt0, lt1, quad, p.Dv);
 }

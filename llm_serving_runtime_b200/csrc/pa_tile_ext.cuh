@@ -8,18 +8,21 @@
 //   s = scale * (q . k_j),  capped c * tanh(s / c),  minus slope * |i - j|
 //   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m)
 //
-// 8-bit caches.  k_j = ks * c_j and v_j = vs * d_j with codes c, d and the
-// block's scales ks, vs.  Codes widen to fp16 without rounding, so both products
-// run as fp16 MMAs whatever the query's type; ks multiplies the finished dot
-// product.  A bf16 query row is brought to fp16 by a power of two of its own
-// that puts its largest element into [2^14, 2^15): 8-bit significands fit
-// fp16's 11, and only elements 2^29 below the row's largest lose bits.
-// vs goes into the weights: the accumulator's reference is
-//   mo = max_j (x_j + log2 vs_j),  weights w_j = 2^(x_j + log2 vs_j - mo + 14)
-// apart from the sum's reference m = max_j x_j, so a block of large scale and no
-// weight cannot push the others' weights out of fp16's range.  w is rounded to
-// fp16 (11 bits, at most 2^-11 of each weight), normal down to 2^-28 of the
-// largest.  At the end of a piece the accumulator returns to the reference m.
+// 8-bit caches (attend_unit_8, 32 tokens at a time).  k_j = ks * c_j and v_j =
+// vs * d_j with codes c, d and the block's scales ks, vs.  Codes widen to fp16
+// without rounding, so both products run as fp16 MMAs whatever the query's type;
+// ks multiplies the finished dot product.  A bf16 query row is brought to fp16 by
+// a power of two of its own that puts its largest element into [2^14, 2^15): 8-bit
+// significands fit fp16's 11, and only elements 2^29 below the row's largest lose
+// bits.  vs goes into the weights, and the running reference is that of the
+// weighted values:
+//   m = max_j (x_j + log2 vs_j),  w_j = 2^(x_j + log2 vs_j - m + 14)
+//   out = sum_j w_j d_j / (2^14 sum_j 2^-14 w_j / vs_j)
+// so a block of large scale and little weight cannot push the others' weights
+// out of fp16's range, and one exponential serves both sums.  w is rounded to
+// fp16 for the product (at most 2^-11 of each weight; normal down to 2^-28 of the
+// largest), the norm takes it unrounded.  Scales other than 0 are taken to be at
+// least 2^-100 (the append writes no smaller ones).
 //
 // What a mask hides never reaches a row: hidden scores are -inf whatever K
 // holds, and where rows of one tile see different keys, tokens whose V row is
@@ -44,16 +47,6 @@ struct kIs8 {
   static constexpr bool value = sizeof(C) == 1;
 };
 
-// Element type of the P V product.
-template <typename T, typename C>
-struct PvType {
-  using type = T;
-};
-template <typename T>
-struct PvType<T, e4m3_t> {
-  using type = __half;
-};
-
 // Two e4m3 codes (bits 0-7, 8-15) to two fp16 values, exactly.
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
   uint32_t d;
@@ -69,16 +62,27 @@ __device__ __forceinline__ float lg2(float x) {
   return y;
 }
 
+// Tokens of an 8-bit unit: two k-steps of the P.V product, so that a unit's fixed
+// work (barrier, copies, maxima) is spread over the same bytes as a 16-bit one's.
+constexpr int kUnit8Tokens = 32;
+
+// 1 / x (approximate instruction; 1 / inf = 0).
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Element layout of a unit's tile in shared memory.  16-bit: 64-element column
-// halves of 16 rows x 128 bytes, 128-byte swizzle.  8-bit: 16 rows of D bytes,
+// halves of 16 rows x 128 bytes, 128-byte swizzle.  8-bit: 32 rows of D bytes,
 // swizzled over 128 bytes (D = 128) or 64 bytes (D = 64).
 template <typename C, int D>
 struct TileLayout {
   static constexpr bool k8 = kIs8<C>::value;
   static constexpr int kHalves = k8 ? 1 : D / 64;           // TMA boxes across a row
-  static constexpr int kBoxElems = k8 ? D : 64;             // elements of a box row
   static constexpr uint32_t kRowBytes = k8 ? D : 128;       // bytes of a box row
-  static constexpr uint32_t kHalfBytes = 16 * kRowBytes;    // one box of 16 tokens
+  static constexpr int kTokens = k8 ? kUnit8Tokens : kUnitTokens;
+  static constexpr uint32_t kHalfBytes = kTokens * kRowBytes;
   static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
 };
 
@@ -106,8 +110,7 @@ __device__ __forceinline__ int frag_col(int nd, int quad) {
 
 // Running state of a warp's rows lane/4 (index 0) and lane/4 + 8 (index 1).
 struct RowState {
-  float m[2], l[2];    // max and sum of 2^(x - m)
-  float mo[2];         // 8-bit: max of x + log2 vs
+  float m[2], l[2];    // the softmax's reference and norm
   float c[2];          // dot product -> x (scale * log2 e, and the query row's power of two)
   int first[2], end[2];  // keys the row sees
   float slope[2];      // distance bias, log2 domain
@@ -136,7 +139,7 @@ __device__ __forceinline__ void init_rows(RowState& st, const DecodeParams& p, i
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     const int qr = qr0 + 8 * r;
-    st.m[r] = st.mo[r] = -INFINITY;
+    st.m[r] = -INFINITY;
     st.l[r] = 0.f;
     st.first[r] = 0;  // rows past the group's last see everything and are not stored
     st.end[r] = INT_MAX;
@@ -204,52 +207,124 @@ __device__ __forceinline__ void load_query_frags_8(uint32_t (&qa)[D / 16][4], co
       qa[ks][i] = pack2<__half>(lo_half<T>(qa[ks][i]) * mul[i & 1], hi_half<T>(qa[ks][i]) * mul[i & 1]);
 }
 
-// c * tanh(x / c) in the log2 domain (cap, inv_cap = 1 / cap, both of it).
-// tanh y = 1 - 2 / (1 + e^2y) loses its low bits near 0, where the odd Taylor
-// series y - y^3/3 + 2y^5/15 - 17y^7/315 takes over (at |y| <= 0.25 its first
-// left-out term, 62y^9/2835, is 3.4e-7 of y).
+// c * tanh(x / c) in the log2 domain (cap, inv_cap = 1 / cap, both of it), with
+// tanh y = 1 - 2 / (1 + e^2y).  Near 0 that is off by 2^-22 of the cap (the
+// exponential's and the division's error), so up to kDirectCap a score is off by
+// less than 4e-5, far below the rounding of its weight.
+constexpr float kDirectCap = 128.f;
+__device__ __forceinline__ float softcap_direct(float x, float cap, float inv_cap) {
+  return fmaf(-2.f * cap, rcp_approx(1.f + ex2(x * inv_cap * 2.8853900817779268f)), cap);
+}
+
+// The same for larger caps: near 0 the odd Taylor series y - y^3/3 + 2y^5/15 -
+// 17y^7/315 takes over (at |y| <= 0.25 its first left-out term, 62y^9/2835, is
+// 3.4e-7 of y).
 __device__ __forceinline__ float softcap_log2(float x, float cap, float inv_cap) {
   const float y = x * inv_cap;
-  const float e = ex2(y * 2.8853900817779268f);
-  const float big = 1.f - __fdividef(2.f, 1.f + fminf(e, 1e30f));
   const float y2 = y * y;
   const float p = fmaf(y2, fmaf(y2, fmaf(y2, -17.f / 315.f, 2.f / 15.f), -1.f / 3.f), 1.f);
   // NaN fails the comparison and comes out of the series' argument
-  return fabsf(y) > 0.25f ? cap * big : x * p;
+  return fabsf(y) > 0.25f ? softcap_direct(x, cap, inv_cap) : x * p;
 }
 
-// One unit.  ks / vs: the scales of tokens 0-7 and 8-15 (8-bit caches).
+// Capped and biased scores of n-tiles of 8 tokens (log2 domain).
+template <int N>
+__device__ __forceinline__ void change_scores(float (&x)[N][4], const RowState& st, int tok_base,
+                                              const DecodeParams& p, int quad) {
+  if (p.softcap_log2 > 0.f) {
+    const float cap = p.softcap_log2, inv = p.inv_softcap_log2;
+    if (p.softcap <= kDirectCap) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = softcap_direct(x[n][i], cap, inv);
+    } else {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = softcap_log2(x[n][i], cap, inv);
+    }
+  }
+  if (p.alibi_slopes != nullptr) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+        x[n][i] = fmaf(-st.slope[i >> 1], fabsf((float)(st.pos[i >> 1] - tok)), x[n][i]);
+      }
+  }
+}
+
+// -inf for the keys a row does not see.
+template <int N>
+__device__ __forceinline__ void hide_keys(float (&x)[N][4], const RowState& st, int tok_base, int quad) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+      if (tok < st.first[i >> 1] || tok >= st.end[i >> 1]) x[n][i] = -INFINITY;
+    }
+}
+
+// Once a row's reference settles, alpha is exactly 1: the accumulator is only
+// rescaled when some row of the warp moved its reference.
+template <int D>
+__device__ __forceinline__ void rescale_rows(float (&o_acc)[D / 8][4], const float (&alpha)[2]) {
+  if (!__any_sync(0xffffffffu, (alpha[0] != 1.f) | (alpha[1] != 1.f))) return;
+#pragma unroll
+  for (int nd = 0; nd < D / 8; ++nd) {
+    o_acc[nd][0] *= alpha[0];
+    o_acc[nd][1] *= alpha[0];
+    o_acc[nd][2] *= alpha[1];
+    o_acc[nd][3] *= alpha[1];
+  }
+}
+
+__device__ __forceinline__ uint4 load_chunk(uint32_t addr) {
+  uint4 w;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(addr));
+  return w;
+}
+
+// Whether one of two 16-bit values (four codes) is not finite.
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  const uint32_t em = kSplitProbabilities<T>::value ? 0x7f80u : 0x7c00u;
+  return (w & em) == em || (w & (em << 16)) == (em << 16);
+}
+__device__ __forceinline__ bool nan4(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u; }
+
+// Mask of the 16-bit pair of tokens t, t + 1 of a unit: seen by some row and not
+// taken out of the MMA.
+__device__ __forceinline__ uint32_t keep_pair(int tok_base, int t, int tok_lo, int tok_hi, uint32_t odd_tokens) {
+  const int a = tok_base + t;
+  const bool k0 = a >= tok_lo && a < tok_hi && !((odd_tokens >> t) & 1u);
+  const bool k1 = a + 1 >= tok_lo && a + 1 < tok_hi && !((odd_tokens >> (t + 1)) & 1u);
+  return (k0 ? 0x0000ffffu : 0u) | (k1 ? 0xffff0000u : 0u);
+}
+
+// One 16-token unit of a 16-bit cache with changed scores.
 // tok_base: position of the unit's first token; tokens before tok_lo or at or
 // past tok_hi are seen by no row of the tile (their V may be anything); units
 // outside [full_lo, full_hi) hold keys that some row does not see.
-template <typename T, typename C, int D, bool kScored>
-__device__ __forceinline__ void attend_unit_ext(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
-                                                float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
-                                                int tok_hi, int full_lo, int full_hi, const float (&ks)[2],
-                                                const float (&vs)[2], const DecodeParams& p, int lane) {
-  constexpr bool k8 = kIs8<C>::value;
+template <typename T, int D>
+__device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
+                                                   float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
+                                                   int tok_hi, int full_lo, int full_hi, const DecodeParams& p,
+                                                   int lane) {
   constexpr int NDT = D / 8;
   const int quad = lane & 3;
 
   // ---- S = Q K^T ----
   float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-  if constexpr (k8) {
-    const int tok = ((lane >> 4) << 3) | (lane & 7);
-#pragma unroll
-    for (int kp = 0; kp < D / 32; ++kp) {
-      uint32_t r0, r1, r2, r3;  // tokens 0-7: k-steps 2kp, 2kp+1; tokens 8-15: the same
-      ldsm_x4(tile_chunk_addr<C, D>(kbase, tok, 2 * kp + ((lane >> 3) & 1)), r0, r1, r2, r3);
-      Mma16816<__half>::run(x[0], qa[2 * kp], e4m3x2_to_f16x2(r0), e4m3x2_to_f16x2(r0 >> 16));
-      Mma16816<__half>::run(x[1], qa[2 * kp], e4m3x2_to_f16x2(r2), e4m3x2_to_f16x2(r2 >> 16));
-      Mma16816<__half>::run(x[0], qa[2 * kp + 1], e4m3x2_to_f16x2(r1), e4m3x2_to_f16x2(r1 >> 16));
-      Mma16816<__half>::run(x[1], qa[2 * kp + 1], e4m3x2_to_f16x2(r3), e4m3x2_to_f16x2(r3 >> 16));
-    }
-  } else {
+  {
     const int tok = ((lane >> 4) << 3) | (lane & 7);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       uint32_t r0, r1, r2, r3;
-      ldsm_x4(tile_chunk_addr<C, D>(kbase, tok, 2 * kk + ((lane >> 3) & 1)), r0, r1, r2, r3);
+      ldsm_x4(tile_chunk_addr<T, D>(kbase, tok, 2 * kk + ((lane >> 3) & 1)), r0, r1, r2, r3);
       Mma16816<T>::run(x[0], qa[kk], r0, r1);
       Mma16816<T>::run(x[1], qa[kk], r2, r3);
     }
@@ -257,60 +332,21 @@ __device__ __forceinline__ void attend_unit_ext(uint32_t kbase, uint32_t vbase, 
 
   // ---- scores in the log2 domain ----
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const float c0 = k8 ? st.c[0] * ks[n] : st.c[0], c1 = k8 ? st.c[1] * ks[n] : st.c[1];
-    x[n][0] *= c0;
-    x[n][1] *= c0;
-    x[n][2] *= c1;
-    x[n][3] *= c1;
-  }
-  if constexpr (kScored) {
-    if (p.softcap_log2 > 0.f) {
+  for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = softcap_log2(x[n][i], p.softcap_log2, p.inv_softcap_log2);
-    }
-    if (p.alibi_slopes != nullptr) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
-          x[n][i] = fmaf(-st.slope[i >> 1], fabsf((float)(st.pos[i >> 1] - tok)), x[n][i]);
-        }
-    }
-  }
+    for (int i = 0; i < 4; ++i) x[n][i] *= st.c[i >> 1];
+  change_scores<2>(x, st, tok_base, p, quad);
   const bool boundary = tok_base < full_lo || tok_base + kUnitTokens > full_hi;
   uint32_t odd_tokens = 0;  // tokens of a boundary unit whose V row is not finite
   if (boundary) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
-        if (tok < st.first[i >> 1] || tok >= st.end[i >> 1]) x[n][i] = -INFINITY;
-      }
+    hide_keys<2>(x, st, tok_base, quad);
     // lane pair 2t, 2t+1 looks over V row t
     const int t = lane >> 1;
     bool odd = false;
-    constexpr int CH = D * (int)sizeof(C) / 16;  // 16-byte chunks of a row
 #pragma unroll
-    for (int ch = 0; ch < CH / 2; ++ch) {
-      uint32_t w0, w1, w2, w3;
-      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                   : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3)
-                   : "r"(tile_chunk_addr<C, D>(vbase, t, 2 * ch + (lane & 1))));
-      const uint32_t w[4] = {w0, w1, w2, w3};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (k8) {
-          odd |= __vcmpeq4(w[j] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u;
-        } else {
-          const uint32_t em = kSplitProbabilities<T>::value ? 0x7f80u : 0x7c00u;
-          odd |= (w[j] & em) == em || (w[j] & (em << 16)) == (em << 16);
-        }
-      }
+    for (int ch = 0; ch < D / 16; ++ch) {
+      const uint4 w = load_chunk(tile_chunk_addr<T, D>(vbase, t, 2 * ch + (lane & 1)));
+      odd |= not_finite2<T>(w.x) | not_finite2<T>(w.y) | not_finite2<T>(w.z) | not_finite2<T>(w.w);
     }
     const uint32_t pairs = __ballot_sync(0xffffffffu, odd && tok_base + t >= tok_lo && tok_base + t < tok_hi);
     const uint32_t either = pairs | (pairs >> 1);  // bit 2t: token t
@@ -322,106 +358,51 @@ __device__ __forceinline__ void attend_unit_ext(uint32_t kbase, uint32_t vbase, 
 
   // ---- online softmax ----
   float alpha[2], w[2][4];
-  const float lvs[2] = {k8 ? lg2(vs[0]) : 0.f, k8 ? lg2(vs[1]) : 0.f};
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
-    float mx[2];  // of tokens 0-7 and 8-15
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      mx[n] = fmaxf(x[n][2 * r], x[n][2 * r + 1]);
-      mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 1));
-      mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], 2));
-    }
-    const float mn = fmaxf(st.m[r], fmaxf(mx[0], mx[1]));
+    float mx = fmaxf(fmaxf(x[0][2 * r], x[0][2 * r + 1]), fmaxf(x[1][2 * r], x[1][2 * r + 1]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float mn = fmaxf(st.m[r], mx);
     const float base = mn == -INFINITY ? 0.f : mn;
-    const float a = ex2(st.m[r] - base);
-    float pr[4];
+    alpha[r] = ex2(st.m[r] - base);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) pr[i] = ex2(x[i >> 1][2 * r + (i & 1)] - base);
-    st.l[r] = st.l[r] * a + ((pr[0] + pr[1]) + (pr[2] + pr[3]));
+    for (int i = 0; i < 4; ++i) w[r][i] = ex2(x[i >> 1][2 * r + (i & 1)] - base);
+    st.l[r] = st.l[r] * alpha[r] + ((w[r][0] + w[r][1]) + (w[r][2] + w[r][3]));
     st.m[r] = mn;
-    if constexpr (k8) {
-      const float on = fmaxf(st.mo[r], fmaxf(mx[0] + lvs[0], mx[1] + lvs[1]));
-      const float obase = (on == -INFINITY ? 0.f : on) - 14.f;
-      alpha[r] = ex2(st.mo[r] - 14.f - obase);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float xi = x[i >> 1][2 * r + (i & 1)];
-        // a hidden score stays without weight even beside a scale that is not finite
-        w[r][i] = xi == -INFINITY ? 0.f : ex2(xi + (lvs[i >> 1] - obase));
-      }
-      st.mo[r] = on;
-    } else {
-      alpha[r] = a;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[r][i] = pr[i];
-    }
   }
-  if (__any_sync(0xffffffffu, (alpha[0] != 1.f) | (alpha[1] != 1.f))) {
-#pragma unroll
-    for (int nd = 0; nd < NDT; ++nd) {
-      o_acc[nd][0] *= alpha[0];
-      o_acc[nd][1] *= alpha[0];
-      o_acc[nd][2] *= alpha[1];
-      o_acc[nd][3] *= alpha[1];
-    }
-  }
+  rescale_rows<D>(o_acc, alpha);
 
   // ---- O += P V ----
-  using P = typename PvType<T, C>::type;
-  uint32_t pa[4] = {pack2<P>(w[0][0], w[0][1]), pack2<P>(w[1][0], w[1][1]), pack2<P>(w[0][2], w[0][3]),
-                    pack2<P>(w[1][2], w[1][3])};
-  constexpr bool kSplitP = !k8 && kSplitProbabilities<T>::value;
+  uint32_t pa[4] = {pack2<T>(w[0][0], w[0][1]), pack2<T>(w[1][0], w[1][1]), pack2<T>(w[0][2], w[0][3]),
+                    pack2<T>(w[1][2], w[1][3])};
+  constexpr bool kSplitP = kSplitProbabilities<T>::value;
   uint32_t plo[4] = {0u, 0u, 0u, 0u};
   if constexpr (kSplitP) {
-    plo[0] = pack2<P>(w[0][0] - lo_half<P>(pa[0]), w[0][1] - hi_half<P>(pa[0]));
-    plo[1] = pack2<P>(w[1][0] - lo_half<P>(pa[1]), w[1][1] - hi_half<P>(pa[1]));
-    plo[2] = pack2<P>(w[0][2] - lo_half<P>(pa[2]), w[0][3] - hi_half<P>(pa[2]));
-    plo[3] = pack2<P>(w[1][2] - lo_half<P>(pa[3]), w[1][3] - hi_half<P>(pa[3]));
+    plo[0] = pack2<T>(w[0][0] - lo_half<T>(pa[0]), w[0][1] - hi_half<T>(pa[0]));
+    plo[1] = pack2<T>(w[1][0] - lo_half<T>(pa[1]), w[1][1] - hi_half<T>(pa[1]));
+    plo[2] = pack2<T>(w[0][2] - lo_half<T>(pa[2]), w[0][3] - hi_half<T>(pa[2]));
+    plo[3] = pack2<T>(w[1][2] - lo_half<T>(pa[3]), w[1][3] - hi_half<T>(pa[3]));
   }
   uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
   if (boundary) {
-    uint32_t keep = 0;  // this lane's tokens 2 quad, +1, +8, +9
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int t = 2 * quad + (j & 1) + 8 * (j >> 1);
-      const bool k = tok_base + t >= tok_lo && tok_base + t < tok_hi && !((odd_tokens >> t) & 1u);
-      keep |= (uint32_t)k << j;
-    }
-    vm0 = ((keep & 1u) ? 0x0000ffffu : 0u) | ((keep & 2u) ? 0xffff0000u : 0u);
-    vm1 = ((keep & 4u) ? 0x0000ffffu : 0u) | ((keep & 8u) ? 0xffff0000u : 0u);
+    vm0 = keep_pair(tok_base, 2 * quad, tok_lo, tok_hi, odd_tokens);
+    vm1 = keep_pair(tok_base, 2 * quad + 8, tok_lo, tok_hi, odd_tokens);
   }
   const int tok = (((lane >> 3) & 1) << 3) | (lane & 7);
-  if constexpr (k8) {
 #pragma unroll
-    for (int c = 0; c < D / 16; c += 2) {
-      uint32_t r0, r1, r2, r3;  // chunk c: tokens 0-7, 8-15; chunk c + 1: the same
-      ldsm_x4_trans(tile_chunk_addr<C, D>(vbase, tok, c + (lane >> 4)), r0, r1, r2, r3);
-      const uint32_t r[4] = {r0, r1, r2, r3};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // bytes (token 2q: even, odd column; token 2q+1: even, odd) -> (even, even, odd, odd)
-        const uint32_t a = __byte_perm(r[2 * j], 0u, 0x3120), b = __byte_perm(r[2 * j + 1], 0u, 0x3120);
-        Mma16816<__half>::run(o_acc[2 * (c + j)], pa, e4m3x2_to_f16x2(a) & vm0, e4m3x2_to_f16x2(b) & vm1);
-        Mma16816<__half>::run(o_acc[2 * (c + j) + 1], pa, e4m3x2_to_f16x2(a >> 16) & vm0,
-                              e4m3x2_to_f16x2(b >> 16) & vm1);
-      }
-    }
-  } else {
-#pragma unroll
-    for (int nd = 0; nd < NDT; nd += 2) {
-      uint32_t v0, v1, v2, v3;
-      ldsm_x4_trans(tile_chunk_addr<C, D>(vbase, tok, nd + (lane >> 4)), v0, v1, v2, v3);
-      v0 &= vm0;
-      v1 &= vm1;
-      v2 &= vm0;
-      v3 &= vm1;
-      Mma16816<T>::run(o_acc[nd], pa, v0, v1);
-      Mma16816<T>::run(o_acc[nd + 1], pa, v2, v3);
-      if constexpr (kSplitP) {
-        Mma16816<T>::run(o_acc[nd], plo, v0, v1);
-        Mma16816<T>::run(o_acc[nd + 1], plo, v2, v3);
-      }
+  for (int nd = 0; nd < NDT; nd += 2) {
+    uint32_t v0, v1, v2, v3;
+    ldsm_x4_trans(tile_chunk_addr<T, D>(vbase, tok, nd + (lane >> 4)), v0, v1, v2, v3);
+    v0 &= vm0;
+    v1 &= vm1;
+    v2 &= vm0;
+    v3 &= vm1;
+    Mma16816<T>::run(o_acc[nd], pa, v0, v1);
+    Mma16816<T>::run(o_acc[nd + 1], pa, v2, v3);
+    if constexpr (kSplitP) {
+      Mma16816<T>::run(o_acc[nd], plo, v0, v1);
+      Mma16816<T>::run(o_acc[nd + 1], plo, v2, v3);
     }
   }
   // Tokens taken out above, for the rows that see them (rare: one is not finite).
@@ -438,40 +419,180 @@ __device__ __forceinline__ void attend_unit_ext(uint32_t kbase, uint32_t vbase, 
       for (int nd = 0; nd < NDT; ++nd)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          // column of element (nd, j) before end_piece_columns()
-          const int col = k8 ? (nd >> 1) * 16 + 4 * quad + 2 * j + (nd & 1) : nd * 8 + 2 * quad + j;
-          const uint32_t addr = tile_chunk_addr<C, D>(vbase, t, col * (int)sizeof(C) / 16) +
-                                (uint32_t)(col * (int)sizeof(C) % 16);
-          float v;
-          if constexpr (k8) {
-            uint32_t code;
-            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(addr));
-            v = lo_half<__half>(e4m3x2_to_f16x2(code));
-          } else {
-            unsigned short h;
-            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr));
-            v = lo_half<T>((uint32_t)h);
-          }
-          o_acc[nd][2 * r + j] = fmaf(wt, v, o_acc[nd][2 * r + j]);
+          const int col = nd * 8 + 2 * quad + j;
+          const uint32_t addr = tile_chunk_addr<T, D>(vbase, t, col / 8) + (uint32_t)(col % 8 * 2);
+          unsigned short h;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr));
+          o_acc[nd][2 * r + j] = fmaf(wt, lo_half<T>((uint32_t)h), o_acc[nd][2 * r + j]);
         }
     }
   }
 }
 
-// End of a piece of an 8-bit row: the accumulator back to the reference m, and
-// its columns in the order of frag_col().
-template <int D>
-__device__ __forceinline__ void end_piece_columns(float (&o_acc)[D / 8][4], const RowState& st) {
-  float f[2];
+// One 32-token unit of an 8-bit cache (parameters as above).  ks4 / vs4: the
+// scales of its four groups of 8 tokens.
+template <typename T, int D, bool kScored>
+__device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
+                                              float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
+                                              int tok_hi, int full_lo, int full_hi, const float4 ks4,
+                                              const float4 vs4, const DecodeParams& p, int lane) {
+  constexpr int NDT = D / 8;
+  const int quad = lane & 3;
+  const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w}, vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
+
+  // ---- S = Q K^T: n-tile n holds tokens 8n .. 8n + 7 ----
+  float x[4][4];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) f[r] = st.mo[r] == -INFINITY ? 0.f : ex2(st.mo[r] - 14.f - st.m[r]);
+  for (int n = 0; n < 4; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
+  {
+    const int tok = ((lane >> 4) << 3) | (lane & 7);
 #pragma unroll
-  for (int nd = 0; nd < D / 8; ++nd) {
-    o_acc[nd][0] *= f[0];
-    o_acc[nd][1] *= f[0];
-    o_acc[nd][2] *= f[1];
-    o_acc[nd][3] *= f[1];
+    for (int kp = 0; kp < D / 32; ++kp)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r0, r1, r2, r3;  // tokens 0-7: k-steps 2kp, 2kp+1; tokens 8-15: the same
+        ldsm_x4(tile_chunk_addr<e4m3_t, D>(kbase, tok + 16 * h, 2 * kp + ((lane >> 3) & 1)), r0, r1, r2, r3);
+        Mma16816<__half>::run(x[2 * h], qa[2 * kp], e4m3x2_to_f16x2(r0), e4m3x2_to_f16x2(r0 >> 16));
+        Mma16816<__half>::run(x[2 * h + 1], qa[2 * kp], e4m3x2_to_f16x2(r2), e4m3x2_to_f16x2(r2 >> 16));
+        Mma16816<__half>::run(x[2 * h], qa[2 * kp + 1], e4m3x2_to_f16x2(r1), e4m3x2_to_f16x2(r1 >> 16));
+        Mma16816<__half>::run(x[2 * h + 1], qa[2 * kp + 1], e4m3x2_to_f16x2(r3), e4m3x2_to_f16x2(r3 >> 16));
+      }
   }
+
+  // ---- scores in the log2 domain ----
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const float c0 = st.c[0] * ks[n], c1 = st.c[1] * ks[n];
+    x[n][0] *= c0;
+    x[n][1] *= c0;
+    x[n][2] *= c1;
+    x[n][3] *= c1;
+  }
+  if constexpr (kScored) change_scores<4>(x, st, tok_base, p, quad);
+  const bool boundary = tok_base < full_lo || tok_base + kUnit8Tokens > full_hi;
+  uint32_t odd_tokens = 0;  // tokens of a boundary unit whose V row is not finite
+  if (boundary) {
+    hide_keys<4>(x, st, tok_base, quad);
+    bool odd = false;  // lane t looks over V row t
+#pragma unroll
+    for (int ch = 0; ch < D / 16; ++ch) {
+      const uint4 w = load_chunk(tile_chunk_addr<e4m3_t, D>(vbase, lane, ch));
+      odd |= nan4(w.x) | nan4(w.y) | nan4(w.z) | nan4(w.w);
+    }
+    odd_tokens = __ballot_sync(0xffffffffu, odd && tok_base + lane >= tok_lo && tok_base + lane < tok_hi);
+  }
+
+  // ---- online softmax, weighted by the V scales ----
+  // (a comparison that NaN fails keeps a NaN scale's NaN)
+  float lvs[4], ivs[4];
+  constexpr float kLeast = 7.8886090522101181e-31f;  // 2^-100
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    lvs[n] = vs[n] < kLeast ? -100.f : lg2(vs[n]);
+    ivs[n] = (vs[n] < kLeast ? 1.2676506002282294e30f : rcp_approx(vs[n])) * 6.103515625e-05f;  // 2^-14 / vs
+  }
+  float alpha[2], w[2][8];
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) mx = fmaxf(mx, fmaxf(x[n][2 * r], x[n][2 * r + 1]) + lvs[n]);
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float mn = fmaxf(st.m[r], mx);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    alpha[r] = ex2(st.m[r] - base);
+    float l = st.l[r] * alpha[r];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const float off = lvs[n] - base + 14.f;
+      w[r][2 * n] = ex2(x[n][2 * r] + off);
+      w[r][2 * n + 1] = ex2(x[n][2 * r + 1] + off);
+    }
+    if (boundary) {
+      // a hidden score has no weight, and no part in the norm, beside any scale
+#pragma unroll
+      for (int n = 0; n < 4; ++n) {
+        if (x[n][2 * r] == -INFINITY) w[r][2 * n] = 0.f;
+        if (x[n][2 * r + 1] == -INFINITY) w[r][2 * n + 1] = 0.f;
+        const float g = w[r][2 * n] + w[r][2 * n + 1];
+        if (g != 0.f) l = fmaf(g, ivs[n], l);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) l = fmaf(w[r][2 * n] + w[r][2 * n + 1], ivs[n], l);
+    }
+    st.l[r] = l;
+    st.m[r] = mn;
+  }
+  rescale_rows<D>(o_acc, alpha);
+
+  // ---- O += P V: two k-steps of 16 tokens ----
+  uint32_t pa[2][4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    pa[h][0] = pack2<__half>(w[0][4 * h], w[0][4 * h + 1]);
+    pa[h][1] = pack2<__half>(w[1][4 * h], w[1][4 * h + 1]);
+    pa[h][2] = pack2<__half>(w[0][4 * h + 2], w[0][4 * h + 3]);
+    pa[h][3] = pack2<__half>(w[1][4 * h + 2], w[1][4 * h + 3]);
+  }
+  if (fminf(fminf(vs[0], vs[1]), fminf(vs[2], vs[3])) == 0.f) {  // a zero scale: values of 0
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (vs[n] == 0.f) pa[n >> 1][2 * (n & 1)] = pa[n >> 1][2 * (n & 1) + 1] = 0u;
+  }
+  uint32_t vm[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+  if (boundary) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) vm[n] = keep_pair(tok_base, 8 * n + 2 * quad, tok_lo, tok_hi, odd_tokens);
+  }
+  const int tok = (((lane >> 3) & 1) << 3) | (lane & 7);
+#pragma unroll
+  for (int c = 0; c < D / 16; c += 2)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t r[4];  // chunk c: tokens 0-7, 8-15; chunk c + 1: the same
+      ldsm_x4_trans(tile_chunk_addr<e4m3_t, D>(vbase, tok + 16 * h, c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // bytes (token 2q: even, odd column; token 2q+1: even, odd) -> (even, even, odd, odd)
+        const uint32_t a = __byte_perm(r[2 * j], 0u, 0x3120), b = __byte_perm(r[2 * j + 1], 0u, 0x3120);
+        Mma16816<__half>::run(o_acc[2 * (c + j)], pa[h], e4m3x2_to_f16x2(a) & vm[2 * h],
+                              e4m3x2_to_f16x2(b) & vm[2 * h + 1]);
+        Mma16816<__half>::run(o_acc[2 * (c + j) + 1], pa[h], e4m3x2_to_f16x2(a >> 16) & vm[2 * h],
+                              e4m3x2_to_f16x2(b >> 16) & vm[2 * h + 1]);
+      }
+    }
+  // Tokens taken out above, for the rows that see them (rare: a code is NaN).
+  while (odd_tokens) {
+    const int t = __ffs(odd_tokens) - 1;
+    odd_tokens &= odd_tokens - 1;
+    const int src = (lane & ~3) | ((t & 7) >> 1);  // the quad lane that holds column t
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const bool second = t & 1, g1 = t & 8, g2 = t & 16;
+      const float p0 = second ? w[r][1] : w[r][0], p1 = second ? w[r][3] : w[r][2];
+      const float p2 = second ? w[r][5] : w[r][4], p3 = second ? w[r][7] : w[r][6];
+      const float mine = g2 ? (g1 ? p3 : p2) : (g1 ? p1 : p0);
+      const float wt = __shfl_sync(0xffffffffu, mine, src);
+      if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
+#pragma unroll
+      for (int nd = 0; nd < NDT; ++nd)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int col = (nd >> 1) * 16 + 4 * quad + 2 * j + (nd & 1);  // before end_piece_columns()
+          const uint32_t addr = tile_chunk_addr<e4m3_t, D>(vbase, t, col / 16) + (uint32_t)(col % 16);
+          uint32_t code;
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(addr));
+          o_acc[nd][2 * r + j] = fmaf(wt, lo_half<__half>(e4m3x2_to_f16x2(code)), o_acc[nd][2 * r + j]);
+        }
+    }
+  }
+}
+
+// End of a piece of an 8-bit row: its columns in the order of frag_col().
+template <int D>
+__device__ __forceinline__ void end_piece_columns(float (&o_acc)[D / 8][4]) {
 #pragma unroll
   for (int nd = 0; nd < D / 8; nd += 2)
 #pragma unroll
@@ -484,8 +605,10 @@ __device__ __forceinline__ void end_piece_columns(float (&o_acc)[D / 8][4], cons
 
 // 1 / l of a finished row.  A row without weight is zero when it sees no key, and
 // NaN (0 / 0) when all its scores are -inf; so is one whose sum is NaN.
+template <typename KV>
 __device__ __forceinline__ float row_norm(float l, bool sees_a_key) {
-  return l > 0.f ? 1.f / l : (l == 0.f && !sees_a_key) ? 0.f : __int_as_float(0x7fffffff);
+  constexpr float lift = kIs8<KV>::value ? 6.103515625e-05f : 1.f;  // the weights' 2^14, which only the sum carries
+  return l > 0.f ? 1.f / l * lift : (l == 0.f && !sees_a_key) ? 0.f : __int_as_float(0x7fffffff);
 }
 
 // store_rows with the norms inv0 / inv1 and the columns of frag_col<KV>().
