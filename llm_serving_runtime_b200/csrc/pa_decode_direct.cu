@@ -187,11 +187,11 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     phase ^= 1u << slot;
     const uint32_t kbase = ring + (uint32_t)slot * STAGE_BYTES;
     if constexpr (k8)
-      attend_unit_8<T, D, kScored>(kbase, kbase + TILE_BYTES, qa, o_acc, st, u * UT, tok_lo, tok_hi, full_lo, full_hi,
+      attend_unit_8<T, D, kScored, true>(kbase, kbase + TILE_BYTES, qa, o_acc, st, u * UT, tok_lo, tok_hi, full_lo, full_hi,
                                    s_scales[2 * (warp * stages + slot)], s_scales[2 * (warp * stages + slot) + 1], p,
                                    lane);
     else
-      attend_unit_scored<T, D>(kbase, kbase + TILE_BYTES, qa, o_acc, st, u * UT, tok_lo, tok_hi, full_lo, full_hi, p,
+      attend_unit_scored<T, D, true>(kbase, kbase + TILE_BYTES, qa, o_acc, st, u * UT, tok_lo, tok_hi, full_lo, full_hi, p,
                                lane);
     __syncwarp();
     if (next < w1) {
@@ -203,7 +203,6 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
 
   // ---- the CTA's state: (m, l, acc) of eight warps, acc in each warp's own ring ----
-  if constexpr (k8) end_piece_columns<D>(o_acc);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     float l = st.l[r] + __shfl_xor_sync(0xffffffffu, st.l[r], 1);
@@ -216,7 +215,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   float* acc = reinterpret_cast<float*>(smem + (size_t)(warp * stages) * STAGE_BYTES);
 #pragma unroll
   for (int nd = 0; nd < D / 8; ++nd) {
-    const int d = frag_col<KV>(nd, quad);
+    const int d = nd * 8 + 2 * quad;
     *reinterpret_cast<float2*>(acc + (lane >> 2) * D + d) = make_float2(o_acc[nd][0], o_acc[nd][1]);
     *reinterpret_cast<float2*>(acc + ((lane >> 2) + 8) * D + d) = make_float2(o_acc[nd][2], o_acc[nd][3]);
   }

@@ -810,11 +810,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
     // ---- QK^T, masked online softmax, PV on tensor cores ----
     if constexpr (kExt) {
       if constexpr (k8)
-        attend_unit_8<T, D, kScored>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi,
+        attend_unit_8<T, D, kScored, true>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi,
                                      s_scales[2 * (warp * stages + slot)], s_scales[2 * (warp * stages + slot) + 1],
                                      p, lane);
       else
-        attend_unit_scored<T, D>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi, p,
+        attend_unit_scored<T, D, true>(kbase, vbase, qa, o_acc, st, unit_token(cc), tok_lo, tok_hi, full_lo, full_hi, p,
                                  lane);
     } else {
       attend_unit<T, D>(kbase, vbase, qa, o_acc, m0, m1, l0, l1, unit_token(cc), L, lim0, lim1, mask_from,
@@ -835,7 +835,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
     if (row_end || cf + 1 == we) {
       if constexpr (kExt) {
         m0 = st.m[0], m1 = st.m[1], l0 = st.l[0], l1 = st.l[1];
-        if constexpr (k8) end_piece_columns<D>(o_acc);
       }
       float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
       float lt1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
@@ -863,7 +862,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
           const long long ridx1 = (rb + qa1 % p.G) * p.q_len + qa1 / p.G;
           store_rows_folded<T, D>(op0, op1, o_acc, mm0, mm1, ll0, ll1, ridx0, ridx1, p, quad);
         } else if constexpr (kExt) {
-          store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm<KV>(ll0, st.first[0] < st.end[0]),
+          store_rows_ext<T, D>(op0, op1, o_acc, row_norm<KV>(ll0, st.first[0] < st.end[0]),
                                    row_norm<KV>(ll1, st.first[1] < st.end[1]), quad, p.Dv);
         } else {
           store_rows<T, D>(op0, op1, o_acc, ll0, ll1, quad, p.Dv);
@@ -889,7 +888,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
         float* so = sl + 2 * p.slot_rows;
 #pragma unroll
         for (int nd = 0; nd < NDT; ++nd) {
-          const int d = frag_col<KV>(nd, quad);
+          const int d = nd * 8 + 2 * quad;
           if (r0_ok)
             *reinterpret_cast<float2*>(so + qrow0 * D + d) = make_float2(o_acc[nd][0], o_acc[nd][1]);
           if (r1_ok)
@@ -958,7 +957,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
                 const float* so = slot_ptr(i) + 2 * p.slot_rows;
 #pragma unroll
                 for (int nd = 0; nd < NDT; ++nd) {
-                  const int d = frag_col<KV>(nd, quad);
+                  const int d = nd * 8 + 2 * quad;
                   const float2 a0 = r0_ok ? __ldcg(reinterpret_cast<const float2*>(so + qrow0 * D + d))
                                           : make_float2(0.f, 0.f);
                   const float2 a1 = r1_ok ? __ldcg(reinterpret_cast<const float2*>(so + (qrow0 + 8) * D + d))

@@ -243,10 +243,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
       const int tok0 = (u_first + u) * UT;
       if (tok0 < tok_hi && tok0 + UT > tok_lo) {  // some row of the warp sees some key of the unit
         if constexpr (k8)
-          attend_unit_8<T, D, kScored>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo,
+          attend_unit_8<T, D, kScored, false>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo,
                                        full_hi, s_scales[2 * slot], s_scales[2 * slot + 1], p, lane);
         else
-          attend_unit_scored<T, D>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo, full_hi,
+          attend_unit_scored<T, D, false>(kbase, kbase + TILE_BYTES, qa, o_acc, st, tok0, tok_lo, tok_hi, full_lo, full_hi,
                                    p, lane);
       }
     } else if (u < n_w) {
@@ -258,13 +258,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1)
   }
 
   if constexpr (kExt) l0 = st.l[0], l1 = st.l[1];
-  if constexpr (k8) end_piece_columns<D>(o_acc);
   float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
   float lt1 = l1 + __shfl_xor_sync(0xffffffffu, l1, 1);
   lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
   lt1 += __shfl_xor_sync(0xffffffffu, lt1, 2);
   if constexpr (kExt)
-    store_rows_ext<T, KV, D>(op0, op1, o_acc, row_norm<KV>(lt0, st.first[0] < st.end[0]),
+    store_rows_ext<T, D>(op0, op1, o_acc, row_norm<KV>(lt0, st.first[0] < st.end[0]),
                              row_norm<KV>(lt1, st.first[1] < st.end[1]), quad, p.Dv);
   else
     store_rows<T, D>(op0, op1, o_acc, lt0, lt1, quad, p.Dv);

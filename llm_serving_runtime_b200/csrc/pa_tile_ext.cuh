@@ -10,13 +10,15 @@
 //
 // 8-bit caches (attend_unit_8, 32 tokens at a time).  k_j = ks * c_j and v_j =
 // vs * d_j with codes c, d and the block's scales ks, vs.  Codes widen to fp16
-// without rounding, so both products run as fp16 MMAs whatever the query's type;
-// ks multiplies the finished dot product.  A bf16 query row is brought to fp16 by
-// a power of two of its own that puts its largest element into [2^14, 2^15): 8-bit
-// significands fit fp16's 11, and only elements 2^29 below the row's largest lose
-// bits.  vs goes into the weights, and the running reference is that of the
-// weighted values:
-//   m = max_j (x_j + log2 vs_j),  w_j = 2^(x_j + log2 vs_j - m + 14)
+// without rounding, so both products run as fp16 MMAs whatever the query's type
+// (mma.sync has no 8-bit float unit here: an e4m3 MMA expands to two fp16 ones and
+// ten conversions, measured 0.17 a clock against 0.40 for fp16); ks multiplies the
+// finished dot product.  A bf16 query row is brought to fp16 by a power of two of
+// its own that puts its largest element into [2^14, 2^15): 8-bit significands fit
+// fp16's 11, and only elements 2^29 below the row's largest lose bits.  V comes
+// out of a byte transpose (ldmatrix b8).  vs goes into the weights, and the running
+// reference is that of the weighted values:
+//   m = max_j (x_j + log2 vs_j) - 14,  w_j = 2^(x_j + log2 vs_j - m)
 //   out = sum_j w_j d_j / (2^14 sum_j 2^-14 w_j / vs_j)
 // so a block of large scale and little weight cannot push the others' weights
 // out of fp16's range, and one exponential serves both sums.  w is rounded to
@@ -25,8 +27,9 @@
 // least 2^-100 (the append writes no smaller ones).
 //
 // What a mask hides never reaches a row: hidden scores are -inf whatever K
-// holds, and where rows of one tile see different keys, tokens whose V row is
-// not finite are taken out of the MMA (0 * inf) and added row by row.
+// holds, and in units where rows see different keys (or none), V rows that are not
+// finite (0 * inf) are added row by row and then, like rows nobody sees, zeroed in
+// shared memory before the MMA (or masked out of it where other warps read the tile).
 #pragma once
 
 #include <limits.h>
@@ -42,23 +45,32 @@ struct e4m3_t {
   uint8_t bits;
 };
 
+template <bool b>
+struct Bool {
+  static constexpr bool value = b;
+};
+
 template <typename C>
 struct kIs8 {
   static constexpr bool value = sizeof(C) == 1;
 };
 
-// Two e4m3 codes (bits 0-7, 8-15) to two fp16 values, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+// Two e4m3 codes (bits 0-15, or 16-31) to two fp16 values, exactly.
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t codes) {
   uint32_t d;
-  const unsigned short h = (unsigned short)two;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(h));
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(d) : "r"(codes));
+  return d;
+}
+__device__ __forceinline__ uint32_t e4m3x2_hi_to_f16x2(uint32_t codes) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, hi;\n\t}" : "=r"(d) : "r"(codes));
   return d;
 }
 
-// log2 (approximate instruction; exact powers of two come out as integers).
+// log2 (approximate instruction).
 __device__ __forceinline__ float lg2(float x) {
   float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -97,16 +109,10 @@ __device__ __forceinline__ uint32_t tile_chunk_addr(uint32_t base, int tok, int 
     return base + (uint32_t)tok * 64u + ((uint32_t)(chunk ^ ((tok >> 1) & 3)) << 4);
 }
 
-// Output column of accumulator element (nd, 0) of a lane (element 1 is the next
-// column) once a piece has ended.  8-bit tiles come out of the byte transpose
-// with even and odd columns in separate n-tiles; end_piece_columns() pairs them.
-template <typename C>
-__device__ __forceinline__ int frag_col(int nd, int quad) {
-  if constexpr (kIs8<C>::value)
-    return (nd >> 1) * 16 + 4 * quad + 2 * (nd & 1);
-  else
-    return nd * 8 + 2 * quad;
-}
+// tile_chunk_addr() of a lane's chunk c ^ i for even i (c: the lane's own, 0 or 1 more
+// than an even one) is this with i << 4 exchanged: tiles are aligned to
+// the swizzle, so the chunk is a field of the address.
+__device__ __forceinline__ uint32_t flip_chunk(uint32_t addr, int i) { return addr ^ ((uint32_t)i << 4); }
 
 // Running state of a warp's rows lane/4 (index 0) and lane/4 + 8 (index 1).
 struct RowState {
@@ -227,8 +233,18 @@ __device__ __forceinline__ float softcap_log2(float x, float cap, float inv_cap)
   return fabsf(y) > 0.25f ? softcap_direct(x, cap, inv_cap) : x * p;
 }
 
+// Token (within a unit) of a lane's element i of n-tile n.  The two n-tiles of an
+// 8-bit unit's 16 tokens follow the order in which ldmatrix b8 hands out V's rows,
+// chosen so that neither K's nor V's loads conflict (see v_row_8): the second
+// tile's halves are exchanged.
+template <bool k8>
+__device__ __forceinline__ int frag_token(int n, int i, int quad) {
+  const int c = 2 * quad + (i & 1);
+  return n * 8 + (k8 && (n & 1) ? c ^ 4 : c);
+}
+
 // Capped and biased scores of n-tiles of 8 tokens (log2 domain).
-template <int N>
+template <int N, bool k8>
 __device__ __forceinline__ void change_scores(float (&x)[N][4], const RowState& st, int tok_base,
                                               const DecodeParams& p, int quad) {
   if (p.softcap_log2 > 0.f) {
@@ -250,20 +266,20 @@ __device__ __forceinline__ void change_scores(float (&x)[N][4], const RowState& 
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+        const int tok = tok_base + frag_token<k8>(n, i, quad);
         x[n][i] = fmaf(-st.slope[i >> 1], fabsf((float)(st.pos[i >> 1] - tok)), x[n][i]);
       }
   }
 }
 
 // -inf for the keys a row does not see.
-template <int N>
+template <int N, bool k8>
 __device__ __forceinline__ void hide_keys(float (&x)[N][4], const RowState& st, int tok_base, int quad) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int tok = tok_base + n * 8 + 2 * quad + (i & 1);
+      const int tok = tok_base + frag_token<k8>(n, i, quad);
       if (tok < st.first[i >> 1] || tok >= st.end[i >> 1]) x[n][i] = -INFINITY;
     }
 }
@@ -296,20 +312,23 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 }
 __device__ __forceinline__ bool nan4(uint32_t w) { return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u; }
 
-// Mask of the 16-bit pair of tokens t, t + 1 of a unit: seen by some row and not
-// taken out of the MMA.
-__device__ __forceinline__ uint32_t keep_pair(int tok_base, int t, int tok_lo, int tok_hi, uint32_t odd_tokens) {
-  const int a = tok_base + t;
-  const bool k0 = a >= tok_lo && a < tok_hi && !((odd_tokens >> t) & 1u);
-  const bool k1 = a + 1 >= tok_lo && a + 1 < tok_hi && !((odd_tokens >> (t + 1)) & 1u);
-  return (k0 ? 0x0000ffffu : 0u) | (k1 ? 0xffff0000u : 0u);
+// Mask of a register of two 16-bit values, tokens t and t + 1 of a unit whose
+// dropped tokens are the set bits.
+__device__ __forceinline__ uint32_t keep_pair(uint32_t dropped, int t) {
+  return (((dropped >> t) & 1u) ? 0u : 0x0000ffffu) | (((dropped >> t) & 2u) ? 0u : 0xffff0000u);
+}
+
+__device__ __forceinline__ void zero_chunk(uint32_t addr) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0u) : "memory");
 }
 
 // One 16-token unit of a 16-bit cache with changed scores.
 // tok_base: position of the unit's first token; tokens before tok_lo or at or
 // past tok_hi are seen by no row of the tile (their V may be anything); units
-// outside [full_lo, full_hi) hold keys that some row does not see.
-template <typename T, int D>
+// outside [full_lo, full_hi) hold keys that some row does not see.  kOwnTile: no
+// other warp reads the tile, so rows to be left out can be zeroed in place; else
+// their registers are masked.
+template <typename T, int D, bool kOwnTile>
 __device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
                                                    float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
                                                    int tok_hi, int full_lo, int full_hi, const DecodeParams& p,
@@ -321,10 +340,11 @@ __device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbas
   float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
   {
     const int tok = ((lane >> 4) << 3) | (lane & 7);
+    const uint32_t at = tile_chunk_addr<T, D>(kbase, tok, (lane >> 3) & 1);
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       uint32_t r0, r1, r2, r3;
-      ldsm_x4(tile_chunk_addr<T, D>(kbase, tok, 2 * kk + ((lane >> 3) & 1)), r0, r1, r2, r3);
+      ldsm_x4(flip_chunk(at, (2 * kk) & 7) + (kk >> 2) * TileLayout<T, D>::kHalfBytes, r0, r1, r2, r3);
       Mma16816<T>::run(x[0], qa[kk], r0, r1);
       Mma16816<T>::run(x[1], qa[kk], r2, r3);
     }
@@ -335,26 +355,9 @@ __device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbas
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[n][i] *= st.c[i >> 1];
-  change_scores<2>(x, st, tok_base, p, quad);
+  change_scores<2, false>(x, st, tok_base, p, quad);
   const bool boundary = tok_base < full_lo || tok_base + kUnitTokens > full_hi;
-  uint32_t odd_tokens = 0;  // tokens of a boundary unit whose V row is not finite
-  if (boundary) {
-    hide_keys<2>(x, st, tok_base, quad);
-    // lane pair 2t, 2t+1 looks over V row t
-    const int t = lane >> 1;
-    bool odd = false;
-#pragma unroll
-    for (int ch = 0; ch < D / 16; ++ch) {
-      const uint4 w = load_chunk(tile_chunk_addr<T, D>(vbase, t, 2 * ch + (lane & 1)));
-      odd |= not_finite2<T>(w.x) | not_finite2<T>(w.y) | not_finite2<T>(w.z) | not_finite2<T>(w.w);
-    }
-    const uint32_t pairs = __ballot_sync(0xffffffffu, odd && tok_base + t >= tok_lo && tok_base + t < tok_hi);
-    const uint32_t either = pairs | (pairs >> 1);  // bit 2t: token t
-    if (either & 0x55555555u) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) odd_tokens |= ((either >> (2 * j)) & 1u) << j;
-    }
-  }
+  if (boundary) hide_keys<2, false>(x, st, tok_base, quad);
 
   // ---- online softmax ----
   float alpha[2], w[2][4];
@@ -373,6 +376,54 @@ __device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbas
   }
   rescale_rows<D>(o_acc, alpha);
 
+  [[maybe_unused]] uint32_t dropped = 0;  // tokens left out of the MMA
+  if (boundary) {
+    // Lane pair 2t, 2t+1 looks over V row t.
+    const int t = lane >> 1;
+    const bool seen = tok_base + t >= tok_lo && tok_base + t < tok_hi;
+    bool odd = false;
+#pragma unroll
+    for (int ch = 0; ch < D / 16; ++ch) {
+      const uint4 v = load_chunk(tile_chunk_addr<T, D>(vbase, t, 2 * ch + (lane & 1)));
+      odd |= not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w);
+    }
+    const uint32_t pairs = __ballot_sync(0xffffffffu, odd && seen);
+    uint32_t left = (pairs | (pairs >> 1)) & 0x55555555u;  // bit 2t: token t
+    const uint32_t drop = __ballot_sync(0xffffffffu, !seen) | left | (left << 1);
+    while (left) {
+      const int to = (__ffs(left) - 1) >> 1;
+      left &= left - 1;
+      const int src = (lane & ~3) | ((to & 7) >> 1);  // the quad lane that holds column to
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float lo = (to >> 3) ? w[r][2] : w[r][0], hi = (to >> 3) ? w[r][3] : w[r][1];
+        const float wt = __shfl_sync(0xffffffffu, (to & 1) ? hi : lo, src);
+        if (tok_base + to < st.first[r] || tok_base + to >= st.end[r]) continue;
+#pragma unroll
+        for (int nd = 0; nd < NDT; ++nd)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = nd * 8 + 2 * quad + j;
+            const uint32_t addr = tile_chunk_addr<T, D>(vbase, to, col / 8) + (uint32_t)(col % 8 * 2);
+            unsigned short h;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr) : "memory");
+            o_acc[nd][2 * r + j] = fmaf(wt, lo_half<T>((uint32_t)h), o_acc[nd][2 * r + j]);
+          }
+      }
+    }
+    if constexpr (kOwnTile) {
+      __syncwarp();
+      if ((drop >> lane) & 1u) {
+#pragma unroll
+        for (int ch = 0; ch < D / 16; ++ch) zero_chunk(tile_chunk_addr<T, D>(vbase, t, 2 * ch + (lane & 1)));
+      }
+      __syncwarp();
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) dropped |= ((drop >> (2 * j)) & 1u) << j;
+    }
+  }
+
   // ---- O += P V ----
   uint32_t pa[4] = {pack2<T>(w[0][0], w[0][1]), pack2<T>(w[1][0], w[1][1]), pack2<T>(w[0][2], w[0][3]),
                     pack2<T>(w[1][2], w[1][3])};
@@ -384,54 +435,64 @@ __device__ __forceinline__ void attend_unit_scored(uint32_t kbase, uint32_t vbas
     plo[2] = pack2<T>(w[0][2] - lo_half<T>(pa[2]), w[0][3] - hi_half<T>(pa[2]));
     plo[3] = pack2<T>(w[1][2] - lo_half<T>(pa[3]), w[1][3] - hi_half<T>(pa[3]));
   }
-  uint32_t vm0 = 0xffffffffu, vm1 = 0xffffffffu;
-  if (boundary) {
-    vm0 = keep_pair(tok_base, 2 * quad, tok_lo, tok_hi, odd_tokens);
-    vm1 = keep_pair(tok_base, 2 * quad + 8, tok_lo, tok_hi, odd_tokens);
-  }
-  const int tok = (((lane >> 3) & 1) << 3) | (lane & 7);
+  const uint32_t vat = tile_chunk_addr<T, D>(vbase, (((lane >> 3) & 1) << 3) | (lane & 7), lane >> 4);
+  auto pv = [&](auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
+    const uint32_t vm0 = kMasked ? keep_pair(dropped, 2 * quad) : 0u;
+    const uint32_t vm1 = kMasked ? keep_pair(dropped, 2 * quad + 8) : 0u;
 #pragma unroll
-  for (int nd = 0; nd < NDT; nd += 2) {
-    uint32_t v0, v1, v2, v3;
-    ldsm_x4_trans(tile_chunk_addr<T, D>(vbase, tok, nd + (lane >> 4)), v0, v1, v2, v3);
-    v0 &= vm0;
-    v1 &= vm1;
-    v2 &= vm0;
-    v3 &= vm1;
-    Mma16816<T>::run(o_acc[nd], pa, v0, v1);
-    Mma16816<T>::run(o_acc[nd + 1], pa, v2, v3);
-    if constexpr (kSplitP) {
-      Mma16816<T>::run(o_acc[nd], plo, v0, v1);
-      Mma16816<T>::run(o_acc[nd + 1], plo, v2, v3);
+    for (int nd = 0; nd < NDT; nd += 2) {
+      uint32_t v0, v1, v2, v3;
+      ldsm_x4_trans(flip_chunk(vat, nd & 7) + (nd >> 3) * TileLayout<T, D>::kHalfBytes, v0, v1, v2, v3);
+      if constexpr (kMasked) v0 &= vm0, v1 &= vm1, v2 &= vm0, v3 &= vm1;
+      Mma16816<T>::run(o_acc[nd], pa, v0, v1);
+      Mma16816<T>::run(o_acc[nd + 1], pa, v2, v3);
+      if constexpr (kSplitP) {
+        Mma16816<T>::run(o_acc[nd], plo, v0, v1);
+        Mma16816<T>::run(o_acc[nd + 1], plo, v2, v3);
+      }
     }
-  }
-  // Tokens taken out above, for the rows that see them (rare: one is not finite).
-  while (odd_tokens) {
-    const int t = __ffs(odd_tokens) - 1;
-    odd_tokens &= odd_tokens - 1;
-    const int src = (lane & ~3) | ((t & 7) >> 1);  // the quad lane that holds column t
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float lo = (t >> 3) ? w[r][2] : w[r][0], hi = (t >> 3) ? w[r][3] : w[r][1];
-      const float wt = __shfl_sync(0xffffffffu, (t & 1) ? hi : lo, src);
-      if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
-#pragma unroll
-      for (int nd = 0; nd < NDT; ++nd)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = nd * 8 + 2 * quad + j;
-          const uint32_t addr = tile_chunk_addr<T, D>(vbase, t, col / 8) + (uint32_t)(col % 8 * 2);
-          unsigned short h;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(addr));
-          o_acc[nd][2 * r + j] = fmaf(wt, lo_half<T>((uint32_t)h), o_acc[nd][2 * r + j]);
-        }
-    }
-  }
+  };
+  if (kOwnTile || !boundary)
+    pv(Bool<false>{});
+  else
+    pv(Bool<true>{});
+}
+
+// m16n8k16 fp16 MMA on a zero accumulator.
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Two transposed 16 x 16 byte matrices, row addresses from lanes 0-15 and 16-31.
+// A lane gets bytes (rows 4 (lane % 4) .. + 3, column lane / 4) and the same of
+// column lane / 4 + 8 of each.
+__device__ __forceinline__ void ldsm_b8_x2_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
+                                                 uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr)
+               : "memory");
+}
+
+// Token (of 16) that V's matrix row i holds.  A lane's four bytes are rows 4q ..
+// 4q + 3; with i = (q1, q0, j, e) in bits, bytes 0, 1 (j = 0) become the B operand's
+// first register, whose k are columns 2q, 2q + 1 of the first score tile, bytes 2, 3
+// (j = 1) the second.  Tokens 8 j + 4 (q1 ^ j) + 2 q0 + e: any 8 rows loaded
+// together (fixed q1), and any 8 of a score tile (fixed j), differ modulo 8, which
+// is what the swizzles keep apart.
+__device__ __forceinline__ int v_row_8(int i) {
+  const int e = i & 1, j = (i >> 1) & 1, q0 = (i >> 2) & 1, q1 = (i >> 3) & 1;
+  return 8 * j + 4 * (q1 ^ j) + 2 * q0 + e;
 }
 
 // One 32-token unit of an 8-bit cache (parameters as above).  ks4 / vs4: the
 // scales of its four groups of 8 tokens.
-template <typename T, int D, bool kScored>
+template <typename T, int D, bool kScored, bool kOwnTile>
 __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, const uint32_t (&qa)[D / 16][4],
                                               float (&o_acc)[D / 8][4], RowState& st, int tok_base, int tok_lo,
                                               int tok_hi, int full_lo, int full_hi, const float4 ks4,
@@ -440,22 +501,27 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
   const int quad = lane & 3;
   const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w}, vs[4] = {vs4.x, vs4.y, vs4.z, vs4.w};
 
-  // ---- S = Q K^T: n-tile n holds tokens 8n .. 8n + 7 ----
+  // ---- S = Q K^T: n-tile n holds tokens 8n .. 8n + 7 (frag_token) ----
   float x[4][4];
-#pragma unroll
-  for (int n = 0; n < 4; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
   {
-    const int tok = ((lane >> 4) << 3) | (lane & 7);
+    // matrices: (tile 0, chunk 2kp), (0, 2kp + 1), (1, 2kp), (1, 2kp + 1)
+    const int second = lane >> 4;
+    const int tok = 8 * second + ((lane & 7) ^ (4 * second));
+    const uint32_t at = tile_chunk_addr<e4m3_t, D>(kbase, tok, (lane >> 3) & 1);
 #pragma unroll
     for (int kp = 0; kp < D / 32; ++kp)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t r0, r1, r2, r3;  // tokens 0-7: k-steps 2kp, 2kp+1; tokens 8-15: the same
-        ldsm_x4(tile_chunk_addr<e4m3_t, D>(kbase, tok + 16 * h, 2 * kp + ((lane >> 3) & 1)), r0, r1, r2, r3);
-        Mma16816<__half>::run(x[2 * h], qa[2 * kp], e4m3x2_to_f16x2(r0), e4m3x2_to_f16x2(r0 >> 16));
-        Mma16816<__half>::run(x[2 * h + 1], qa[2 * kp], e4m3x2_to_f16x2(r2), e4m3x2_to_f16x2(r2 >> 16));
-        Mma16816<__half>::run(x[2 * h], qa[2 * kp + 1], e4m3x2_to_f16x2(r1), e4m3x2_to_f16x2(r1 >> 16));
-        Mma16816<__half>::run(x[2 * h + 1], qa[2 * kp + 1], e4m3x2_to_f16x2(r3), e4m3x2_to_f16x2(r3 >> 16));
+        uint32_t r[4];
+        ldsm_x4(flip_chunk(at, 2 * kp) + 16u * h * TileLayout<e4m3_t, D>::kRowBytes, r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b0 = e4m3x2_to_f16x2(r[j]), b1 = e4m3x2_hi_to_f16x2(r[j]);
+          if (kp == 0 && (j & 1) == 0)
+            mma_f16_first(x[2 * h + (j >> 1)], qa[0], b0, b1);
+          else
+            Mma16816<__half>::run(x[2 * h + (j >> 1)], qa[2 * kp + (j & 1)], b0, b1);
+        }
       }
   }
 
@@ -468,19 +534,9 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
     x[n][2] *= c1;
     x[n][3] *= c1;
   }
-  if constexpr (kScored) change_scores<4>(x, st, tok_base, p, quad);
+  if constexpr (kScored) change_scores<4, true>(x, st, tok_base, p, quad);
   const bool boundary = tok_base < full_lo || tok_base + kUnit8Tokens > full_hi;
-  uint32_t odd_tokens = 0;  // tokens of a boundary unit whose V row is not finite
-  if (boundary) {
-    hide_keys<4>(x, st, tok_base, quad);
-    bool odd = false;  // lane t looks over V row t
-#pragma unroll
-    for (int ch = 0; ch < D / 16; ++ch) {
-      const uint4 w = load_chunk(tile_chunk_addr<e4m3_t, D>(vbase, lane, ch));
-      odd |= nan4(w.x) | nan4(w.y) | nan4(w.z) | nan4(w.w);
-    }
-    odd_tokens = __ballot_sync(0xffffffffu, odd && tok_base + lane >= tok_lo && tok_base + lane < tok_hi);
-  }
+  if (boundary) hide_keys<4, true>(x, st, tok_base, quad);
 
   // ---- online softmax, weighted by the V scales ----
   // (a comparison that NaN fails keeps a NaN scale's NaN)
@@ -499,33 +555,83 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
     for (int n = 0; n < 4; ++n) mx = fmaxf(mx, fmaxf(x[n][2 * r], x[n][2 * r + 1]) + lvs[n]);
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const float mn = fmaxf(st.m[r], mx);
+    const float mn = fmaxf(st.m[r], mx - 14.f);  // the reference, lowered so that weights reach 2^14
     const float base = mn == -INFINITY ? 0.f : mn;
     alpha[r] = ex2(st.m[r] - base);
-    float l = st.l[r] * alpha[r];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-      const float off = lvs[n] - base + 14.f;
+      const float off = lvs[n] - base;
       w[r][2 * n] = ex2(x[n][2 * r] + off);
       w[r][2 * n + 1] = ex2(x[n][2 * r + 1] + off);
     }
-    if (boundary) {
-      // a hidden score has no weight, and no part in the norm, beside any scale
+    st.l[r] *= alpha[r];
+    st.m[r] = mn;
+  }
+  rescale_rows<D>(o_acc, alpha);
+
+  [[maybe_unused]] uint32_t dropped = 0;  // tokens left out of the MMA
+  if (!boundary) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      st.l[0] = fmaf(w[0][2 * n] + w[0][2 * n + 1], ivs[n], st.l[0]);
+      st.l[1] = fmaf(w[1][2 * n] + w[1][2 * n + 1], ivs[n], st.l[1]);
+    }
+  } else {
+    // a hidden score has no weight, and no part in the norm, beside any scale
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
         if (x[n][2 * r] == -INFINITY) w[r][2 * n] = 0.f;
         if (x[n][2 * r + 1] == -INFINITY) w[r][2 * n + 1] = 0.f;
         const float g = w[r][2 * n] + w[r][2 * n + 1];
-        if (g != 0.f) l = fmaf(g, ivs[n], l);
+        if (g != 0.f) st.l[r] = fmaf(g, ivs[n], st.l[r]);
       }
-    } else {
+    // Lane t looks over V row t.
+    const bool seen = tok_base + lane >= tok_lo && tok_base + lane < tok_hi;
+    bool odd = false;
 #pragma unroll
-      for (int n = 0; n < 4; ++n) l = fmaf(w[r][2 * n] + w[r][2 * n + 1], ivs[n], l);
+    for (int ch = 0; ch < D / 16; ++ch) {
+      const uint4 v = load_chunk(tile_chunk_addr<e4m3_t, D>(vbase, lane, ch));
+      odd |= nan4(v.x) | nan4(v.y) | nan4(v.z) | nan4(v.w);
     }
-    st.l[r] = l;
-    st.m[r] = mn;
+    uint32_t left = __ballot_sync(0xffffffffu, odd && seen);
+    const bool drop = !seen || odd;
+    while (left) {
+      const int t = __ffs(left) - 1;
+      left &= left - 1;
+      const int c = (t & 7) ^ ((t >> 1) & 4);  // its column in tile t / 8
+      const int src = (lane & ~3) | (c >> 1);
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const bool second = c & 1, g1 = t & 8, g2 = t & 16;
+        const float p0 = second ? w[r][1] : w[r][0], p1 = second ? w[r][3] : w[r][2];
+        const float p2 = second ? w[r][5] : w[r][4], p3 = second ? w[r][7] : w[r][6];
+        const float wt = __shfl_sync(0xffffffffu, g2 ? (g1 ? p3 : p2) : (g1 ? p1 : p0), src);
+        if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
+#pragma unroll
+        for (int nd = 0; nd < NDT; ++nd)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int col = nd * 8 + 2 * quad + j;
+            const uint32_t addr = tile_chunk_addr<e4m3_t, D>(vbase, t, col / 16) + (uint32_t)(col % 16);
+            uint32_t code;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(addr) : "memory");
+            o_acc[nd][2 * r + j] = fmaf(wt, lo_half<__half>(e4m3x2_to_f16x2(code)), o_acc[nd][2 * r + j]);
+          }
+      }
+    }
+    if constexpr (kOwnTile) {
+      __syncwarp();
+      if (drop) {
+#pragma unroll
+        for (int ch = 0; ch < D / 16; ++ch) zero_chunk(tile_chunk_addr<e4m3_t, D>(vbase, lane, ch));
+      }
+      __syncwarp();
+    } else {
+      dropped = __ballot_sync(0xffffffffu, drop);
+    }
   }
-  rescale_rows<D>(o_acc, alpha);
 
   // ---- O += P V: two k-steps of 16 tokens ----
   uint32_t pa[2][4];
@@ -541,66 +647,30 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
     for (int n = 0; n < 4; ++n)
       if (vs[n] == 0.f) pa[n >> 1][2 * (n & 1)] = pa[n >> 1][2 * (n & 1) + 1] = 0u;
   }
-  uint32_t vm[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-  if (boundary) {
-#pragma unroll
-    for (int n = 0; n < 4; ++n) vm[n] = keep_pair(tok_base, 8 * n + 2 * quad, tok_lo, tok_hi, odd_tokens);
-  }
-  const int tok = (((lane >> 3) & 1) << 3) | (lane & 7);
-#pragma unroll
-  for (int c = 0; c < D / 16; c += 2)
+  const uint32_t vat = tile_chunk_addr<e4m3_t, D>(vbase, v_row_8(lane & 15), lane >> 4);
+  auto pv = [&](auto masked) {
+    constexpr bool kMasked = decltype(masked)::value;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint32_t r[4];  // chunk c: tokens 0-7, 8-15; chunk c + 1: the same
-      ldsm_x4_trans(tile_chunk_addr<e4m3_t, D>(vbase, tok + 16 * h, c + (lane >> 4)), r[0], r[1], r[2], r[3]);
+      const uint32_t vm0 = kMasked ? keep_pair(dropped, 16 * h + 2 * quad) : 0u;
+      const uint32_t vm1 = kMasked ? keep_pair(dropped, 16 * h + 8 + ((2 * quad) ^ 4)) : 0u;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // bytes (token 2q: even, odd column; token 2q+1: even, odd) -> (even, even, odd, odd)
-        const uint32_t a = __byte_perm(r[2 * j], 0u, 0x3120), b = __byte_perm(r[2 * j + 1], 0u, 0x3120);
-        Mma16816<__half>::run(o_acc[2 * (c + j)], pa[h], e4m3x2_to_f16x2(a) & vm[2 * h],
-                              e4m3x2_to_f16x2(b) & vm[2 * h + 1]);
-        Mma16816<__half>::run(o_acc[2 * (c + j) + 1], pa[h], e4m3x2_to_f16x2(a >> 16) & vm[2 * h],
-                              e4m3x2_to_f16x2(b >> 16) & vm[2 * h + 1]);
+      for (int c = 0; c < D / 16; c += 2) {
+        uint32_t r[4];  // chunk c: columns 0-7, 8-15; chunk c + 1: the same
+        ldsm_b8_x2_trans(flip_chunk(vat, c) + 16u * h * TileLayout<e4m3_t, D>::kRowBytes, r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t b0 = e4m3x2_to_f16x2(r[j]), b1 = e4m3x2_hi_to_f16x2(r[j]);
+          if constexpr (kMasked) b0 &= vm0, b1 &= vm1;
+          Mma16816<__half>::run(o_acc[2 * c + j], pa[h], b0, b1);
+        }
       }
     }
-  // Tokens taken out above, for the rows that see them (rare: a code is NaN).
-  while (odd_tokens) {
-    const int t = __ffs(odd_tokens) - 1;
-    odd_tokens &= odd_tokens - 1;
-    const int src = (lane & ~3) | ((t & 7) >> 1);  // the quad lane that holds column t
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const bool second = t & 1, g1 = t & 8, g2 = t & 16;
-      const float p0 = second ? w[r][1] : w[r][0], p1 = second ? w[r][3] : w[r][2];
-      const float p2 = second ? w[r][5] : w[r][4], p3 = second ? w[r][7] : w[r][6];
-      const float mine = g2 ? (g1 ? p3 : p2) : (g1 ? p1 : p0);
-      const float wt = __shfl_sync(0xffffffffu, mine, src);
-      if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
-#pragma unroll
-      for (int nd = 0; nd < NDT; ++nd)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int col = (nd >> 1) * 16 + 4 * quad + 2 * j + (nd & 1);  // before end_piece_columns()
-          const uint32_t addr = tile_chunk_addr<e4m3_t, D>(vbase, t, col / 16) + (uint32_t)(col % 16);
-          uint32_t code;
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(code) : "r"(addr));
-          o_acc[nd][2 * r + j] = fmaf(wt, lo_half<__half>(e4m3x2_to_f16x2(code)), o_acc[nd][2 * r + j]);
-        }
-    }
-  }
-}
-
-// End of a piece of an 8-bit row: its columns in the order of frag_col().
-template <int D>
-__device__ __forceinline__ void end_piece_columns(float (&o_acc)[D / 8][4]) {
-#pragma unroll
-  for (int nd = 0; nd < D / 8; nd += 2)
-#pragma unroll
-    for (int r = 0; r < 4; r += 2) {
-      const float t = o_acc[nd][r + 1];  // column 4q + 2; the odd tile holds 4q + 1, 4q + 3
-      o_acc[nd][r + 1] = o_acc[nd + 1][r];
-      o_acc[nd + 1][r] = t;
-    }
+  };
+  if (kOwnTile || !boundary)
+    pv(Bool<false>{});
+  else
+    pv(Bool<true>{});
 }
 
 // 1 / l of a finished row.  A row without weight is zero when it sees no key, and
@@ -611,13 +681,13 @@ __device__ __forceinline__ float row_norm(float l, bool sees_a_key) {
   return l > 0.f ? 1.f / l * lift : (l == 0.f && !sees_a_key) ? 0.f : __int_as_float(0x7fffffff);
 }
 
-// store_rows with the norms inv0 / inv1 and the columns of frag_col<KV>().
-template <typename T, typename KV, int D>
+// store_rows with the norms inv0 / inv1.
+template <typename T, int D>
 __device__ __forceinline__ void store_rows_ext(T* op0, T* op1, const float (&o_acc)[D / 8][4], float inv0, float inv1,
                                                int quad, int Dv) {
 #pragma unroll
   for (int nd = 0; nd < D / 8; ++nd) {
-    const int d = frag_col<KV>(nd, quad);
+    const int d = nd * 8 + 2 * quad;
     if (d >= Dv) break;
     if (op0) *reinterpret_cast<uint32_t*>(op0 + d) = pack2<T>(o_acc[nd][0] * inv0, o_acc[nd][1] * inv0);
     if (op1) *reinterpret_cast<uint32_t*>(op1 + d) = pack2<T>(o_acc[nd][2] * inv1, o_acc[nd][3] * inv1);
