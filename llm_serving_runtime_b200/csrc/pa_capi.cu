@@ -725,14 +725,29 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
       if (e != cudaSuccess) return cuda_fail(e, "multi-query launch");
       return PA_OK;
     }
-    static const long long direct_rows = getenv("DIRECT_ROWS") ? atoll(getenv("DIRECT_ROWS")) : info->num_sms;
-    if ((long long)p.B * p.Hkv * p.NMG <= direct_rows) {
+    // CTAs of their own for each row, where no more rows than SMs split over the
+    // GPU, or where no row can be long: up to kDirectUnits units (a bound by the
+    // table's width, or the window) one CTA ends before balance matters.  Measured
+    // against the stream-K kernel, us a call: 1 x 32k 24 for 66; 24 rows of 16 to 300
+    // tokens 10.3 for 17.4, 96 of 1500 to 2048 76 for 82, 160 with a window of
+    // 1024 101 for 102; but 40 of 256 to 8192 61 (split further) for 53.
+    constexpr long long kDirectUnits = 130;
+    const long long rows = (long long)p.B * p.Hkv * p.NMG;
+    long long tokens = (long long)a->max_blocks * bs;
+    if (p.window > 0) tokens = std::min(tokens, (long long)p.window + p.q_len);
+    const bool few = rows <= info->num_sms;
+    if (few || tokens / (sc != nullptr ? 32 : 16) + 2 <= kDirectUnits) {
+      const pa::DirectShape d = pa::decode_direct_shape(sc != nullptr, !few);
+      // the CTAs of an SM share its memory, 1 KB of it and the static part (5.2 KB) reserved for each
+      const size_t share = (budget + 1152) / d.ctas_per_sm - 1024 - 6144;
       int n = 8;
-      while (n > 2 && pa::decode_direct_smem_bytes(D, n, sc != nullptr) > budget - 6144) --n;
+      while (n > 2 && pa::decode_direct_smem_bytes(D, n, d.warps, sc != nullptr) > share) --n;
       p.stages = n;
-      g_last_kernel = "pa::decode_direct_kernel";
-      e = pa::launch_decode_direct(p, tmk, tmv, dtype, info->num_sms,
-                                   pa::decode_direct_smem_bytes(D, n, sc != nullptr), pdl, strm);
+      p.chunk_units = 2 * d.warps;
+      const int splits = few ? (int)std::min<long long>(pa::kDirectMaxSplits, info->num_sms / rows) : 1;
+      g_last_kernel = few ? "pa::decode_direct_kernel<few>" : "pa::decode_direct_kernel<many>";
+      e = pa::launch_decode_direct(p, tmk, tmv, dtype, splits, !few,
+                                   pa::decode_direct_smem_bytes(D, n, d.warps, sc != nullptr), pdl, strm);
       if (e != cudaSuccess) return cuda_fail(e, "decode launch");
       return PA_OK;
     }

@@ -5,12 +5,13 @@
 // crosses rows pays for each start and end, a warp's least share is several units,
 // and a long row's many pieces are merged by one warp.  With no more rows than
 // CTAs fit the GPU none of that is needed: CTA (row, s) takes the s-th of S equal
-// ranges of the row's units, its eight warps an eighth of it each (their own ring
+// ranges of the row's units, its warps an equal part of it each (their own ring
 // of TMA tiles, as there), and merges their states in shared memory; the last CTA
 // of a row to finish merges the S partial states, all threads together, with the
-// log-sum-exp rule, in the order of the ranges.  S is what fills the GPU, at most
-// kMaxSplits, and no more than leaves every CTA kMinUnits units (known on the
-// device only: further CTAs leave at once).
+// log-sum-exp rule, in the order of the ranges.  S is at most the launch's second
+// dimension and leaves every CTA chunk_units units or more (known on the device
+// only: further CTAs leave at once).  The rule on shapes and sizes that calls it
+// is in pa_capi.cu, with what was measured.
 #include "pa_common.cuh"
 #include "pa_internal.h"
 #include "pa_tile_ext.cuh"
@@ -19,19 +20,23 @@
 namespace pa {
 
 namespace {
-constexpr int kWarps = 8;
-constexpr int kMaxSplits = 64;
-#ifndef DIRECT_MIN_UNITS
-#define DIRECT_MIN_UNITS 16
-#endif
-constexpr int kMinUnits = DIRECT_MIN_UNITS;  // units of a CTA before its row is split further
+constexpr int kMaxSplits = kDirectMaxSplits;
+// Warps of a CTA, and CTAs an SM is built for.  Few rows: one CTA with all warps,
+// so that a row's share is spread widest.  Many rows: several smaller CTAs, whose
+// starts and ends overlap the others' work.
+template <typename KV, bool kMany>
+struct Shape {
+  static constexpr int kWarps = kIs8<KV>::value ? (kMany ? 4 : 12) : (kMany ? 6 : 8);
+  static constexpr int kCtas = kMany ? (kIs8<KV>::value ? 3 : 2) : 1;
+};
 }  // namespace
 
-template <typename T, int D, typename KV, bool kScored>
-__global__ void __launch_bounds__(kWarps * 32, 1)
+template <typename T, int D, typename KV, bool kScored, bool kMany>
+__global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany>::kCtas)
     decode_direct_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                          const DecodeParams p) {
   constexpr bool k8 = kIs8<KV>::value;
+  constexpr int kWarps = Shape<KV, kMany>::kWarps;
   using TL = TileLayout<KV, D>;
   constexpr int UT = TL::kTokens;
   constexpr int HALVES = TL::kHalves;
@@ -89,7 +94,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   }
   const int u_first = lo / UT;
   const int n = hi > lo ? (hi + UT - 1) / UT - u_first : 0;
-  const int S = max(1, min((int)gridDim.y, n / kMinUnits));
+  const int S = max(1, min((int)gridDim.y, (n + p.chunk_units - 1) / p.chunk_units));
   if (split >= S) return;
   const int c0 = (int)((long long)n * split / S), c1 = (int)((long long)n * (split + 1) / S);
   const int w0 = u_first + c0 + (c1 - c0) * warp / kWarps, w1 = u_first + c0 + (c1 - c0) * (warp + 1) / kWarps;
@@ -202,7 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
     slot = slot + 1 == stages ? 0 : slot + 1;
   }
 
-  // ---- the CTA's state: (m, l, acc) of eight warps, acc in each warp's own ring ----
+  // ---- the CTA's state: (m, l, acc) of its warps, acc in each warp's own ring ----
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     float l = st.l[r] + __shfl_xor_sync(0xffffffffu, st.l[r], 1);
@@ -316,16 +321,26 @@ __global__ void __launch_bounds__(kWarps * 32, 1)
   if (tid == 0) atomicExch(&p.counters[row], 0);
 }
 
-size_t decode_direct_smem_bytes(int D, int stages, bool eight) {
+DirectShape decode_direct_shape(bool eight, bool many) {
+  DirectShape d;
+  d.warps = eight ? (many ? Shape<e4m3_t, true>::kWarps : Shape<e4m3_t, false>::kWarps)
+                  : (many ? Shape<__half, true>::kWarps : Shape<__half, false>::kWarps);
+  d.ctas_per_sm = eight ? (many ? Shape<e4m3_t, true>::kCtas : Shape<e4m3_t, false>::kCtas)
+                        : (many ? Shape<__half, true>::kCtas : Shape<__half, false>::kCtas);
+  return d;
+}
+
+size_t decode_direct_smem_bytes(int D, int stages, int warps, bool eight) {
   const size_t stage_bytes = 2u * 16u * (size_t)D * 2u;  // 16 tokens of 2 bytes, or 32 of 1
-  return 1024 + (size_t)kWarps * stages * (stage_bytes + 8 + (eight ? 32 : 0));
+  return 1024 + (size_t)warps * stages * (stage_bytes + 8 + (eight ? 32 : 0));
 }
 
 namespace {
 
-template <typename T, int D, typename KV, bool kScored>
+template <typename T, int D, typename KV, bool kScored, bool kMany>
 cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int splits, size_t smem,
                    bool pdl, cudaStream_t stream) {
+  const auto kernel = decode_direct_kernel<T, D, KV, kScored, kMany>;
   // Shared memory beyond the default limit, once per device (the largest a block may have).
   static bool prepared[64] = {false};
   int dev = 0, most = 0;
@@ -336,16 +351,15 @@ cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensor
     e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
     if (e != cudaSuccess) return e;
     cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, decode_direct_kernel<T, D, KV, kScored>);
+    e = cudaFuncGetAttributes(&fa, kernel);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(decode_direct_kernel<T, D, KV, kScored>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             most - (int)fa.sharedSizeBytes);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)fa.sharedSizeBytes);
     if (e != cudaSuccess) return e;
     prepared[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * p.NMG), (unsigned)splits);
-  cfg.blockDim = dim3(kWarps * 32);
+  cfg.blockDim = dim3(Shape<KV, kMany>::kWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -353,29 +367,34 @@ cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensor
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl ? attr : nullptr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, decode_direct_kernel<T, D, KV, kScored>, tmk, tmv, p);
+  return cudaLaunchKernelEx(&cfg, kernel, tmk, tmv, p);
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kMany>
 cudaError_t pick(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int splits, size_t smem,
                  bool pdl, cudaStream_t stream) {
-  if (p.k_scales == nullptr) return launch<T, D, T, true>(p, tmk, tmv, splits, smem, pdl, stream);
-  if (p.scored) return launch<T, D, e4m3_t, true>(p, tmk, tmv, splits, smem, pdl, stream);
-  return launch<T, D, e4m3_t, false>(p, tmk, tmv, splits, smem, pdl, stream);
+  if (p.k_scales == nullptr) return launch<T, D, T, true, kMany>(p, tmk, tmv, splits, smem, pdl, stream);
+  if (p.scored) return launch<T, D, e4m3_t, true, kMany>(p, tmk, tmv, splits, smem, pdl, stream);
+  return launch<T, D, e4m3_t, false, kMany>(p, tmk, tmv, splits, smem, pdl, stream);
+}
+
+template <typename T>
+cudaError_t pick_width(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int splits, bool many,
+                       size_t smem, bool pdl, cudaStream_t stream) {
+  if (p.D == 128)
+    return many ? pick<T, 128, true>(p, tmk, tmv, splits, smem, pdl, stream)
+                : pick<T, 128, false>(p, tmk, tmv, splits, smem, pdl, stream);
+  return many ? pick<T, 64, true>(p, tmk, tmv, splits, smem, pdl, stream)
+              : pick<T, 64, false>(p, tmk, tmv, splits, smem, pdl, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_decode_direct(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
-                                 int num_sms, size_t smem, bool pdl, cudaStream_t stream) {
-  const int rows = p.B * p.Hkv * p.NMG;
-  int splits = num_sms / rows;
-  splits = splits < 1 ? 1 : splits > kMaxSplits ? kMaxSplits : splits;
-  if (dtype == PA_DTYPE_BFLOAT16)
-    return p.D == 128 ? pick<__nv_bfloat16, 128>(p, tmk, tmv, splits, smem, pdl, stream)
-                      : pick<__nv_bfloat16, 64>(p, tmk, tmv, splits, smem, pdl, stream);
-  return p.D == 128 ? pick<__half, 128>(p, tmk, tmv, splits, smem, pdl, stream)
-                    : pick<__half, 64>(p, tmk, tmv, splits, smem, pdl, stream);
+                                 int splits, bool many, size_t smem, bool pdl, cudaStream_t stream) {
+  if (splits < 1 || splits > kMaxSplits) return cudaErrorInvalidValue;
+  return dtype == PA_DTYPE_BFLOAT16 ? pick_width<__nv_bfloat16>(p, tmk, tmv, splits, many, smem, pdl, stream)
+                                    : pick_width<__half>(p, tmk, tmv, splits, many, smem, pdl, stream);
 }
 
 }  // namespace pa

@@ -12,7 +12,7 @@ size_t decode_ext_smem_bytes(int D, int B, int stages, bool eight, bool scored) 
 
 namespace {
 
-template <typename T, int D, typename C, bool kScored>
+template <typename T, int D, typename KV, bool kScored>
 cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int grid, size_t smem,
                    bool pdl, cudaStream_t stream) {
   // Shared memory beyond the default limit, once per device (the largest a block may have).
@@ -25,9 +25,9 @@ cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensor
     e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
     if (e != cudaSuccess) return e;
     cudaFuncAttributes fa;
-    e = cudaFuncGetAttributes(&fa, decode_mma_kernel<T, D, 0, C, kScored>);
+    e = cudaFuncGetAttributes(&fa, decode_mma_kernel<T, D, 0, KV, kScored>);
     if (e != cudaSuccess) return e;
-    e = cudaFuncSetAttribute(decode_mma_kernel<T, D, 0, C, kScored>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    e = cudaFuncSetAttribute(decode_mma_kernel<T, D, 0, KV, kScored>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              most - (int)fa.sharedSizeBytes);
     if (e != cudaSuccess) return e;
     prepared[dev] = true;
@@ -42,7 +42,7 @@ cudaError_t launch(const DecodeParams& p, const CUtensorMap& tmk, const CUtensor
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl ? attr : nullptr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, decode_mma_kernel<T, D, 0, C, kScored>, tmk, tmv, p);
+  return cudaLaunchKernelEx(&cfg, decode_mma_kernel<T, D, 0, KV, kScored>, tmk, tmv, p);
 }
 
 template <typename T, int D>

@@ -117,6 +117,7 @@ struct DecodeParams {
   int64_t ks_sblk, ks_sh, vs_sblk, vs_sh;
   // Changed scores (pa_decode_ext with modifiers), scored != 0.
   int32_t scored;
+  int32_t chunk_units;          // units of a CTA before its row is split (pa_decode_direct.cu)
   int32_t window;               // keys at distance >= window are hidden; 0: none
   float softcap;                // 0: none; c * tanh(s / c)
   float softcap_log2, inv_softcap_log2;  // the cap and its inverse in the log2 domain
@@ -178,11 +179,16 @@ struct ScaleParams {
   int64_t ks_sblk, ks_sh, vs_sblk, vs_sh;
 };
 
-// pa_decode_ext for at most num_sms rows (B * Hkv * NMG): CTAs of their own for
-// each row (pa_decode_direct.cu).
-size_t decode_direct_smem_bytes(int D, int stages, bool eight);
+// pa_decode_ext with CTAs of their own for each row, a sequence's KV head and 16
+// query rows (pa_decode_direct.cu): at most 64 splits of p.chunk_units units or more.
+struct DirectShape {
+  int warps, ctas_per_sm;
+};
+constexpr int kDirectMaxSplits = 64;
+DirectShape decode_direct_shape(bool eight, bool many);
+size_t decode_direct_smem_bytes(int D, int stages, int warps, bool eight);
 cudaError_t launch_decode_direct(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
-                                 int num_sms, size_t smem, bool pdl, cudaStream_t stream);
+                                 int splits, bool many, size_t smem, bool pdl, cudaStream_t stream);
 
 // Caches whose pages move together: byte strides; a page is `segments` runs of
 // segment_bytes, stride_segment apart.
