@@ -311,9 +311,11 @@ typedef struct pa_score_modifiers {
 
 /* pa_decode over an 8-bit cache (scales != NULL: args->dtype is the type of query
  * and out, fp16 or bf16; head_dim a multiple of 16) and / or with changed scores
- * (modifiers != NULL; any dtype).  Same workspace as pa_decode. */
+ * (modifiers != NULL; any dtype).  Same workspace as pa_decode.  error_flags: a word
+ * (device, or pinned host memory that the host reads itself) that receives the
+ * PA_DEVERR_* bits instead of the workspace's first; may be NULL. */
 PA_API int pa_decode_ext(const pa_decode_args* args, const pa_cache_scales* scales,
-                         const pa_score_modifiers* modifiers, void* stream);
+                         const pa_score_modifiers* modifiers, uint32_t* error_flags, void* stream);
 
 /* ---- pages of a cache ------------------------------------------------------
  * Caches whose pages move together, each [num_blocks, ...]: a page is `segments`

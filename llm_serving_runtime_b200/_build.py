@@ -4,6 +4,7 @@ The library exports the C ABI declared in ``include/paged_attention_b200.h``.
 It links only the CUDA runtime (the driver's tensor-map encoder is fetched at
 run time through ``cudaGetDriverEntryPoint``), so it loads on a machine
 without a GPU and can be built there (nvcc cross-compiles for sm_100a).
+``build_host`` compiles the CPython extension ``lib/pa_host.so`` beside it (g++).
 """
 
 from __future__ import annotations
@@ -25,6 +26,10 @@ SOURCES = ["pa_capi.cu", "pa_kv_append.cu", "pa_decode_mma.cu", "pa_decode_f32.c
            "pa_pages.cu"]
 HEADERS = ["pa_common.cuh", "pa_internal.h", "pa_tile_math.cuh", "pa_tile_ext.cuh", "pa_decode_kernel.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
+
+
+HOST_SOURCE = CSRC / "pa_host.cpp"
+HOST_PATH = LIB_DIR / "pa_host.so"
 
 
 def _nvcc() -> str:
@@ -89,9 +94,40 @@ def build_library(force: bool = False, verbose: bool = False, extra_flags: list[
     return LIB_PATH
 
 
+def build_host(force: bool = False) -> Path:
+    """Compile the host extension ``lib/pa_host.so`` against the installed torch
+    and ``libpa_b200.so`` beside it (skipped when up to date)."""
+    header = REPO_DIR / "include" / "paged_attention_b200.h"
+    if not force and HOST_PATH.exists() and HOST_PATH.stat().st_mtime >= max(HOST_SOURCE.stat().st_mtime,
+                                                                             header.stat().st_mtime):
+        return HOST_PATH
+    import sysconfig
+
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    cuda_home = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    cmd = [
+        "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-isystem", str(torch_dir / "include"), "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+        "-isystem", str(cuda_home / "include"), "-isystem", sysconfig.get_paths()["include"],
+        str(HOST_SOURCE), "-o", str(tmp),
+        f"-L{LIB_DIR}", "-l:libpa_b200.so", f"-L{torch_dir / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+        "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_dir / 'lib'}",
+    ]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
+
+
 if __name__ == "__main__":
     import sys
 
     path = build_library(force="--force" in sys.argv, verbose=True,
                          extra_flags=["-Xptxas", "-v"] if "--ptxas-v" in sys.argv else None)
     print(path)
+    print(build_host(force="--force" in sys.argv))

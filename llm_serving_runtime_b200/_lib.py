@@ -11,6 +11,7 @@ import threading
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libpa_b200.so"
+HOST_PATH = LIB_PATH.with_name("pa_host.so")
 
 PA_OK = 0
 PA_ERR_INVALID_ARGUMENT = 1
@@ -254,7 +255,7 @@ def load() -> ctypes.CDLL:
         lib.pa_kv_append_8bit.argtypes = [ctypes.POINTER(KvAppendArgs), ctypes.POINTER(CacheScalesArgs), _vp]
         lib.pa_decode_ext.restype = ctypes.c_int
         lib.pa_decode_ext.argtypes = [ctypes.POINTER(DecodeArgs), ctypes.POINTER(CacheScalesArgs),
-                                      ctypes.POINTER(ScoreModifiersArgs), _vp]
+                                      ctypes.POINTER(ScoreModifiersArgs), _vp, _vp]
         views, tables = ctypes.POINTER(PageViewArgs), ctypes.POINTER(PageTablesArgs)
         lib.pa_pages_scratch_words.restype = _sz
         lib.pa_pages_scratch_words.argtypes = [_i32, _i32]
@@ -312,6 +313,26 @@ def cudart() -> ctypes.CDLL | None:
             f.restype = ctypes.c_int
         _cudart_handle = rt
         return rt
+
+
+_host_handle = None
+
+
+def host():
+    """The extension with the usual calls in one step (csrc/pa_host.cpp)."""
+    global _host_handle
+    if _host_handle is None:
+        load()
+        import importlib.util
+
+        if not HOST_PATH.exists():
+            raise RuntimeError(f"{HOST_PATH} is missing: build it with `python -c \"import __graft_entry__ as g; "
+                               "g.build()\"` (or python llm_serving_runtime_b200/_build.py).")
+        spec = importlib.util.spec_from_file_location("pa_host", HOST_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _host_handle = module
+    return _host_handle
 
 
 def last_error() -> str:

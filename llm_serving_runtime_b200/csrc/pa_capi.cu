@@ -433,7 +433,8 @@ size_t pa_cascade_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t nu
 }
 
 static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, const pa_gather_args* gat,
-                       void* stream, const pa_cache_scales* sc = nullptr, const pa_score_modifiers* sm = nullptr);
+                       void* stream, const pa_cache_scales* sc = nullptr, const pa_score_modifiers* sm = nullptr,
+                       uint32_t* error_flags = nullptr);
 
 int pa_decode(const pa_decode_args* a, void* stream) { return decode_impl(a, nullptr, nullptr, stream); }
 
@@ -503,7 +504,7 @@ int pa_decode_cascade(const pa_decode_args* a, const pa_prefix_groups* grp, void
 }
 
 int pa_decode_ext(const pa_decode_args* a, const pa_cache_scales* scales, const pa_score_modifiers* modifiers,
-                  void* stream) {
+                  uint32_t* error_flags, void* stream) {
   g_last_error[0] = 0;
   if (a == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null args");
   if (scales != nullptr) {
@@ -517,11 +518,12 @@ int pa_decode_ext(const pa_decode_args* a, const pa_cache_scales* scales, const 
       return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be 0 (none) or positive and finite");
     if (modifiers->window < 0) return fail(PA_ERR_INVALID_ARGUMENT, "window must be 0 (none) or positive");
   }
-  return decode_impl(a, nullptr, nullptr, stream, scales, modifiers);
+  return decode_impl(a, nullptr, nullptr, stream, scales, modifiers, error_flags);
 }
 
 static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, const pa_gather_args* gat,
-                       void* stream, const pa_cache_scales* sc, const pa_score_modifiers* sm) {
+                       void* stream, const pa_cache_scales* sc, const pa_score_modifiers* sm,
+                       uint32_t* error_flags) {
   g_last_error[0] = 0;
   if (a == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null args");
   const int dtype = a->dtype;
@@ -601,7 +603,7 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   p.Dv = Dv;
   p.scale = a->scale;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.status = static_cast<uint32_t*>(a->workspace);
+  p.status = error_flags != nullptr ? error_flags : static_cast<uint32_t*>(a->workspace);
   p.slot_rows = s.slot_rows;
   if (sc != nullptr) {
     st = check_cache_8bit(*a, bs, Dv);

@@ -44,14 +44,12 @@ from . import _lib
 from .paged_attention import (
     _VALIDATE_DEFAULT,
     _as_int32,
-    _capturing,
-    _copy_after_call,
-    _raise_landed_errors,
+    _host,
+    _host_words,
+    _HostWord,
     _stream_ptr,
     _with_device,
-    decode_workspace,
-    device_error,
-    read_device_errors,
+    host_word,
 )
 
 __all__ = ["DevicePages", "copy_pages"]
@@ -106,20 +104,13 @@ def _ids(t: torch.Tensor, device: torch.device, name: str) -> torch.Tensor:
     return t
 
 
-def _run(device: torch.device, word: torch.Tensor, validate: bool | None, what: str, call) -> None:
+def _run(word: _HostWord, validate: bool | None, what: str, call) -> None:
     """One C call on the current stream, with the errors of the framework's kernels."""
-    deferred = validate is None and not _VALIDATE_DEFAULT and not _capturing()
-    if deferred:
-        _raise_landed_errors(word)
-    stream = _stream_ptr(device)
-    with _with_device(device):
-        _lib.check(call(stream), what)
-    if deferred:
-        _copy_after_call(word, stream)
-    elif validate if validate is not None else _VALIDATE_DEFAULT:
-        flags = read_device_errors(workspace=word)
-        if flags:
-            raise device_error(flags)
+    if validate is None:
+        word.raise_landed()
+    with _with_device(word.device):
+        _lib.check(call(_stream_ptr(word.device)), what)
+        word.finish(validate)
 
 
 def copy_pages(caches: Sequence[torch.Tensor], src_blocks: torch.Tensor, dst_blocks: torch.Tensor, *,
@@ -133,6 +124,10 @@ def copy_pages(caches: Sequence[torch.Tensor], src_blocks: torch.Tensor, dst_blo
     """
     if not caches:
         raise ValueError("copy_pages needs a cache")
+    if validate is None and not _VALIDATE_DEFAULT:
+        word = _host_words.get(caches[0].device.index)
+        if word is not None and _host.copy_pages(caches, src_blocks, dst_blocks, word.ptr):
+            return
     arr, n_views, num_blocks, device = _views(caches, None, None)
     src, dst = _ids(src_blocks, device, "src_blocks"), _ids(dst_blocks, device, "dst_blocks")
     if src.numel() != dst.numel():
@@ -141,10 +136,10 @@ def copy_pages(caches: Sequence[torch.Tensor], src_blocks: torch.Tensor, dst_blo
         raise ValueError("the caches have no blocks")
     if src.numel() == 0:
         return
-    word = decode_workspace(device)
-    _run(device, word, validate, "pa_pages_copy",
+    word = host_word(device)
+    _run(word, validate, "pa_pages_copy",
          lambda stream: _lib.load().pa_pages_copy(arr, n_views, num_blocks, src.data_ptr(), dst.data_ptr(),
-                                                  src.numel(), word.data_ptr(), stream))
+                                                  src.numel(), word.ptr, stream))
 
 
 class DevicePages:
@@ -195,7 +190,7 @@ class DevicePages:
         words = _lib.load().pa_pages_scratch_words(self.max_seqs, self.num_blocks)
         self._scratch = torch.empty(words, dtype=torch.int32, device=self.device)
         # its own error word: two objects on two streams do not share one
-        self._word = torch.zeros(256, dtype=torch.uint8, device=self.device)
+        self._word = _HostWord(self.device)
 
     @property
     def max_seqs(self) -> int:
@@ -207,17 +202,24 @@ class DevicePages:
 
     def read_errors(self) -> int:
         """The PA_DEVERR_* bits of this object's calls so far, cleared.  Synchronises."""
-        return read_device_errors(workspace=self._word)
+        return self._word.take()
 
     def _args(self) -> _lib.PageTablesArgs:
         t = self.block_tables
         return _lib.PageTablesArgs(t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[0], t.shape[1],
                                    self.seq_lens.data_ptr(), self.ref_counts.data_ptr(), self.num_blocks,
-                                   self.block_size, self._scratch.data_ptr(), self._word.data_ptr())
+                                   self.block_size, self._scratch.data_ptr(), self._word.ptr)
 
     def _call(self, what: str, validate: bool | None, *rest) -> None:
         args, fn = self._args(), getattr(_lib.load(), what)
-        _run(self.device, self._word, validate, what, lambda stream: fn(ctypes.byref(args), *rest, stream))
+        _run(self._word, validate, what, lambda stream: fn(ctypes.byref(args), *rest, stream))
+
+    def _fast(self, op: int, validate: bool | None, a=None, b=None, caches=()):
+        """The call in one step, when its arguments are the kernels' already; else None."""
+        if validate is not None or _VALIDATE_DEFAULT:
+            return None
+        return _host.pages(op, self.block_tables, self.seq_lens, self.ref_counts, self.block_size, self._scratch,
+                           self._word.ptr, a, b, caches)
 
     def _slots(self, t: torch.Tensor, name: str) -> torch.Tensor:
         t = _ids(t, self.device, name)
@@ -228,6 +230,8 @@ class DevicePages:
     def free(self, slots: torch.Tensor, *, validate: bool | None = None) -> None:
         """Empty the slots; pages nobody holds any more are free.  A slot named twice
         is freed once, an empty one stays empty."""
+        if self._fast(0, validate, slots):
+            return
         slots = self._slots(slots, "slots")
         self._call("pa_pages_free", validate, slots.data_ptr(), slots.numel())
 
@@ -235,6 +239,8 @@ class DevicePages:
              validate: bool | None = None) -> None:
         """Each empty slot children[i] gets the tokens of parents[i]: the full pages are
         shared, the page in use is copied in every cache to the child's own."""
+        if self._fast(1, validate, parents, children, caches):
+            return
         parents, children = self._slots(parents, "parents"), self._slots(children, "children")
         if parents.numel() != children.numel():
             raise ValueError(f"{parents.numel()} parents but {children.numel()} children")
@@ -243,6 +249,8 @@ class DevicePages:
 
     def reserve(self, slots: torch.Tensor, n_tokens: torch.Tensor, *, validate: bool | None = None) -> None:
         """Slot slots[i] grows by n_tokens[i] tokens, with new pages where needed."""
+        if self._fast(2, validate, slots, n_tokens):
+            return
         slots, n_tokens = self._slots(slots, "slots"), _ids(n_tokens, self.device, "n_tokens")
         if slots.numel() != n_tokens.numel():
             raise ValueError(f"{slots.numel()} slots but {n_tokens.numel()} numbers of tokens")
@@ -252,6 +260,9 @@ class DevicePages:
                 validate: bool | None = None) -> torch.Tensor:
         """Move the live pages to ids [0, live) in every cache and in the tables; returns
         ``live`` as a device int32 [1] (``out`` when given)."""
+        live = self._fast(3, validate, caches=caches) if out is None else None
+        if live is not None:
+            return live
         arr, n, _, _ = _views(caches, self.num_blocks, self.device)
         if out is None:
             out = torch.empty(1, dtype=torch.int32, device=self.device)

@@ -127,6 +127,17 @@ _VALIDATE_DEFAULT = os.environ.get("PA_B200_VALIDATE", "0") == "1"
 # every SM's share equal.
 _SM_SHARES = os.environ.get("PA_B200_SM_SHARES", "1") != "0"
 
+class _Host:
+    """The host extension's calls, loaded on first use."""
+
+    def __getattr__(self, name: str):
+        fn = getattr(_lib.host(), name)
+        setattr(self, name, fn)
+        return fn
+
+
+_host = _Host()
+
 # One workspace per device: status word + merge counters + partial slots.
 _ws_lock = threading.Lock()
 _workspaces: dict[int, torch.Tensor] = {}
@@ -164,10 +175,18 @@ def read_device_errors(device: torch.device | None = None, *, clear: bool = True
     """Read (and clear) the PA_DEVERR_* bits the kernels recorded.  Synchronises.
 
     Clearing also drops the copy of the word that the next call would have
-    checked: the bits it holds have been read here."""
+    checked: the bits it holds have been read here.  Without ``workspace`` the
+    bits of the extended operators' calls (``host_word``) are among them."""
+    host = 0
     if workspace is None:
         device = device or torch.device("cuda", torch.cuda.current_device())
         workspace = decode_workspace(device)
+        word = _host_words.get(workspace.device.index)
+        if word is not None:
+            torch.cuda.current_stream(word.device).synchronize()
+            host = int(word.word.value)
+            if clear:
+                word.word.value = 0
     if clear:
         with _checks_lock:
             c = _checks.get((workspace.device.index, workspace.data_ptr()))
@@ -180,7 +199,7 @@ def read_device_errors(device: torch.device | None = None, *, clear: bool = True
         ),
         "pa_read_device_errors",
     )
-    return int(flags.value)
+    return int(flags.value) | host
 
 
 # The workspace's first bytes: the device error word at 0, then (at
@@ -277,6 +296,56 @@ def sm_speeds(device: torch.device) -> SmSpeeds:
         if t is None:
             t = _speeds[idx] = SmSpeeds(torch.cuda.get_device_properties(idx).multi_processor_count)
         return t
+
+
+class _HostWord:
+    """A device error word in pinned host memory, for the kernels of the extended
+    operators (8-bit caches, score modifiers, pages): a kernel's atomic OR reaches it
+    directly, so looking for the errors of earlier calls is one host read, with
+    no copy queued behind each call."""
+
+    __slots__ = ("host", "ptr", "word", "device")
+
+    def __init__(self, device: torch.device):
+        self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        self.ptr = self.host.data_ptr()
+        self.word = ctypes.c_uint32.from_address(self.ptr)
+        self.device = device
+
+    def take(self) -> int:
+        """The bits so far, cleared, once the work on the current stream is done."""
+        torch.cuda.current_stream(self.device).synchronize()
+        flags, self.word.value = self.word.value, 0
+        return int(flags)
+
+    def raise_landed(self) -> None:
+        if self.word.value and not _capturing():
+            raise device_error(self.take())
+
+    def finish(self, validate: bool | None) -> None:
+        """End of a call: the check that ``validate`` asks for."""
+        if (validate if validate is not None else _VALIDATE_DEFAULT) and not _capturing():
+            flags = self.take()
+            if flags:
+                raise device_error(flags)
+
+
+_host_words: dict[int, _HostWord] = {}
+
+
+def host_word(device: torch.device) -> _HostWord:
+    """The device's error word of calls that are given no workspace (created on first use)."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    w = _host_words.get(idx)
+    if w is None:
+        with _ws_lock:
+            w = _host_words.get(idx)
+            if w is None:
+                if _capturing():
+                    raise RuntimeError("the error word must exist before CUDA-graph capture: run the same call once "
+                                       "eagerly first")
+                w = _host_words[idx] = _HostWord(torch.device("cuda", idx))
+    return w
 
 
 class _PendingCheck:
@@ -525,6 +594,11 @@ def kv_append(
     from one row of the call (another row's are left out and flagged).
     head_dim is a multiple of 16, block_size a power of two in [8, 256].
     """
+    if key_scales is not None and error_word is None and validate is None and not _VALIDATE_DEFAULT:
+        host = _host_words.get(key_cache.device.index)
+        if host is not None and _host.append8(key, value, key_cache, value_cache, key_scales, value_scales,
+                                              slot_mapping, block_tables, positions, position_offset, host.ptr):
+            return
     _check_cache_pair(key_cache, value_cache)
     device = key_cache.device
     if key.dim() != 4:
@@ -577,6 +651,16 @@ def kv_append(
         args.position_offset = int(position_offset)
     args.batch, args.q_len, args.num_kv_heads, args.head_dim, args.block_size = B, q_len, Hkv, Dc, bs
     args.dtype = _DTYPE_CODE[key.dtype]
+    if scales is not None and error_word is None:
+        host = host_word(device)
+        if validate is None:
+            host.raise_landed()
+        args.error_flags = host.ptr
+        with _with_device(device):
+            _lib.check(_lib.load().pa_kv_append_8bit(ctypes.byref(args), ctypes.byref(scales), _stream_ptr(device)),
+                       "pa_kv_append_8bit")
+        host.finish(validate)
+        return
     if error_word is None:
         error_word = decode_workspace(device)
     args.error_flags = error_word.data_ptr()
@@ -648,6 +732,17 @@ def paged_attention_decode(
     built by ``sharding.FusedHeadGather``) makes ``out`` this rank's gathered
     output [B, total query heads, q_len, D] and writes the local heads' rows to
     every rank's gathered output in the same kernel."""
+    if (key_scales is not None or score_modifiers is not None) and workspace is None and validate is None \
+            and gather is None and prefix_groups is None and not _VALIDATE_DEFAULT:
+        idx = key_cache.device.index
+        ws, host, speeds = _workspaces.get(idx), _host_words.get(idx), _speeds.get(idx)
+        if ws is not None and host is not None and speeds is not None:
+            done = _host.decode(query, key_cache, value_cache, block_tables, context_lens, scale, slot_mapping, key,
+                                value, out, context_lens_include_new, key_scales, value_scales,
+                                None if score_modifiers is None else score_modifiers.astuple(), ws, host.ptr,
+                                speeds.weights_ptr, speeds.n if _SM_SHARES else 0)
+            if done is not None:
+                return done
     _check_cache_pair(key_cache, value_cache)
     device = key_cache.device
     if query.dim() != 4:
@@ -703,11 +798,17 @@ def paged_attention_decode(
         need = _cascade_workspace_bytes(B, Hq, Hkv, q_len, D, dcode, device.index, prefix_groups)
     else:
         need = _workspace_bytes(B, Hq, Hkv, q_len, D, dcode, device.index)
+    # The extended kernels report into the host word, unless the caller brings a
+    # workspace to hold the errors of its own calls.
+    host = host_word(device) if workspace is None and (scales is not None or modifiers is not None) else None
     if workspace is None:
         workspace = decode_workspace(device, need)
     deferred = validate is None and not _VALIDATE_DEFAULT and not _capturing()
     if deferred:
-        _raise_landed_errors(workspace)
+        if host is not None:
+            host.raise_landed()
+        else:
+            _raise_landed_errors(workspace)
     stream_ptr = _stream_ptr(device)
 
     appended = False
@@ -716,7 +817,8 @@ def paged_attention_decode(
             key, value, key_cache, value_cache, slot_mapping,
             block_tables=block_tables, positions=context_lens,
             position_offset=-q_len if context_lens_include_new else 0,
-            error_word=workspace, validate=False, key_scales=key_scales, value_scales=value_scales,
+            error_word=None if host is not None and scales is not None else workspace, validate=False,
+            key_scales=key_scales, value_scales=value_scales,
         )
         appended = True
 
@@ -744,7 +846,7 @@ def paged_attention_decode(
     if speeds.n and _SM_SHARES:
         args.sm_weights = speeds.weights_ptr
         args.num_sm_weights = speeds.n
-        if deferred and speeds.learning and query.dtype != torch.float32 and _copy_is_free(workspace) \
+        if deferred and host is None and speeds.learning and query.dtype != torch.float32 and _copy_is_free(workspace) \
                 and speeds.want_sample():
             tag = speeds.new_tag()
             args.sm_timing_tag = tag
@@ -761,7 +863,8 @@ def paged_attention_decode(
                 rc = lib.pa_decode(ctypes.byref(args), stream_ptr)
             else:
                 rc = lib.pa_decode_ext(ctypes.byref(args), ctypes.byref(scales) if scales is not None else None,
-                                       ctypes.byref(modifiers) if modifiers is not None else None, stream_ptr)
+                                       ctypes.byref(modifiers) if modifiers is not None else None,
+                                       host.ptr if host is not None else None, stream_ptr)
             if rc == _lib.PA_ERR_UNSUPPORTED and B > 1 and _BATCH_LIMIT_TEXT in _lib.last_error():
                 # More sequences than the kernel's shared-memory tables hold:
                 # the rows are independent, so attend the two halves one after
@@ -777,7 +880,9 @@ def paged_attention_decode(
                                            else score_modifiers.rows(lo, hi))
             else:
                 _lib.check(rc, "pa_decode")
-    if deferred:
+    if host is not None:
+        host.finish(validate)
+    elif deferred:
         _copy_after_call(workspace, stream_ptr, tag, speeds)
     elif validate if validate is not None else _VALIDATE_DEFAULT:
         flags = read_device_errors(workspace=workspace)

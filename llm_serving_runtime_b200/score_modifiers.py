@@ -72,6 +72,9 @@ class ScoreModifiers:
             a.prefix_lens = p.data_ptr()
         return a
 
+    def astuple(self) -> tuple:
+        return self.softcap, self.window, self.alibi_slopes, self.key_starts, self.prefix_lens
+
     def rows(self, lo: int, hi: int) -> "ScoreModifiers":
         """The modifiers of batch rows [lo, hi)."""
         return ScoreModifiers(

@@ -74,22 +74,22 @@ def _decode_args():
 def test_ext_argument_errors():
     lib = _lib.load()
     a, sc, sm = _decode_args(), _lib.CacheScalesArgs(), _lib.ScoreModifiersArgs()
-    assert lib.pa_decode_ext(None, None, None, None) == _lib.PA_ERR_INVALID_ARGUMENT
-    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), None, None) == _lib.PA_ERR_INVALID_ARGUMENT
+    assert lib.pa_decode_ext(None, None, None, None, None) == _lib.PA_ERR_INVALID_ARGUMENT
+    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), None, None, None) == _lib.PA_ERR_INVALID_ARGUMENT
     assert "key_scales" in _lib.last_error()
     sc.key_scales = sc.value_scales = 256
     a.dtype = _lib.PA_DTYPE_FLOAT32
-    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), None, None) == _lib.PA_ERR_UNSUPPORTED
+    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), None, None, None) == _lib.PA_ERR_UNSUPPORTED
     a.dtype = _lib.PA_DTYPE_BFLOAT16
     for cap in (-1.0, float("nan"), float("inf")):
         sm.softcap = cap
-        assert lib.pa_decode_ext(ctypes.byref(a), None, ctypes.byref(sm), None) == _lib.PA_ERR_INVALID_ARGUMENT
+        assert lib.pa_decode_ext(ctypes.byref(a), None, ctypes.byref(sm), None, None) == _lib.PA_ERR_INVALID_ARGUMENT
         assert "softcap" in _lib.last_error()
     sm.softcap, sm.window = 0.0, -1
-    assert lib.pa_decode_ext(ctypes.byref(a), None, ctypes.byref(sm), None) == _lib.PA_ERR_INVALID_ARGUMENT
+    assert lib.pa_decode_ext(ctypes.byref(a), None, ctypes.byref(sm), None, None) == _lib.PA_ERR_INVALID_ARGUMENT
     assert "window" in _lib.last_error()
     a.batch, sm.window = 0, 0
-    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), ctypes.byref(sm), None) == _lib.PA_OK
+    assert lib.pa_decode_ext(ctypes.byref(a), ctypes.byref(sc), ctypes.byref(sm), None, None) == _lib.PA_OK
 
 
 def _append_args(**kw):
