@@ -722,6 +722,12 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   if (ext) {
     // as below: many query rows per KV head share K/V tiles, few split the work
     if (p.GQ >= 64 && (long long)p.B * p.Hkv * ((p.GQ + 127) / 128) >= info->num_sms) {
+      if (sc == nullptr && rows16 && multiquery_policy() != kPolicyMma) {
+        g_last_kernel = "pa::prefill_umma_kernel<scored>";
+        e = pa::launch_prefill_umma_scored(p, tmk, tmv, dtype, pdl, strm);
+        if (e != cudaSuccess) return cuda_fail(e, "tcgen05 multi-query launch");
+        return PA_OK;
+      }
       g_last_kernel = "pa::prefill_mma_kernel<ext>";
       e = pa::launch_prefill_ext(p, tmk, tmv, dtype, pdl, strm);
       if (e != cudaSuccess) return cuda_fail(e, "multi-query launch");

@@ -247,6 +247,9 @@ cudaError_t launch_prefill_ext(const DecodeParams& p, const CUtensorMap& tmk, co
                                bool pdl, cudaStream_t stream);
 cudaError_t launch_prefill_umma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                 bool pdl, cudaStream_t stream);
+// With changed scores (p.scored).
+cudaError_t launch_prefill_umma_scored(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                                       int dtype, bool pdl, cudaStream_t stream);
 // The same on pairs of SMs (tcgen05 cta_group::2, clusters of 2 CTAs): head_dim
 // 128 (p.D), block_size >= 16 only.
 cudaError_t launch_prefill_umma2(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,

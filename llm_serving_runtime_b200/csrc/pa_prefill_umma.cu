@@ -37,10 +37,22 @@
 // store) only when a chunk raises the row max by more than 2^8, so p stays
 // below 256 and the arithmetic is exact; most chunks skip the rescale.  Every
 // wait is bounded; TMEM is always released before the CTA exits.
+//
+// kScored (pa_decode_ext's modifiers on 16-bit caches; arithmetic and masks as in
+// pa_tile_ext.cuh): a CTA streams from the first to the last key that one of its
+// rows sees; a thread caps, biases and masks its row's scores in registers
+// (a cap costs two more instructions of the exponential's unit a score).  A
+// V row that is not finite would reach rows that do not see it through their zero
+// weights (0 * inf), and 128 rows share one MMA: chunks that some row sees only in
+// part are looked over, and a CTA that finds such a row computes its own rows anew
+// on CUDA cores, key by key.  4 x 1021 tokens of packed documents: 200 us on the
+// mma.sync kernel, figures of this one in the launcher's rule (pa_capi.cu).
+#include <limits.h>
 #include <math.h>
 
 #include "pa_common.cuh"
 #include "pa_internal.h"
+#include "pa_tile_ext.cuh"
 #include "pa_tile_math.cuh"
 
 namespace pa {
@@ -158,6 +170,48 @@ __device__ __forceinline__ void split_bf16_pair(float p0, float p1, uint32_t& hi
   lo = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x7632);
 }
 
+// A CTA's rows once more, key by key, a row a warp at a time: the rare case that
+// a V row some row must not see is not finite.  Query row qr of KV head h of
+// sequence b; lanes span the columns.
+template <typename T>
+__device__ __forceinline__ void attend_row_plain(const DecodeParams& p, int b, int h, int L, int qr, int lane) {
+  const int t = qr / p.G, g = qr - t * p.G;
+  const T* qrow = static_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)(h * p.G + g) * p.q_sh +
+                  (long long)t * p.q_st;
+  T* orow = static_cast<T*>(p.out) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + (long long)t * p.o_st;
+  const KeyRange kr = row_keys<true>(p, b, L, t);
+  const float slope = p.alibi_slopes != nullptr ? p.alibi_slopes[h * p.G + g] * 1.4426950408889634f : 0.f;
+  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) q[k] = lane + 32 * k < p.Dv ? (float)qrow[lane + 32 * k] : 0.f;
+  for (int j = kr.first; j < kr.end; ++j) {
+    const int phys = p.block_tables[(long long)b * p.bt_stride + j / p.bs];
+    if (phys < 0 || phys >= p.num_blocks) continue;  // flagged by the producer
+    const T* krow = static_cast<const T*>(p.k_cache) + phys * p.k_sblk + h * p.k_sh + (j % p.bs) * p.k_st;
+    const T* vrow = static_cast<const T*>(p.v_cache) + phys * p.v_sblk + h * p.v_sh + (j % p.bs) * p.v_st;
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane + 32 * k < p.Dv) x = fmaf(q[k], (float)krow[lane + 32 * k], x);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
+    x *= p.scale_log2;
+    if (p.softcap_log2 > 0.f) x = softcap_log2(x, p.softcap_log2, p.inv_softcap_log2);
+    x = fmaf(-slope, fabsf((float)(L - p.q_len + t - j)), x);
+    const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
+    const float a = ex2(m - base), w = ex2(x - base);
+    l = fmaf(l, a, w);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane + 32 * k < p.Dv) o[k] = fmaf(w, (float)vrow[lane + 32 * k], o[k] * a);
+    m = mn;
+  }
+  const float inv = row_norm<T>(l, kr.first < kr.end);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (lane + 32 * k < p.Dv) orow[lane + 32 * k] = from_float<T>(o[k] * inv);
+}
+
 // Byte offset of 16-byte chunk `c` of row `r` in a 128-byte-swizzled region.
 __device__ __forceinline__ uint32_t sw128_chunk(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
 
@@ -169,7 +223,7 @@ __device__ __forceinline__ uint32_t sw128_chunk(int r, int c) { return (uint32_t
 // group, kv head) -- row r is row r % GQ of member r / GQ -- attends the
 // group's shared blocks in the split's token range through the first member's
 // block table, and leaves (m, l, unnormalised O) per row.
-template <typename T, int D, bool kPrefix>
+template <typename T, int D, bool kPrefix, bool kScored = false>
 __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
     prefill_umma_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                         const DecodeParams p) {
@@ -194,6 +248,9 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
   uint64_t* q_ready = pv_done + 4;       // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 1);
   __shared__ int s_last;
+  // Changed scores: keys that some / every row of the CTA sees, and whether a V row
+  // that is not finite turned up among keys some row does not see.
+  __shared__ int s_lo, s_hi, s_full_lo, s_full_hi, s_odd;
 
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -256,6 +313,28 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
     kv_lo = 0;
     kv_end = L;
     n_chunks = lim_cta < 0 ? 0 : (lim_cta + kChunk) / kChunk;
+    if constexpr (kScored) {
+      if (tid == 0) {
+        s_lo = s_full_hi = INT_MAX;
+        s_hi = s_full_lo = s_odd = 0;
+      }
+      __syncthreads();
+      if (tid < rows_cta) {
+        const KeyRange kr = row_keys<true>(p, b_kv, L, (row0 + tid) / p.G);
+        if (kr.first < kr.end) {
+          atomicMin(&s_lo, kr.first);
+          atomicMax(&s_hi, kr.end);
+        }
+        atomicMax(&s_full_lo, kr.first);
+        atomicMin(&s_full_hi, kr.end);
+      }
+      __syncthreads();
+      // from the block (or 16-token unit of a larger one) of the first key
+      const int grain = min(p.bs, kUnitTokens);
+      kv_end = s_hi;
+      kv_lo = s_lo < s_hi ? s_lo / grain * grain : 0;
+      n_chunks = s_lo < s_hi ? (kv_end - kv_lo + kChunk - 1) / kChunk : 0;
+    }
   }
   const int ntiles = (row0 + 128 < rows_total) ? 2 : 1;  // MMA tiles holding rows
 
@@ -500,6 +579,8 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
     const bool row_ok = tile_on && qr < rows_total;
     int tq = 0, g = 0, b = b_kv;
     int lim = -1;  // last attendable position of this row
+    [[maybe_unused]] KeyRange kr = {0, 0};
+    [[maybe_unused]] float slope = 0.f;
     if (row_ok) {
       int r_in = qr;
       if constexpr (kPrefix) {
@@ -513,6 +594,10 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       const int Lb = min(max(p.context_lens[b] + p.len_offset, 0), cap);
       lim = Lb - p.q_len + tq;
       if constexpr (kPrefix) lim = min(lim, kv_end - 1);
+      if constexpr (kScored) {
+        kr = row_keys<true>(p, b, Lb, tq);
+        if (p.alibi_slopes != nullptr) slope = __ldg(&p.alibi_slopes[h * p.G + g]) * 1.4426950408889634f;
+      }
     }
     // Q rows -> swizzled K-major tile t.  The warp loads its 32 rows together,
     // whole rows per instruction (a row's 16-byte pieces from consecutive
@@ -547,6 +632,8 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem + (uint32_t)(t * 256) + lane_base;  // S / P buffers of this tile
     const uint32_t t_o = t_s + 128u;                               // O of this tile
+    // scores that are more than scaled and masked
+    [[maybe_unused]] const bool changed = p.softcap_log2 > 0.f || p.alibi_slopes != nullptr || !(p.scale_log2 > 0.f);
     float m_ref = -INFINITY;  // reference max (log2 domain) of this row
     float l = 0.f;
     bool ok = true;
@@ -570,7 +657,31 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
         }
       }
       const int tok0 = kv_lo + j * kChunk;
-      if (tok0 + kChunk - 1 > lim) {  // causal / end-of-range mask in this chunk
+      if constexpr (kScored) {
+        if (changed) {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) x[i] *= p.scale_log2;
+        }
+        if (p.softcap_log2 > 0.f) {
+          if (p.softcap <= kDirectCap) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) x[i] = softcap_direct(x[i], p.softcap_log2, p.inv_softcap_log2);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) x[i] = softcap_log2(x[i], p.softcap_log2, p.inv_softcap_log2);
+          }
+        }
+        if (p.alibi_slopes != nullptr) {
+          const float d0 = (float)(lim - tok0);  // lim is the row's own position
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) x[i] = fmaf(-slope, fabsf(d0 - (float)i), x[i]);
+        }
+        if (tok0 < kr.first || tok0 + kChunk > kr.end) {
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i)
+            if (tok0 + i < kr.first || tok0 + i >= kr.end) x[i] = -INFINITY;
+        }
+      } else if (tok0 + kChunk - 1 > lim) {  // causal / end-of-range mask in this chunk
 #pragma unroll
         for (int i = 0; i < kChunk; ++i)
           if (tok0 + i > lim) x[i] = -INFINITY;
@@ -578,7 +689,7 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       float mx_raw = -INFINITY;
 #pragma unroll
       for (int i = 0; i < kChunk; ++i) mx_raw = fmaxf(mx_raw, x[i]);
-      const float sl2 = p.scale_log2;  // > 0, so max(x * s) = s * max(x)
+      const float sl2 = kScored && changed ? 1.f : p.scale_log2;  // > 0, so max(x * s) = s * max(x)
       const float mx = mx_raw * sl2;
       // reference max: move it (and rescale O) only when the row max grows a lot
       float alpha = 1.f;
@@ -633,7 +744,32 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       // there).  Tile 0's warpgroup does it before its P is published; the PV of
       // tile 1 is issued after tile 0's, so it sees the zeros too.
       const int valid = kv_end - tok0;
-      if (t == 0 && valid < kChunk) {
+      if constexpr (kScored) {
+        // Keys that some row does not see: thread r looks over half of V row r / 2.
+        // (The chunk's own barrier has completed; waiting on it here makes the
+        // copied bytes visible to this thread.)
+        if (t == 0 && (tok0 < s_full_lo || tok0 + kChunk > s_full_hi)) {
+          if (!mbar_test_then_wait(smem_addr(&kv_full[j % S]), (uint32_t)((j / S) & 1))) {
+            ok = false;
+            break;
+          }
+          uint8_t* vbase = s_kv + (j % S) * KV_BYTES + HALVES * HALF_BYTES;
+          const int row = r >> 1, tok = tok0 + row;
+          const bool seen = tok >= s_lo && tok < kv_end;
+          bool odd = false;
+#pragma unroll
+          for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint4* at = reinterpret_cast<uint4*>(vbase + hf * HALF_BYTES + row * 128 + (r & 1) * 64 + c * 16);
+              const uint4 v = *at;
+              odd |= not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w);
+              if (!seen) *at = make_uint4(0u, 0u, 0u, 0u);
+            }
+          if (odd && seen) s_odd = 1;
+          fence_proxy_async_smem();
+        }
+      } else if (t == 0 && valid < kChunk) {
         uint8_t* vbase = s_kv + (j % S) * KV_BYTES + HALVES * HALF_BYTES;
         const int nrows = kChunk - valid;
         for (int i = r; i < nrows * HALVES * 8; i += 128) {
@@ -769,7 +905,8 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
     } else {
       T* orow = static_cast<T*>(p.out) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh +
                 (long long)tq * p.o_st;
-      const float inv = (ok && l > 0.f) ? 1.f / l : 0.f;
+      float inv = (ok && l > 0.f) ? 1.f / l : 0.f;
+      if constexpr (kScored) inv = ok ? row_norm<T>(l, kr.first < kr.end) : 0.f;
       // As in the prefix epilogue: the warp's rows go out through shared
       // memory (this tile's Q tile, free once its last P.V has completed),
       // whole rows per store instruction.
@@ -835,6 +972,14 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
           }
         }
       }
+      if constexpr (kScored) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
+        if (*reinterpret_cast<volatile int*>(&s_odd) != 0) {
+          const int L = min(max(p.context_lens[b_kv] + p.len_offset, 0), cap);
+          const int first = row0 + warp * 32, last = min(first + 32, rows_total);
+          for (int i = first; i < last; ++i) attend_row_plain<T>(p, b_kv, h, L, i, lane);
+        }
+      }
     }
   }
 
@@ -852,7 +997,7 @@ size_t prefill_umma_smem_bytes(int D) {
   return 1024 + stages * 2 * halves * kChunk * 128 + 2 * halves * 128 * 128 + 256;
 }
 
-template <typename T, int D, bool kPrefix>
+template <typename T, int D, bool kPrefix, bool kScored = false>
 static cudaError_t launch_umma_impl(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, bool pdl,
                                     cudaStream_t stream) {
   const size_t smem = prefill_umma_smem_bytes(D);
@@ -860,7 +1005,7 @@ static cudaError_t launch_umma_impl(const DecodeParams& p, const CUtensorMap& tm
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !prepared[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_umma_kernel<T, D, kPrefix>,
+    cudaError_t e = cudaFuncSetAttribute(prefill_umma_kernel<T, D, kPrefix, kScored>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     prepared[dev] = true;
@@ -878,18 +1023,18 @@ static cudaError_t launch_umma_impl(const DecodeParams& p, const CUtensorMap& tm
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl ? attr : nullptr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, prefill_umma_kernel<T, D, kPrefix>, tmk, tmv, p);
+  return cudaLaunchKernelEx(&cfg, prefill_umma_kernel<T, D, kPrefix, kScored>, tmk, tmv, p);
 }
 
-template <bool kPrefix>
+template <bool kPrefix, bool kScored = false>
 static cudaError_t launch_umma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                bool pdl, cudaStream_t stream) {
   if (dtype == PA_DTYPE_BFLOAT16) {
-    if (p.D == 128) return launch_umma_impl<__nv_bfloat16, 128, kPrefix>(p, tmk, tmv, pdl, stream);
-    if (p.D == 64) return launch_umma_impl<__nv_bfloat16, 64, kPrefix>(p, tmk, tmv, pdl, stream);
+    if (p.D == 128) return launch_umma_impl<__nv_bfloat16, 128, kPrefix, kScored>(p, tmk, tmv, pdl, stream);
+    if (p.D == 64) return launch_umma_impl<__nv_bfloat16, 64, kPrefix, kScored>(p, tmk, tmv, pdl, stream);
   } else if (dtype == PA_DTYPE_FLOAT16) {
-    if (p.D == 128) return launch_umma_impl<__half, 128, kPrefix>(p, tmk, tmv, pdl, stream);
-    if (p.D == 64) return launch_umma_impl<__half, 64, kPrefix>(p, tmk, tmv, pdl, stream);
+    if (p.D == 128) return launch_umma_impl<__half, 128, kPrefix, kScored>(p, tmk, tmv, pdl, stream);
+    if (p.D == 64) return launch_umma_impl<__half, 64, kPrefix, kScored>(p, tmk, tmv, pdl, stream);
   }
   return cudaErrorInvalidValue;
 }
@@ -897,6 +1042,11 @@ static cudaError_t launch_umma(const DecodeParams& p, const CUtensorMap& tmk, co
 cudaError_t launch_prefill_umma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                 bool pdl, cudaStream_t stream) {
   return launch_umma<false>(p, tmk, tmv, dtype, pdl, stream);
+}
+
+cudaError_t launch_prefill_umma_scored(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv,
+                                       int dtype, bool pdl, cudaStream_t stream) {
+  return launch_umma<false, true>(p, tmk, tmv, dtype, pdl, stream);
 }
 
 cudaError_t launch_prefix_umma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,

@@ -105,8 +105,30 @@ def test_several_tokens(dtype, kind):
 @pytest.mark.parametrize("dtype,D,bs", [(BF, 128, 16), (HF, 64, 8), (FP8, 128, 32), (FP8, 64, 8)])
 def test_chunks(dtype, D, bs, kind):
     lens = [0, 40, 97, 16, 3] * 4
-    kernel = f"pa::prefill_mma_kernel<{'ext'}>"
+    kernel = "pa::prefill_mma_kernel<ext>" if dtype == FP8 else "pa::prefill_umma_kernel<scored>"
     _run(_setup(dtype, lens, 37, 16, 8, D, bs, 3), _mods(kind, lens, 37, 16), kernel=kernel)
+
+
+@pytest.mark.parametrize("kind", ["all", "documents", "window"])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_chunks_of_unaligned_rows(dtype, kind):
+    """Query rows that are not 16-byte aligned go to the mma.sync kernel."""
+    lens = [0, 40, 97, 16, 3] * 4
+    s = list(_setup(dtype, lens, 37, 16, 8, 64, 16, 3))
+    wide = torch.zeros(20, 16, 37, 66, dtype=dtype, device="cuda")
+    wide[..., 2:] = s[0]
+    s[0] = wide[..., 2:]
+    _run(s, _mods(kind, lens, 37, 16), kernel="pa::prefill_mma_kernel<ext>")
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_long_chunks(dtype):
+    """Several row blocks and chunks a sequence; documents, windows and a prefix across them."""
+    lens = [5, 300, 130, 700, 64, 0, 411]
+    s = _setup(dtype, lens, 150, 16, 8, 64, 16, 30)
+    _run(s, ScoreModifiers(key_starts=_starts(lens, 150, 110), softcap=8.0), kernel="pa::prefill_umma_kernel<scored>")
+    _run(s, ScoreModifiers(window=70, alibi_slopes=_slopes(16)), kernel="pa::prefill_umma_kernel<scored>")
+    _run(s, ScoreModifiers(prefix_lens=_i32([333] * 7)), kernel="pa::prefill_umma_kernel<scored>")
 
 
 @pytest.mark.parametrize("Hq,Hkv,D,bs", [(14, 2, 64, 16), (4, 4, 96, 8), (16, 1, 128, 64), (8, 2, 32, 256), (6, 3, 80, 32)])
