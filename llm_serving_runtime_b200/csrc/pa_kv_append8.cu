@@ -15,18 +15,25 @@
 // 2^-6 * scale).  A scale found in the cache need not be a power of two.
 //
 // A block's codes and scale have to be written together, so the work item is a
-// run: all tokens of one call for one block.  One CTA takes a run, its warps
-// take (head, K or V) pairs in turn.  Through a block table a row's runs follow
+// run: all tokens of one call for one block.  A CTA takes a run and up to eight
+// (head, K or V) pairs of it, a warp each.  Through a block table a row's runs follow
 // from its position; through slot_mapping the CTA of each token looks whether
 // that token opens a run (the row's previous slot lies in another block).  Two
 // runs of one call in one block would race, so a CTA looks for an earlier run in
-// its block first; it then leaves its own unwritten and flags it.  The runs'
-// bytes are few, so latency decides; measured figures stand at the launcher.
+// its block first; it then leaves its own unwritten and flags it.
+//
+// The bytes are few, so latency decides: a warp loads its share of the run (up to
+// 256 pieces of 8 elements, a 16-token block of 128 columns) into registers at once,
+// before the look at the other runs, and rounds it from there; longer runs
+// are read twice.  Four CTAs an SM (64 registers) hold a prefill chunk in one wave.
+// Measured: 8 x 509 tokens, 8 heads of 128 (25 MB) 9.3 us (18.5 with a warp reading
+// piece by piece for two pairs, 20.9 with two CTAs an SM); 64 rows of one token 4.3 us.
 #include <cuda_fp8.h>
 #include <math.h>
 
 #include "pa_common.cuh"
 #include "pa_internal.h"
+#include "pa_tile_math.cuh"
 
 namespace pa {
 
@@ -34,39 +41,45 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxBlock = 256;  // tokens of a block
+constexpr int kBatch = 8;       // pieces of 8 elements that a lane holds
 
+// Eight neighbouring elements as they are in memory, and widened; kWide: loaded
+// 16 bytes at a time.
 template <typename T>
-__device__ __forceinline__ float widen(T x);
-template <>
-__device__ __forceinline__ float widen<float>(float x) {
-  return x;
-}
-template <>
-__device__ __forceinline__ float widen<__half>(__half x) {
-  return __half2float(x);
-}
-template <>
-__device__ __forceinline__ float widen<__nv_bfloat16>(__nv_bfloat16 x) {
-  return __bfloat162float(x);
-}
+struct Piece {
+  static constexpr int kWords = 8 * sizeof(T) / 4;
+  uint32_t w[kWords];
 
-// Eight neighbouring elements; kWide: as 16-byte loads.
-template <typename T, bool kWide>
-__device__ __forceinline__ void load8(const T* src, float (&x)[8]) {
-  if constexpr (kWide) {
-    constexpr int N = 16 / sizeof(T);
+  template <bool kWide>
+  __device__ __forceinline__ void load(const T* src) {
+    if constexpr (kWide) {
 #pragma unroll
-    for (int i = 0; i < 8 / N; ++i) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
-      const T* e = reinterpret_cast<const T*>(&v);
+      for (int i = 0; i < kWords / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src) + i);
+        w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) x[i * N + j] = widen<T>(e[j]);
+      for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(__ldg(src + i));
+    } else {
+      const unsigned short* u = reinterpret_cast<const unsigned short*>(src);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__ldg(u + 2 * i) | ((uint32_t)__ldg(u + 2 * i + 1) << 16);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = widen<T>(__ldg(src + i));
   }
-}
+  __device__ __forceinline__ void widen(float (&x)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x[2 * i] = lo_half<T>(w[i]);
+        x[2 * i + 1] = hi_half<T>(w[i]);
+      }
+    }
+  }
+};
 
 __device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
@@ -102,36 +115,52 @@ __device__ __forceinline__ long long first_position(const AppendParams& p, int b
 }  // namespace
 
 template <typename T, bool kWide>
-__global__ void __launch_bounds__(kThreads) kv_append8_kernel(const AppendParams p, const ScaleParams sc,
-                                                              const int runs_per_row, const int bs_log2) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
+    kv_append8_kernel(const AppendParams p, const ScaleParams sc, const int runs_per_row, const int bs_log2,
+                      const int chunks_log2) {
   // the attention that follows may start its prologue; it waits for every write below
   pdl_launch_dependents();
-  __shared__ int s_token[kMaxBlock];  // token of the row written at each offset, -1: none
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // The run's tokens: offset in the block (low byte) and token of the row, in any
+  // order; and which offsets of the block they take.
+  __shared__ int2 s_run[kMaxBlock];
+  __shared__ int s_token[kMaxBlock];  // slot form: token of the row at each offset, -1: none
+  __shared__ int s_count;
+  __shared__ uint32_t s_taken[kMaxBlock / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int b = blockIdx.x / runs_per_row, k = blockIdx.x - b * runs_per_row;
   const int bs = 1 << bs_log2;
-  for (int o = tid; o < bs; o += kThreads) s_token[o] = -1;
-  __syncthreads();
+
+  // Block of run r of the call (-1: none), for the look at earlier runs.
+  auto block_of_run = [&](int r) -> long long {
+    const int b2 = r / runs_per_row;
+    const long long q0 = first_position(p, b2);
+    const long long lb2 = ((q0 < 0 ? 0 : q0) >> bs_log2) + (r - b2 * runs_per_row);
+    return ((lb2 << bs_log2) < q0 + p.q_len) && q0 + p.q_len > 0 ? table_block(p, b2, lb2) : -1;
+  };
+  // (the first of them in flight beside this run's own)
+  const bool tables = p.slot_mapping == nullptr;
+  const long long other = tables && tid < (int)blockIdx.x ? block_of_run(tid) : -1;
 
   long long blk;
-  bool earlier = false;  // another run of the call writes this block before this one
-  if (p.slot_mapping == nullptr) {
+  int count;
+  if (tables) {
     const long long pos0 = first_position(p, b);
-    if (pos0 < 0 && k == 0 && tid == 0) raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
+    if (pos0 < 0 && k == 0 && tid == 0 && blockIdx.y == 0) raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
     const long long lb = ((pos0 < 0 ? 0 : pos0) >> bs_log2) + k;
     const long long t0 = max(0LL, (lb << bs_log2) - pos0), t1 = min((long long)p.q_len, ((lb + 1) << bs_log2) - pos0);
     if (t0 >= t1) return;
     if (lb >= p.max_blocks) {
-      if (tid == 0) raise_flag(p.error_flags, PA_DEVERR_TABLE_UNDERRUN);
+      if (tid == 0 && blockIdx.y == 0) raise_flag(p.error_flags, PA_DEVERR_TABLE_UNDERRUN);
       return;
     }
     blk = table_block(p, b, lb);
-    for (long long t = t0 + tid; t < t1; t += kThreads) s_token[(int)((pos0 + t) & (bs - 1))] = (int)t;
-    for (int r = tid; r < (int)blockIdx.x; r += kThreads) {
-      const int b2 = r / runs_per_row;
-      const long long q0 = first_position(p, b2);
-      const long long lb2 = ((q0 < 0 ? 0 : q0) >> bs_log2) + (r - b2 * runs_per_row);
-      if (((lb2 << bs_log2) < q0 + p.q_len) && q0 + p.q_len > 0) earlier |= table_block(p, b2, lb2) == blk;
+    count = (int)(t1 - t0);
+    for (int i = tid; i < count; i += threads) s_run[i] = make_int2((int)((pos0 + t0 + i) & (bs - 1)), (int)t0 + i);
+    if (tid < kMaxBlock / 32) {  // offsets first .. first + count - 1
+      const int first = (int)((pos0 + t0) & (bs - 1)) - 32 * tid, last = first + count;
+      const uint32_t from = first <= 0 ? ~0u : first >= 32 ? 0u : ~0u << first;
+      const uint32_t to = last >= 32 ? ~0u : last <= 0 ? 0u : ~(~0u << last);
+      s_taken[tid] = from & to;
     }
   } else {
     const int64_t* row = p.slot_mapping + (long long)b * p.q_len;
@@ -140,97 +169,161 @@ __global__ void __launch_bounds__(kThreads) kv_append8_kernel(const AppendParams
     int prev = k - 1;
     while (prev >= 0 && row[prev] < 0) --prev;
     if (prev >= 0 && (row[prev] >> bs_log2) == blk) return;  // not the first token of its run
+    for (int o = tid; o < bs; o += threads) s_token[o] = -1;
+    if (tid < kMaxBlock / 32) s_taken[tid] = 0u;
+    if (tid == 0) s_count = 0;
+    __syncthreads();
     // the run: up to the next slot of another block
     int end = k + 1;
     while (end < p.q_len && (row[end] < 0 || (row[end] >> bs_log2) == blk)) ++end;
-    for (int t = k + tid; t < end; t += kThreads)
+    for (int t = k + tid; t < end; t += threads)
       if (row[t] >= 0) atomicMax(&s_token[(int)(row[t] & (bs - 1))], t);  // a slot given twice: the last one
-    for (int i = tid; i < (int)blockIdx.x; i += kThreads)
+    __syncthreads();
+    for (int o = tid; o < bs; o += threads)
+      if (s_token[o] >= 0) {
+        s_run[atomicAdd(&s_count, 1)] = make_int2(o, s_token[o]);
+        atomicOr(&s_taken[o >> 5], 1u << (o & 31));
+      }
+    __syncthreads();
+    count = s_count;
+  }
+  __syncthreads();  // the run is complete
+
+  // ---- this warp's pair: K or V of one head ----
+  const int hv = blockIdx.y * (kThreads / 32) + warp;
+  const bool mine = hv < 2 * p.Hkv;
+  const int h = hv >> 1;
+  const bool is_v = hv & 1;
+  const int chunks = p.D >> 3;  // of 8 elements
+  const int items = mine ? count * chunks : 0;
+  const T* src = is_v ? static_cast<const T*>(p.value) + (long long)b * p.v_sb + (long long)h * p.v_sh
+                      : static_cast<const T*>(p.key) + (long long)b * p.k_sb + (long long)h * p.k_sh;
+  const int64_t src_t = is_v ? p.v_st : p.k_st;
+  // Piece i of the run: 8 elements from column 8 c of its i / chunks-th token.
+  auto token_of = [&](int i) -> int { return chunks_log2 >= 0 ? i >> chunks_log2 : i / chunks; };
+  Piece<T> x[kBatch];
+  auto load = [&](int base) {
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      const int i = base + n * 32 + lane;
+      if (i >= items) continue;
+      const int r = token_of(i);
+      x[n].template load<kWide>(src + s_run[r].y * src_t + (i - r * chunks) * 8);
+    }
+  };
+  load(0);
+  const bool in_pool = blk >= 0 && blk < p.num_blocks;
+  float* scale_at = is_v ? sc.v_scales + blk * sc.vs_sblk + h * sc.vs_sh
+                         : sc.k_scales + blk * sc.ks_sblk + h * sc.ks_sh;
+  float held = in_pool && mine ? *scale_at : 0.f;
+
+  bool earlier = other == blk && blk >= 0;  // another run of the call writes this block before this one
+  if (tables) {
+    for (int r = tid + threads; r < (int)blockIdx.x; r += threads) earlier |= block_of_run(r) == blk;
+  } else {
+    for (int i = tid; i < (int)blockIdx.x; i += threads)
       earlier |= p.slot_mapping[i] >= 0 && (p.slot_mapping[i] >> bs_log2) == blk;
   }
-  const bool any_earlier = __syncthreads_or(earlier);  // also: s_token is complete
-  if (blk < 0 || blk >= p.num_blocks) {
-    if (tid == 0)
+  const bool any_earlier = __syncthreads_or(earlier);
+  if (!in_pool) {
+    if (tid == 0 && blockIdx.y == 0)
       raise_flag(p.error_flags, p.slot_mapping != nullptr ? PA_DEVERR_SLOT_RANGE : PA_DEVERR_BLOCK_ID_RANGE);
     return;
   }
   if (any_earlier) {
-    if (tid == 0) raise_flag(p.error_flags, PA_DEVERR_BLOCK_CONFLICT);
+    if (tid == 0 && blockIdx.y == 0) raise_flag(p.error_flags, PA_DEVERR_BLOCK_CONFLICT);
     return;
   }
-  const bool fresh = s_token[0] >= 0;
-  const int chunks = p.D >> 3;  // of 8 elements
-  const int items = bs * chunks;
+  if (!mine) return;
+  const bool fresh = s_taken[0] & 1u;
+  uint8_t* dst = is_v ? static_cast<uint8_t*>(p.v_cache) + blk * p.vc_sblk + (long long)h * p.vc_sh
+                      : static_cast<uint8_t*>(p.k_cache) + blk * p.kc_sblk + (long long)h * p.kc_sh;
+  const int64_t dst_t = is_v ? p.vc_st : p.kc_st;
+  held = (!fresh && held > 0.f && held < INFINITY) ? held : 0.f;
 
-  for (int hv = warp; hv < 2 * p.Hkv; hv += kThreads / 32) {
-    const int h = hv >> 1;
-    const bool is_v = hv & 1;
-    const T* src = is_v ? static_cast<const T*>(p.value) + (long long)b * p.v_sb + (long long)h * p.v_sh
-                        : static_cast<const T*>(p.key) + (long long)b * p.k_sb + (long long)h * p.k_sh;
-    const int64_t src_t = is_v ? p.v_st : p.k_st;
-    uint8_t* dst = is_v ? static_cast<uint8_t*>(p.v_cache) + blk * p.vc_sblk + (long long)h * p.vc_sh
-                        : static_cast<uint8_t*>(p.k_cache) + blk * p.kc_sblk + (long long)h * p.kc_sh;
-    const int64_t dst_t = is_v ? p.vc_st : p.kc_st;
-    float* scale_at = is_v ? sc.v_scales + blk * sc.vs_sblk + h * sc.vs_sh
-                           : sc.k_scales + blk * sc.ks_sblk + h * sc.ks_sh;
-    float held = *scale_at;
-    held = (!fresh && held > 0.f && held < INFINITY) ? held : 0.f;
-
-    float amax = 0.f;
-    for (int i = lane; i < items; i += 32) {
-      const int o = i / chunks, t = s_token[o];
-      if (t < 0) continue;
-      float x[8];
-      load8<T, kWide>(src + t * src_t + (i - o * chunks) * 8, x);
+  float amax = 0.f;
+  for (int base = 0; base < items; base += kBatch * 32) {
+    if (base > 0) load(base);
+#pragma unroll
+    for (int n = 0; n < kBatch; ++n) {
+      if (base + n * 32 + lane >= items) continue;
+      float v[8];
+      x[n].widen(v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float a = fabsf(x[j]);
+        const float a = fabsf(v[j]);
         if (a < INFINITY) amax = fmaxf(amax, a);  // not for NaN either
       }
     }
+  }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float scale = fmaxf(held, needed_scale(amax));
-    const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0u;
-    const float inv = 1.f / scale;  // exact where scale is a power of two
-    for (int i = lane; i < items; i += 32) {
-      const int o = i / chunks, t = s_token[o];
-      if (t < 0) continue;
-      float x[8];
-      load8<T, kWide>(src + t * src_t + (i - o * chunks) * 8, x);
+  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float scale = fmaxf(held, needed_scale(amax));
+  const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0u;
+  const float inv = 1.f / scale;  // exact where scale is a power of two
+  for (int base = 0; base < items; base += kBatch * 32) {
+    if (items > kBatch * 32) load(base);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = pow2 ? x[j] * inv : __fdiv_rn(x[j], scale);
-      *reinterpret_cast<uint2*>(dst + o * dst_t + (i - o * chunks) * 8) =
-          make_uint2(codes4(x[0], x[1], x[2], x[3]), codes4(x[4], x[5], x[6], x[7]));
+    for (int n = 0; n < kBatch; ++n) {
+      const int i = base + n * 32 + lane;
+      if (i >= items) continue;
+      float v[8];
+      x[n].widen(v);
+      if (pow2) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], scale);
+      }
+      const int r = token_of(i);
+      *reinterpret_cast<uint2*>(dst + s_run[r].x * dst_t + (i - r * chunks) * 8) =
+          make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
     }
-    if (!fresh && scale != held) {
-      const float ratio = __fdiv_rn(held, scale);
-      for (int i = lane; i < items; i += 32) {
-        const int o = i / chunks;
-        if (s_token[o] >= 0) continue;
-        uint2* at = reinterpret_cast<uint2*>(dst + o * dst_t + (i - o * chunks) * 8);
-        const uint2 c = *at;
-        float2 f[4] = {two_values(c.x), two_values(c.x >> 16), two_values(c.y), two_values(c.y >> 16)};
+  }
+  if (!fresh && scale != held) {
+    // the block's other tokens to the new scale
+    const float ratio = __fdiv_rn(held, scale);
+    for (int base = 0; base < bs * chunks; base += kBatch * 32) {
+      uint2 c[kBatch];
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int i = base + n * 32 + lane, o = token_of(i);
+        if (i < bs * chunks && !((s_taken[o >> 5] >> (o & 31)) & 1u))
+          c[n] = *reinterpret_cast<const uint2*>(dst + o * dst_t + (i - o * chunks) * 8);
+      }
+#pragma unroll
+      for (int n = 0; n < kBatch; ++n) {
+        const int i = base + n * 32 + lane, o = token_of(i);
+        if (i >= bs * chunks || ((s_taken[o >> 5] >> (o & 31)) & 1u)) continue;
+        float2 f[4] = {two_values(c[n].x), two_values(c[n].x >> 16), two_values(c[n].y), two_values(c[n].y >> 16)};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           f[j].x *= ratio;
           f[j].y *= ratio;
         }
-        *at = make_uint2(codes4(f[0].x, f[0].y, f[1].x, f[1].y), codes4(f[2].x, f[2].y, f[3].x, f[3].y));
+        *reinterpret_cast<uint2*>(dst + o * dst_t + (i - o * chunks) * 8) =
+            make_uint2(codes4(f[0].x, f[0].y, f[1].x, f[1].y), codes4(f[2].x, f[2].y, f[3].x, f[3].y));
       }
     }
-    if (lane == 0 && (fresh || scale != held)) *scale_at = scale;
   }
+  if (lane == 0 && (fresh || scale != held)) *scale_at = scale;
 }
 
 template <typename T>
 static cudaError_t launch_typed(const AppendParams& p, const ScaleParams& sc, bool wide, int runs, int bs_log2,
                                 cudaStream_t stream) {
-  const unsigned grid = (unsigned)((long long)p.B * runs);
+  const int pairs = 2 * p.Hkv, warps = kThreads / 32;
+  const dim3 grid((unsigned)((long long)p.B * runs), (unsigned)((pairs + warps - 1) / warps));
+  const int threads = pairs < warps ? 32 * pairs : kThreads;
+  const int chunks = p.D / 8;
+  int chunks_log2 = -1;  // of a power of two
+  if ((chunks & (chunks - 1)) == 0)
+    for (chunks_log2 = 0; (1 << chunks_log2) < chunks;) ++chunks_log2;
   if (wide)
-    kv_append8_kernel<T, true><<<grid, kThreads, 0, stream>>>(p, sc, runs, bs_log2);
+    kv_append8_kernel<T, true><<<grid, threads, 0, stream>>>(p, sc, runs, bs_log2, chunks_log2);
   else
-    kv_append8_kernel<T, false><<<grid, kThreads, 0, stream>>>(p, sc, runs, bs_log2);
+    kv_append8_kernel<T, false><<<grid, threads, 0, stream>>>(p, sc, runs, bs_log2, chunks_log2);
   return cudaGetLastError();
 }
 
