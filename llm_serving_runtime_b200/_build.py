@@ -22,7 +22,7 @@ LIB_PATH = LIB_DIR / "libpa_b200.so"
 
 SOURCES = ["pa_capi.cu", "pa_kv_append.cu", "pa_decode_mma.cu", "pa_decode_f32.cu", "pa_static_ws.cu",
            "pa_prefill_mma.cu", "pa_prefill_umma.cu", "pa_prefill_umma2.cu", "pa_decode_ext.cu", "pa_decode_direct.cu",
-           "pa_kv_append8.cu",
+           "pa_decode_f32_ext.cu", "pa_kv_append8.cu",
            "pa_pages.cu"]
 HEADERS = ["pa_common.cuh", "pa_internal.h", "pa_tile_math.cuh", "pa_tile_ext.cuh", "pa_decode_kernel.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -303,7 +303,9 @@ size_t pa_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num
   DeviceInfo* info = nullptr;
   if (device_info(device, &info) != PA_OK) return 0;
   const DecodeShape s = decode_shape(num_q_heads, num_kv_heads, q_len);
-  if (dtype == PA_DTYPE_FLOAT32) return pa::kWsHeaderBytes;
+  if (dtype == PA_DTYPE_FLOAT32)  // what pa_decode_ext needs; pa_decode takes the header alone
+    return pa::kWsFixedBytes + pa::ws_counter_bytes(info->num_sms * pa::kDecodeWarps) +
+           pa::f32_ext_partial_bytes(info->num_sms);
   const int DP = padded_head_dim(head_dim, dtype);
   if (DP == 0) return pa::kWsHeaderBytes;  // not served: pa_decode itself reports it
   return workspace_bytes_impl(s.slot_rows, DP, info->num_sms * pa::kDecodeWarps);
@@ -634,6 +636,19 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   if (dtype == PA_DTYPE_FLOAT32) {
     if (!aligned_ptr(a->key_cache.data, 4) || !aligned_ptr(a->value_cache.data, 4))
       return fail(PA_ERR_UNSUPPORTED, "cache base must be 4-byte aligned");
+    if (sm != nullptr) {
+      const int nw = info->num_sms * pa::kDecodeWarps;
+      const size_t need = pa::kWsFixedBytes + pa::ws_counter_bytes(nw) + pa::f32_ext_partial_bytes(info->num_sms);
+      if (a->workspace_bytes < need)
+        return fail(PA_ERR_WORKSPACE, "workspace too small: %zu bytes given, %zu needed", a->workspace_bytes, need);
+      char* ws = static_cast<char*>(a->workspace);
+      p.counters = reinterpret_cast<int32_t*>(ws + pa::kWsFixedBytes);
+      p.partials = reinterpret_cast<float*>(ws + pa::kWsFixedBytes + pa::ws_counter_bytes(nw));
+      g_last_kernel = "pa::decode_f32_ext_kernel";
+      e = pa::launch_decode_f32_ext(p, info->num_sms, pdl, strm);
+      if (e != cudaSuccess) return cuda_fail(e, "decode_f32_ext launch");
+      return PA_OK;
+    }
     g_last_kernel = "pa::decode_f32_kernel";
     e = pa::launch_decode_f32(p, pdl, strm);
     if (e != cudaSuccess) return cuda_fail(e, "decode_f32 launch");

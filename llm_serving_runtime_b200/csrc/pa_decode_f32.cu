@@ -17,12 +17,6 @@
 // for all rows, then own D/32 output dims for the P.V update.  At the end the
 // warps' states are merged with the log-sum-exp rule.  The fp32 configurations
 // are small, so this kernel aims at latency: many warps in flight per row.
-//
-// kScored (pa_decode_ext's modifiers): scores are capped, c * tanh(s / c), and
-// biased, -slope * |i - j|, before the mask, which then is the row's key range;
-// the blocks before the sequence's first visible key are not read.  P carries -1
-// for hidden keys, whose V (0 * inf is NaN) is left out of the update.
-#include <limits.h>
 #include <math.h>
 
 #include "pa_common.cuh"
@@ -35,15 +29,9 @@ constexpr int kF32Warps = 8;
 constexpr int kF32Chunk = 16;  // tokens per staged chunk
 }  // namespace
 
-__device__ __forceinline__ KeyRange row_keys(const DecodeParams& p, int b, int L, int t) {
-  const int start = p.key_starts != nullptr ? __ldg(&p.key_starts[b * p.kst_sb + t * p.kst_st]) : 0;
-  const int prefix = p.prefix_lens != nullptr ? __ldg(&p.prefix_lens[b]) : 0;
-  return key_range(L, p.q_len, t, p.window, start, prefix);
-}
-
 // DPL = head_dim / 32; kF32Rows = query rows handled per pass (4, 8 or 16,
 // the smallest that holds the GQA group's G * q_len rows).
-template <int DPL, int kF32Rows, bool kScored = false>
+template <int DPL, int kF32Rows>
 __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const DecodeParams p) {
   constexpr int D = DPL * 32;
   constexpr int PITCH = D + 1;
@@ -77,15 +65,6 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
   const int first_limit = L - p.q_len;  // last token row t=0 may attend
   const int ntok_max = L;               // tokens any row may attend
   const int nblk = (ntok_max + p.bs - 1) / p.bs;
-  __shared__ int s_lo;  // changed scores: the sequence's first visible key
-  int lo = 0;
-  if constexpr (kScored) {
-    if (threadIdx.x == 0) s_lo = INT_MAX;
-    __syncthreads();
-    for (int t = threadIdx.x; t < p.q_len; t += blockDim.x) atomicMin(&s_lo, row_keys(p, b, L, t).first);
-    __syncthreads();
-    lo = min(s_lo, ntok_max);
-  }
 
   const float* kc = static_cast<const float*>(p.k_cache);
   const float* vc = static_cast<const float*>(p.v_cache);
@@ -113,7 +92,7 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
       for (int j = 0; j < DPL; ++j) acc[r][j] = 0.f;
     }
 
-    for (int blk = (kScored ? lo / p.bs : 0) + warp; blk < nblk; blk += kF32Warps) {
+    for (int blk = warp; blk < nblk; blk += kF32Warps) {
       const int phys = p.block_tables[(long long)b * p.bt_stride + blk];
       if (phys < 0 || phys >= p.num_blocks) {
         if (lane == 0) raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
@@ -126,7 +105,6 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
         const int cnt = min(kF32Chunk, take - c0);
         const int tok0 = blk * p.bs + c0;  // absolute position of the chunk's first token
         if (tok0 > first_limit + p.q_len - 1) break;  // no row attends past L - 1
-        if (kScored && tok0 + cnt <= lo) continue;
         __syncwarp();
         // Stage the chunk: every copy of the chunk is in flight at once.
 #pragma unroll 4
@@ -160,24 +138,13 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
           const int qr = r0 + r;
           const int t_q = qr - (qr / p.q_len) * p.q_len;
           const int lim = first_limit + t_q;  // last attendable position of this row
-          bool valid = lane < cnt && tok0 + lane <= lim;
-          float s = sc[r] * p.scale;
-          if constexpr (kScored) {
-            const KeyRange kr = row_keys(p, b, L, t_q);
-            valid = lane < cnt && tok0 + lane >= kr.first && tok0 + lane < kr.end;
-            if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
-            if (p.alibi_slopes != nullptr)
-              s -= __ldg(&p.alibi_slopes[h * p.G + qr / p.q_len]) * fabsf((float)(lim - (tok0 + lane)));
-          }
-          const float hidden = kScored && !valid ? -1.f : 0.f;
-          if (!valid) s = -INFINITY;
+          const bool valid = lane < cnt && tok0 + lane <= lim;
+          float s = valid ? sc[r] * p.scale : -INFINITY;
           float bm = s;
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
           if (bm == -INFINITY) {  // nothing attendable for this row in this chunk
-            const bool bad = kScored && s != s;  // a visible score that is NaN makes the row NaN
-            if (lane < kF32Chunk) s_p[r * kF32Chunk + lane] = bad ? s : hidden;
-            if (kScored && __any_sync(0xffffffffu, bad)) l[r] = __int_as_float(0x7fffffff);
+            if (lane < kF32Chunk) s_p[r * kF32Chunk + lane] = 0.f;
             continue;
           }
           const float m_new = fmaxf(m[r], bm);
@@ -190,7 +157,7 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
           m[r] = m_new;
 #pragma unroll
           for (int j = 0; j < DPL; ++j) acc[r][j] *= alpha;
-          if (lane < kF32Chunk) s_p[r * kF32Chunk + lane] = kScored && !valid ? hidden : pv;
+          if (lane < kF32Chunk) s_p[r * kF32Chunk + lane] = pv;
         }
         __syncwarp();
         // acc += P V over the chunk's tokens
@@ -202,7 +169,6 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
           for (int r = 0; r < kF32Rows; ++r) {
             if (r < R) {
               const float pt = s_p[r * kF32Chunk + t];
-              if (kScored && pt < 0.f) continue;
 #pragma unroll
               for (int j = 0; j < DPL; ++j) acc[r][j] = fmaf(pt, vd[j], acc[r][j]);
             }
@@ -241,13 +207,8 @@ __global__ void __launch_bounds__(kF32Warps * 32) decode_f32_kernel(const Decode
       }
       const int qr = r0 + r;
       const int g = qr / p.q_len, t = qr - (qr / p.q_len) * p.q_len;
-      if constexpr (kScored) {
-        // all scores of the keys it sees are -inf: 0 / 0, unlike a row that sees none
-        const KeyRange kr = row_keys(p, b, L, t);
-        if (lsum == 0.f && kr.first < kr.end) a = lsum = __int_as_float(0x7fffffff);
-      }
       static_cast<float*>(p.out)[(long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + (long long)t * p.o_st +
-                                 d] = lsum > 0.f ? a / lsum : kScored ? a : 0.f;
+                                 d] = lsum > 0.f ? a / lsum : 0.f;
     }
   }
 }
@@ -258,14 +219,14 @@ static size_t f32_smem_bytes(int D, int kF32Rows) {
                           (size_t)kF32Warps * (2 * kF32Chunk * pitch + kF32Rows * kF32Chunk));
 }
 
-template <int DPL, int ROWS, bool kScored>
+template <int DPL, int ROWS>
 static cudaError_t launch_f32_impl(const DecodeParams& p, bool pdl, cudaStream_t stream) {
   const size_t smem = f32_smem_bytes(DPL * 32, ROWS);
   static bool prepared[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && !prepared[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(decode_f32_kernel<DPL, ROWS, kScored>,
+    cudaError_t e = cudaFuncSetAttribute(decode_f32_kernel<DPL, ROWS>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     prepared[dev] = true;
@@ -280,19 +241,14 @@ static cudaError_t launch_f32_impl(const DecodeParams& p, bool pdl, cudaStream_t
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = pdl ? attr : nullptr;
   cfg.numAttrs = pdl ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, decode_f32_kernel<DPL, ROWS, kScored>, p);
-}
-
-template <int DPL, bool kScored>
-static cudaError_t launch_f32_rows_of(const DecodeParams& p, bool pdl, cudaStream_t stream) {
-  if (p.GQ <= 4) return launch_f32_impl<DPL, 4, kScored>(p, pdl, stream);
-  if (p.GQ <= 8) return launch_f32_impl<DPL, 8, kScored>(p, pdl, stream);
-  return launch_f32_impl<DPL, 16, kScored>(p, pdl, stream);
+  return cudaLaunchKernelEx(&cfg, decode_f32_kernel<DPL, ROWS>, p);
 }
 
 template <int DPL>
 static cudaError_t launch_f32_rows(const DecodeParams& p, bool pdl, cudaStream_t stream) {
-  return p.scored ? launch_f32_rows_of<DPL, true>(p, pdl, stream) : launch_f32_rows_of<DPL, false>(p, pdl, stream);
+  if (p.GQ <= 4) return launch_f32_impl<DPL, 4>(p, pdl, stream);
+  if (p.GQ <= 8) return launch_f32_impl<DPL, 8>(p, pdl, stream);
+  return launch_f32_impl<DPL, 16>(p, pdl, stream);
 }
 
 cudaError_t launch_decode_f32(const DecodeParams& p, bool pdl, cudaStream_t stream) {

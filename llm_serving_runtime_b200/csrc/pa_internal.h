@@ -240,6 +240,10 @@ cudaError_t launch_kv_append8(const AppendParams& p, const ScaleParams& sc, int 
 cudaError_t launch_decode_mma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv,
                               int dtype, int grid, size_t smem, bool pdl, cudaStream_t stream);
 cudaError_t launch_decode_f32(const DecodeParams& p, bool pdl, cudaStream_t stream);
+// With changed scores (p.scored); partial states of f32_ext_partial_bytes() at
+// p.partials, p.counters as for the tensor-core kernels.
+size_t f32_ext_partial_bytes(int num_sms);
+cudaError_t launch_decode_f32_ext(const DecodeParams& p, int num_sms, bool pdl, cudaStream_t stream);
 cudaError_t launch_prefill_mma(const DecodeParams& p, const CUtensorMap& tmk, const CUtensorMap& tmv, int dtype,
                                bool pdl, cudaStream_t stream);
 // pa_decode_ext's form of the same kernel (8-bit cache and / or changed scores).
