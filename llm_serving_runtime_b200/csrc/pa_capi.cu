@@ -748,18 +748,20 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
       if (e != cudaSuccess) return cuda_fail(e, "multi-query launch");
       return PA_OK;
     }
-    // CTAs of their own for each row, where no more rows than SMs split over the
-    // GPU, or where no row can be long: up to kDirectUnits units (a bound by the
+    // CTAs of their own for each row, where every row has two SMs or more to be split
+    // over, or where no row can be long: up to kDirectUnits units (a bound by the
     // table's width, or the window) one CTA ends before balance matters.  Measured
-    // against the stream-K kernel, us a call: 1 x 32k 24 for 66; 24 rows of 16 to 300
-    // tokens 10.3 for 17.4, 96 of 1500 to 2048 76 for 82, 160 with a window of
-    // 1024 101 for 102; but 40 of 256 to 8192 61 (split further) for 53.
+    // against the stream-K kernel, us a call (8 KV heads a sequence): 1 x 32k 24 for
+    // 66, 4 of 256 to 8192 19 for 35, 8 29 for 32; 24 of 16 to 300 10.3 for 17.4, 96 of
+    // 1500 to 2048 76 for 82, 160 with a window of 1024 101 for 102.  One SM a long row is
+    // balanced only where rows are alike: 18 of 8000 to 8192 54 for 72, but 12 of 256 to
+    // 8192 46 for 33, 18 of 256 to 30,000 146 for 65.
     constexpr long long kDirectUnits = 130;
     const long long rows = (long long)p.B * p.Hkv * p.NMG;
     long long tokens = (long long)a->max_blocks * bs;
     if (p.window > 0) tokens = std::min(tokens, (long long)p.window + p.q_len);
     const bool few = rows <= info->num_sms;
-    if (few || tokens / (sc != nullptr ? 32 : 16) + 2 <= kDirectUnits) {
+    if (2 * rows <= info->num_sms || tokens / (sc != nullptr ? 32 : 16) + 2 <= kDirectUnits) {
       const pa::DirectShape d = pa::decode_direct_shape(sc != nullptr, !few);
       // the CTAs of an SM share its memory, 1 KB of it and the static part (5.2 KB) reserved for each
       const size_t share = (budget + 1152) / d.ctas_per_sm - 1024 - 6144;
