@@ -29,6 +29,7 @@
 // Measured: 8 x 509 tokens, 8 heads of 128 (25 MB) 9.3 us (18.5 with a warp reading
 // piece by piece for two pairs, 20.9 with two CTAs an SM); 64 rows of one token 4.3 us.
 #include <cuda_fp8.h>
+#include <limits.h>
 #include <math.h>
 
 #include "pa_common.cuh"
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
   // order; and which offsets of the block they take.
   __shared__ int2 s_run[kMaxBlock];
   __shared__ int s_token[kMaxBlock];  // slot form: token of the row at each offset, -1: none
-  __shared__ int s_count;
+  __shared__ int s_count, s_found;
   __shared__ uint32_t s_taken[kMaxBlock / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
   const int b = blockIdx.x / runs_per_row, k = blockIdx.x - b * runs_per_row;
@@ -166,16 +167,48 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
     const int64_t* row = p.slot_mapping + (long long)b * p.q_len;
     if (row[k] < 0) return;  // padding
     blk = row[k] >> bs_log2;
-    int prev = k - 1;
-    while (prev >= 0 && row[prev] < 0) --prev;
-    if (prev >= 0 && (row[prev] >> bs_log2) == blk) return;  // not the first token of its run
+    // The row's previous slot decides whether this token opens a run; the next
+    // slot of another block ends it.  Padding between them may be long (a padded
+    // batch): the block looks over kReach slots at a time.
+    constexpr int kReach = 8;  // slots a thread looks at
+    if (tid == 0) s_found = -1;
+    __syncthreads();
+    for (int base = k - 1; base >= 0; base -= threads * kReach) {
+      int mine = -1;
+#pragma unroll
+      for (int j = 0; j < kReach; ++j) {
+        const int i = base - (j * threads + tid);
+        if (i >= 0 && row[i] >= 0) mine = max(mine, i);
+      }
+      if (mine >= 0) atomicMax(&s_found, mine);
+      __syncthreads();
+      const int found = s_found;
+      __syncthreads();
+      if (found >= 0) break;
+    }
+    if (s_found >= 0 && (row[s_found] >> bs_log2) == blk) return;  // not the first token of its run
+    __syncthreads();
     for (int o = tid; o < bs; o += threads) s_token[o] = -1;
     if (tid < kMaxBlock / 32) s_taken[tid] = 0u;
-    if (tid == 0) s_count = 0;
+    if (tid == 0) {
+      s_count = 0;
+      s_found = INT_MAX;
+    }
     __syncthreads();
-    // the run: up to the next slot of another block
-    int end = k + 1;
-    while (end < p.q_len && (row[end] < 0 || (row[end] >> bs_log2) == blk)) ++end;
+    for (int base = k + 1; base < p.q_len; base += threads * kReach) {
+      int mine = INT_MAX;
+#pragma unroll
+      for (int j = 0; j < kReach; ++j) {
+        const int i = base + j * threads + tid;
+        if (i < p.q_len && row[i] >= 0 && (row[i] >> bs_log2) != blk) mine = min(mine, i);
+      }
+      if (mine < INT_MAX) atomicMin(&s_found, mine);
+      __syncthreads();
+      const int found = s_found;
+      __syncthreads();
+      if (found < INT_MAX) break;
+    }
+    const int end = min(s_found, p.q_len);
     for (int t = k + tid; t < end; t += threads)
       if (row[t] >= 0) atomicMax(&s_token[(int)(row[t] & (bs - 1))], t);  // a slot given twice: the last one
     __syncthreads();
@@ -219,8 +252,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
 
   bool earlier = other == blk && blk >= 0;  // another run of the call writes this block before this one
   if (tables) {
+#pragma unroll 4
     for (int r = tid + threads; r < (int)blockIdx.x; r += threads) earlier |= block_of_run(r) == blk;
   } else {
+#pragma unroll 4
     for (int i = tid; i < (int)blockIdx.x; i += threads)
       earlier |= p.slot_mapping[i] >= 0 && (p.slot_mapping[i] >> bs_log2) == blk;
   }

@@ -141,6 +141,8 @@ _host = _Host()
 # One workspace per device: status word + merge counters + partial slots.
 _ws_lock = threading.Lock()
 _workspaces: dict[int, torch.Tensor] = {}
+# Workspaces that a larger one replaced: captured graphs may still write to them.
+_outgrown: list[torch.Tensor] = []
 
 
 def _stream_ptr(device: torch.device) -> int:
@@ -165,6 +167,9 @@ def decode_workspace(device: torch.device, nbytes: int = 256) -> torch.Tensor:
                     "paged decode workspace must be sized before CUDA-graph capture: "
                     "run the same call once eagerly first"
                 )
+            if ws is not None:
+                _outgrown.append(ws)
+                nbytes = max(int(nbytes), 2 * ws.numel())  # what is kept stays below what is used
             ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=torch.device("cuda", idx))
             _workspaces[idx] = ws
         return ws

@@ -138,6 +138,20 @@ def test_values_at_the_types_ends(offset):
     c.append(rows, rows, slots, q=1)
 
 
+def test_long_padding_between_a_blocks_tokens():
+    """Padding of any length neither ends a run nor hides the slot before it."""
+    g = _gen(60)
+    q = 9000
+    slots = torch.full((2 * q,), -1, dtype=torch.int64)
+    slots[0], slots[4000], slots[4001], slots[8999] = 5, 6, 16, 17
+    slots[q + 8500], slots[q + 8999] = 40, 41
+    c = Append(4, 1, 16, 16, 60)
+    rows = torch.zeros(2, 1, q, 16)
+    for i in (0, 4000, 4001, 8500, 8999):
+        rows[:, :, i] = torch.randn(2, 1, 16, generator=g) * 2.0 ** (i % 3)
+    c.append(rows.to(BF), rows.to(BF), slots, q=q)
+
+
 def test_a_slot_given_twice_takes_the_last_token():
     g = _gen(6)
     c = Append(4, 2, 16, 64, 6)
@@ -358,6 +372,32 @@ def test_batches_beyond_the_shared_memory_tables():
     rows = [0, 4499, 4500, 8999]
     ref, bar = attend64(q[rows], kc, kc, bt[rows], lens[rows], 0.125, key_scales=ks, value_scales=ks)
     check(out[rows], ref, bar)
+
+
+def test_caches_past_32_bit_offsets():
+    """Codes beyond 2^32 bytes: appended to and attended at both ends."""
+    g = _gen(61)
+    nb, H, bs, D = 2_200_000, 1, 16, 128
+    codes = torch.zeros(nb, H, bs, D, dtype=torch.uint8, device="cuda").view(F8)
+    scales = torch.zeros(nb, H, device="cuda")
+    bt = torch.tensor([[nb - 1, 3], [nb - 7, nb - 2]], dtype=torch.int32)
+    k = _rows(2, 1, 20, D, g, BF).cuda()
+    zero = torch.zeros(2, dtype=torch.int32, device="cuda")
+    kv_append(k, k, codes, codes, block_tables=bt.cuda(), positions=zero, key_scales=scales, value_scales=scales,
+              validate=True)
+    q = torch.randn(2, 4, 1, D, generator=g).to(BF).cuda()
+    lens = torch.tensor([19, 19], dtype=torch.int32)
+    out = paged_attention_decode(q, codes, codes, bt.cuda(), lens.cuda(), D**-0.5, key_scales=scales,
+                                 value_scales=scales, validate=True)
+    ids = bt.long().reshape(-1)
+    small = torch.arange(4, dtype=torch.int32).reshape(2, 2)
+    c = codes.view(torch.uint8)[ids.cuda()].view(F8)
+    ref, bar = attend64(q, c, c, small, lens, D**-0.5, key_scales=scales[ids.cuda()], value_scales=scales[ids.cuda()])
+    check(out, ref, bar)
+    want = k[1, 0, :16].float()
+    got = codes.view(torch.uint8)[nb - 7, 0].view(F8).float() * scales[nb - 7, 0]
+    # a code is off by half a step of its value, or of the least normal one
+    assert bool(((got - want).abs() <= want.abs() * 2.0**-4 + scales[nb - 7, 0] * 2.0**-10).all())
 
 
 def test_refusals():
