@@ -298,10 +298,10 @@ PA_API int pa_kv_append_8bit(const pa_kv_append_args* args, const pa_cache_scale
  * and the token sees j when key_starts[b, t] <= j, i - j < window (window > 0), and
  * j <= i or j < prefix_lens[b].  A token that sees nothing gives a zero row.  What a
  * token does not see does not reach its row, whatever the cache holds there;
- * blocks before a row's first visible key are not read (their table entries may
- * be anything). */
+ * blocks before the first key that any of a sequence's tokens sees are not read
+ * (their table entries may be anything). */
 typedef struct pa_score_modifiers {
-  float softcap;                 /* 0: none */
+  float softcap;                 /* 0: none; else in (1e-30, 1e30) */
   int32_t window;                /* 0: none */
   const float* alibi_slopes;     /* [num_q_heads] or NULL */
   const int32_t* key_starts;     /* first key of token (b, t) (a document's start), or NULL */

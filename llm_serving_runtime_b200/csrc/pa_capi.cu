@@ -367,6 +367,9 @@ static int append_impl(const pa_kv_append_args* a, const pa_cache_scales* sc, vo
                                                       : ((long long)a->q_len + a->block_size - 2) / a->block_size + 1;
     if (runs * a->batch > (1LL << 30))
       return fail(PA_ERR_UNSUPPORTED, "batch * q_len too large");
+    if ((a->key_cache.num_blocks > 1 && (sc->key_stride_block == 0 || sc->value_stride_block == 0)) ||
+        (a->num_kv_heads > 1 && (sc->key_stride_head == 0 || sc->value_stride_head == 0)))
+      return fail(PA_ERR_INVALID_ARGUMENT, "scales that are written must not overlap");
   }
   pa::AppendParams p;
   p.key = a->key;
@@ -516,8 +519,8 @@ int pa_decode_ext(const pa_decode_args* a, const pa_cache_scales* scales, const 
       return fail(PA_ERR_UNSUPPORTED, "8-bit caches are attended by fp16/bf16 queries");
   }
   if (modifiers != nullptr) {
-    if (!(modifiers->softcap >= 0.f) || !(modifiers->softcap < 1e30f))
-      return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be 0 (none) or positive and finite");
+    if (modifiers->softcap != 0.f && !(modifiers->softcap > 1e-30f && modifiers->softcap < 1e30f))
+      return fail(PA_ERR_INVALID_ARGUMENT, "softcap must be 0 (none) or in (1e-30, 1e30)");
     if (modifiers->window < 0) return fail(PA_ERR_INVALID_ARGUMENT, "window must be 0 (none) or positive");
   }
   return decode_impl(a, nullptr, nullptr, stream, scales, modifiers, error_flags);

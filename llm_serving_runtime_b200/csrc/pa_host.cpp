@@ -15,7 +15,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
-#include <cmath>
 #include <utility>
 
 #include "../../include/paged_attention_b200.h"
@@ -194,7 +193,7 @@ PyObject* py_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
     for (int i = 0; i < 5; ++i) m[i] = PyTuple_GET_ITEM(o[13], i);
     const double cap = PyFloat_AsDouble(m[0]);
     int64_t window;
-    if ((cap == -1.0 && PyErr_Occurred()) || !(cap >= 0.0) || !std::isfinite(cap)) {
+    if ((cap == -1.0 && PyErr_Occurred()) || !(cap == 0.0 || (cap > 1e-30 && cap < 1e30))) {
       PyErr_Clear();
       return none();
     }
@@ -303,7 +302,15 @@ bool page_view(const at::Tensor& t, pa_page_view* v) {
       return false;
     }
   }
-  if ((segments > 1 && stride < run) || (t.size(0) > 1 && t.stride(0) < run + (segments - 1) * stride)) return false;
+  // pages one after the other, or interleaved with one another's runs: no byte twice
+  std::pair<int64_t, int64_t> levels[2] = {{t.stride(0), t.size(0)}, {stride, segments}};
+  std::sort(levels, levels + 2);
+  int64_t extent = run;
+  for (const auto& l : levels) {
+    if (l.second <= 1) continue;
+    if (l.first < extent) return false;
+    extent += (l.second - 1) * l.first;
+  }
   *v = {t.data_ptr(), t.stride(0) * e, segments, stride * e, run * e};
   return true;
 }

@@ -144,7 +144,7 @@ inline KeyRange key_range(int L, int q_len, int t, int window, int start, int pr
   if (shared > r.end) r.end = shared;
   if (pos < 0) r.end = 0;  // a token before the sequence's start
   r.first = start > 0 ? start : 0;
-  if (window > 0 && pos - window + 1 > r.first) r.first = pos - window + 1;
+  if (window > 0 && pos >= window && pos - window + 1 > r.first) r.first = pos - window + 1;
   return r;
 }
 

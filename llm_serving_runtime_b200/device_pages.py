@@ -26,7 +26,7 @@ Errors: a bad slot, a child that is not empty, a block written from two places
 (IndexError) and a pool without enough free pages (RuntimeError) leave the slots
 concerned as they were and raise at the next call, like the other kernels' errors
 (``validate=True``: this call, synchronously; ``read_device_errors`` after a
-captured replay).
+captured replay of ``copy_pages``, ``DevicePages.read_errors`` of the others).
 
 The reference copies pages one tensor at a time (``GpuKVBlockPool.copy_blocks``,
 runtime/phase2/paged_kv_kernel.py:233-250) and allocates on the host
@@ -75,8 +75,12 @@ def _view(t: torch.Tensor) -> _lib.PageViewArgs:
     if len(levels) > 1:
         raise ValueError(f"a page may have one strided dimension, got shape {tuple(t.shape)} with strides {t.stride()}")
     segments, stride = levels[0] if levels else (1, 0)
-    if segments > 1 and stride < run or (t.shape[0] > 1 and t.stride(0) < run + (segments - 1) * stride):
-        raise ValueError("the pages of a cache must not overlap")
+    # pages one after the other, or interleaved with one another's runs: no byte twice
+    extent = run
+    for step, size in sorted(((t.stride(0), t.shape[0]), (stride, segments))):
+        if size > 1 and step < extent:
+            raise ValueError("the pages of a cache must not overlap")
+        extent += (size - 1) * step
     return _lib.PageViewArgs(t.data_ptr(), t.stride(0) * e, segments, stride * e, run * e)
 
 
@@ -146,7 +150,9 @@ class DevicePages:
     """Tables, lengths and page counts of ``max_seqs`` sequence slots on a device.
 
     The tensors may be read at any time and rewritten between calls, as long as
-    they stay consistent.  Calls that use one object must not overlap on the GPU.
+    they stay consistent.  Calls that use one object must not overlap on the GPU,
+    and a graph that captured some needs the object kept.  ``compact`` renames
+    pages: copies of table rows made before it are void.
     """
 
     def __init__(self, num_blocks: int, block_size: int, max_seqs: int, max_blocks_per_seq: int,
@@ -176,8 +182,8 @@ class DevicePages:
             raise ValueError("block_tables must be a CUDA int32 [max_seqs, max_blocks] with contiguous rows")
         if block_tables.shape[0] > 1 and block_tables.stride(0) < block_tables.shape[1]:
             raise ValueError("the rows of block_tables must not overlap")
-        if block_size <= 0:
-            raise ValueError("block_size must be positive")
+        if not 0 < block_size <= 2**30:
+            raise ValueError("block_size must be positive and at most 2^30")
         for name, t in (("seq_lens", seq_lens), ("ref_counts", ref_counts)):
             if t.dim() != 1 or t.dtype != torch.int32 or t.device != block_tables.device or not t.is_contiguous() \
                     or t.numel() == 0:

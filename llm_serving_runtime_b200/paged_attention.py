@@ -309,11 +309,21 @@ class _HostWord:
     directly, so looking for the errors of earlier calls is one host read, with
     no copy queued behind each call."""
 
-    __slots__ = ("host", "ptr", "word", "device")
+    __slots__ = ("ptr", "word", "device")
+
+    # Words come out of slabs that stay: a kernel or captured graph may still report
+    # into the word of an object that is gone.
+    _slabs: list[torch.Tensor] = []
+    _left = 0
+    _lock = threading.Lock()
 
     def __init__(self, device: torch.device):
-        self.host = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-        self.ptr = self.host.data_ptr()
+        with _HostWord._lock:
+            if _HostWord._left == 0:
+                _HostWord._slabs.append(torch.zeros(1024, dtype=torch.int32, pin_memory=True))
+                _HostWord._left = 1024
+            _HostWord._left -= 1
+            self.ptr = _HostWord._slabs[-1].data_ptr() + 4 * _HostWord._left
         self.word = ctypes.c_uint32.from_address(self.ptr)
         self.device = device
 

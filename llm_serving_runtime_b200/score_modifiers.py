@@ -16,9 +16,9 @@ For the query token at position i (``context_lens[b] + t``) and the key at j:
 
 All of them may be given together; the masks intersect, except that a prefix
 lifts the causal limit.  A token that sees no key gets a zero row.  What a token
-does not see cannot reach its row (not even as NaN), and blocks before a row's
-first visible key are never read, so a sliding window's old blocks may be
-recycled while their table entries stay.
+does not see cannot reach its row (not even as NaN), and blocks before the first
+key that any of a sequence's tokens sees are never read, so a sliding window's old
+blocks may be recycled while their table entries stay.
 
 The tensors are read on the device at the call (at the replay, in a captured
 graph), so they may be rewritten in place between steps.
@@ -26,7 +26,6 @@ graph), so they may be rewritten in place between steps.
 
 from __future__ import annotations
 
-import math
 from dataclasses import dataclass
 
 import torch
@@ -47,8 +46,8 @@ class ScoreModifiers:
     def to_args(self, batch: int, num_q_heads: int, q_len: int, device: torch.device) -> _lib.ScoreModifiersArgs:
         """The C arguments for a call of this shape; ValueError where they do not fit it."""
         a = _lib.ScoreModifiersArgs()
-        if not 0.0 <= self.softcap < math.inf:
-            raise ValueError(f"softcap must be 0 (none) or positive and finite, got {self.softcap}")
+        if self.softcap != 0.0 and not 1e-30 < self.softcap < 1e30:
+            raise ValueError(f"softcap must be 0 (none) or in (1e-30, 1e30), got {self.softcap}")
         if not 0 <= self.window < 2**31:
             raise ValueError(f"window must be 0 (none) or positive, got {self.window}")
         a.softcap, a.window = float(self.softcap), int(self.window)

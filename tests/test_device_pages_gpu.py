@@ -67,6 +67,17 @@ def test_copy_pages_of_many_layers_and_large_pages():
     assert torch.equal(a, wa) and torch.equal(b, wb)
 
 
+def test_copy_pages_interleaved_by_layer():
+    """A pool stored layer by layer, its pages [block, layer, ...] as a strided view."""
+    g = torch.Generator().manual_seed(21)
+    pool = torch.randn(5, 40, 3, 16, 64, generator=g).cuda()
+    want = pool.clone()
+    want[:, [7, 39]] = want[:, [0, 12]]
+    copy_pages([pool.transpose(0, 1)], torch.tensor([0, 12], dtype=torch.int32).cuda(),
+               torch.tensor([7, 39], dtype=torch.int32).cuda())
+    assert torch.equal(pool, want)
+
+
 def test_copy_pages_past_32_bit_offsets():
     """A pool of more than 2^32 bytes: pages at both ends."""
     P = 2100

@@ -175,6 +175,10 @@ def test_page_views():
     assert _fields(torch.zeros(10, 3)) == (12, 1, 0, 12)
     assert _fields(torch.zeros(10)) == (4, 1, 0, 4)
     assert _fields(torch.zeros(10, 6, 4).transpose(1, 2)) == (96, 1, 0, 96)  # another order, the same bytes
+    # stored layer by layer: a page is a run of each layer, the pages interleave
+    assert _fields(torch.zeros(4, 10, 6).transpose(0, 1)) == (24, 4, 240, 24)
+    with pytest.raises(ValueError, match="overlap"):
+        _view(torch.zeros(400).as_strided((10, 4, 6), (6, 50, 1)))
     with pytest.raises(ValueError, match="one strided"):
         _view(torch.zeros(10, 4, 8, 8)[:, ::2, ::2, ::2])
     with pytest.raises(ValueError, match="overlap"):
@@ -189,7 +193,7 @@ def test_score_modifier_refusals():
     def args(**kw):
         return ScoreModifiers(**kw).to_args(2, 4, 3, dev)
 
-    for bad in ({"softcap": -1.0}, {"softcap": float("nan")}, {"softcap": float("inf")}, {"window": -1},
+    for bad in ({"softcap": -1.0}, {"softcap": float("nan")}, {"softcap": float("inf")}, {"softcap": 1e-31}, {"window": -1},
                 {"window": 2**31}, {"alibi_slopes": torch.zeros(3)}, {"alibi_slopes": torch.zeros(4).double()},
                 {"alibi_slopes": torch.zeros(8)[::2]}, {"key_starts": torch.zeros(2)},
                 {"key_starts": torch.zeros(2, 2, dtype=torch.int32)}, {"key_starts": torch.zeros(3, dtype=torch.int32)},

@@ -171,6 +171,14 @@ def test_negative_starts_and_prefixes_and_short_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF, HF, FP, FP8])
+@pytest.mark.parametrize("q", [4, 40])
+def test_the_widest_window_over_rows_shorter_than_the_call(dtype, q):
+    """Tokens before the sequence's start see nothing, the others everything."""
+    s = _setup(dtype, [-3 * q // 4, -q // 2, -1, -q, 30], q, 8, 2, 64, 16, 18)
+    _run(s, ScoreModifiers(window=2**31 - 1, prefix_lens=_i32([2, 0, 1, 3, 9])), include=True)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, FP, FP8])
 @pytest.mark.parametrize("q", [1, 4, 40])
 def test_what_is_hidden_may_be_anything(dtype, q):
     """NaN and infinities in keys and values that a row does not see: behind its end,
