@@ -766,8 +766,8 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
     const bool few = rows <= info->num_sms;
     if (2 * rows <= info->num_sms || tokens / (sc != nullptr ? 32 : 16) + 2 <= kDirectUnits) {
       const pa::DirectShape d = pa::decode_direct_shape(sc != nullptr, !few);
-      // the CTAs of an SM share its memory, 1 KB of it and the static part (5.2 KB) reserved for each
-      const size_t share = (budget + 1152) / d.ctas_per_sm - 1024 - 6144;
+      // the CTAs of an SM share its memory, 1 KB of it and the static part (at most 6.5 KB) reserved for each
+      const size_t share = (budget + 1152) / d.ctas_per_sm - 1024 - 6656;
       int n = 8;
       while (n > 2 && pa::decode_direct_smem_bytes(D, n, d.warps, sc != nullptr) > share) --n;
       p.stages = n;

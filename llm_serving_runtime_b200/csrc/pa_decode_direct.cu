@@ -42,6 +42,13 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   constexpr int HALVES = TL::kHalves;
   constexpr uint32_t TILE_BYTES = TL::kTileBytes;
   constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
+  // Rows of the CTA's shared arrays, padded so that the fragments' accesses (8 rows x
+  // 4 lanes) fall into different banks: staged query rows (words; the merge's weights
+  // take their place), and a warp's accumulator (floats).
+  constexpr int WT = k8 ? 72 : 68;
+  constexpr int AS = D + 8;
+  static_assert(D / 2 <= 64 && kMaxSplits <= 64, "rows of s_wt");
+  static_assert(16 * AS * 4 <= 2 * STAGE_BYTES, "an accumulator lies in two stages");
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_addr(smem_raw);
@@ -50,7 +57,9 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (size_t)kWarps * stages * STAGE_BYTES);
   float4* s_scales = reinterpret_cast<float4*>(bars + kWarps * stages);
   __shared__ float s_m[kWarps][16], s_l[kWarps][16];
-  __shared__ float s_wt[16][kMaxSplits];
+  __shared__ __align__(16) float s_wt[16][WT];
+  __shared__ const T* s_qrow[16];
+  __shared__ T* s_orow[16];
   __shared__ float s_ref[16], s_norm[16];
   __shared__ int s_min_start, s_last;
 
@@ -60,8 +69,13 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   const int rows_here = min(16, p.GQ - 16 * mg);
   const int t_first = 16 * mg / p.G, t_last = (16 * mg + rows_here - 1) / p.G;
 
-  if (lane == 0)
-    for (int s = 0; s < stages; ++s) mbar_init(smem_addr(&bars[warp * stages + s]), k8 ? 9 : 1);
+  int L = p.context_lens[b] + p.len_offset;
+  if (lane < stages) mbar_init(smem_addr(&bars[warp * stages + lane]), k8 ? 9 : 1);
+  if (tid < rows_here) {
+    const int t = (16 * mg + tid) / p.G, hq = h * p.G + (16 * mg + tid - t * p.G);
+    s_qrow[tid] = static_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)hq * p.q_sh + (long long)t * p.q_st;
+    s_orow[tid] = static_cast<T*>(p.out) + (long long)b * p.o_sb + (long long)hq * p.o_sh + (long long)t * p.o_st;
+  }
   if (tid == 0) {
     prefetch_tensormap(&tmk);
     prefetch_tensormap(&tmv);
@@ -71,7 +85,6 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   __syncthreads();
 
   // ---- the row's units, and this warp's share ----
-  int L = p.context_lens[b] + p.len_offset;
   const int cap = p.max_blocks * p.bs;
   if (L > cap) {
     if (tid == 0 && h == 0 && mg == 0 && split == 0) raise_flag(p.status, PA_DEVERR_TABLE_UNDERRUN);
@@ -114,6 +127,16 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   // Everything below reads what the previous kernel may write.
   pdl_wait_previous();
 
+  // The 16 query rows, once a CTA: whole rows a load instruction (each warp loading its
+  // fragments itself took 2.6 us of a verify call's 14.6 a CTA).
+  constexpr int kThreads = kWarps * 32, kWords = 16 * (D / 2), kLoads = (kWords + kThreads - 1) / kThreads;
+  uint32_t qw[kLoads];
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    const int i = tid + n * kThreads, r = i / (D / 2), w = i % (D / 2);
+    qw[n] = r < rows_here && 2 * w < p.Dv ? __ldg(reinterpret_cast<const unsigned int*>(s_qrow[r]) + w) : 0u;
+  }
+
   // Lane roles as in pa_decode_kernel.cuh.
   auto issue = [&](int u, int slot) {
     const uint32_t stage = ring + (uint32_t)slot * STAGE_BYTES;
@@ -155,23 +178,35 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
 
   // ---- the warp's query rows and its units ----
   const int qr0 = 16 * mg + (lane >> 2);
-  auto query_row = [&](int qr) -> const T* {
-    if (qr >= p.GQ) return nullptr;
-    const int t = qr / p.G, g = qr - t * p.G;
-    return static_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)(h * p.G + g) * p.q_sh +
-           (long long)t * p.q_st;
-  };
+#pragma unroll
+  for (int n = 0; n < kLoads; ++n) {
+    const int i = tid + n * kThreads;
+    if (kWords % kThreads == 0 || i < kWords) s_wt[i / (D / 2)][i % (D / 2)] = __uint_as_float(qw[n]);
+  }
+  __syncthreads();
   uint32_t qa[D / 16][4];
   float o_acc[D / 8][4];
   RowState st;
   int tok_lo, tok_hi, full_lo, full_hi;
   if constexpr (k8) {
     float qinv[2];
-    load_query_frags_8<T, D>(qa, query_row(qr0), query_row(qr0 + 8), quad, p.Dv, qinv);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint2 v = *reinterpret_cast<const uint2*>(&s_wt[(lane >> 2) + 8 * r][ks * 8 + 2 * quad]);
+        qa[ks][r] = v.x;
+        qa[ks][r + 2] = v.y;
+      }
+    scale_query_frags_8<T, D>(qa, qinv);
     st.c[0] = p.scale_log2 * qinv[0];
     st.c[1] = p.scale_log2 * qinv[1];
   } else {
-    load_query_frags<T, D>(qa, query_row(qr0), query_row(qr0 + 8), quad, p.Dv);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        qa[ks][i] = __float_as_uint(s_wt[(lane >> 2) + 8 * (i & 1)][ks * 8 + quad + 4 * (i >> 1)]);
     st.c[0] = st.c[1] = p.scale_log2;
   }
   init_rows<kScored>(st, p, b, h, L, qr0, tok_lo, tok_hi, full_lo, full_hi);
@@ -221,8 +256,8 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
 #pragma unroll
   for (int nd = 0; nd < D / 8; ++nd) {
     const int d = nd * 8 + 2 * quad;
-    *reinterpret_cast<float2*>(acc + (lane >> 2) * D + d) = make_float2(o_acc[nd][0], o_acc[nd][1]);
-    *reinterpret_cast<float2*>(acc + ((lane >> 2) + 8) * D + d) = make_float2(o_acc[nd][2], o_acc[nd][3]);
+    *reinterpret_cast<float2*>(acc + (lane >> 2) * AS + d) = make_float2(o_acc[nd][0], o_acc[nd][1]);
+    *reinterpret_cast<float2*>(acc + ((lane >> 2) + 8) * AS + d) = make_float2(o_acc[nd][2], o_acc[nd][3]);
   }
   __syncthreads();
   auto sees = [&](int r) -> bool {
@@ -245,27 +280,31 @@ __global__ void __launch_bounds__(Shape<KV, kMany>::kWarps * 32, Shape<KV, kMany
   }
   __syncthreads();
   auto out_pair = [&](int r, int d, float2 a, float inv) {
-    const int qr = 16 * mg + r, t = qr / p.G, g = qr - t * p.G;
-    if (d < p.Dv)
-      *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh +
-                                   (long long)t * p.o_st + d) = pack2<T>(a.x * inv, a.y * inv);
+    if (d < p.Dv) *reinterpret_cast<uint32_t*>(s_orow[r] + d) = pack2<T>(a.x * inv, a.y * inv);
   };
   const int slot_floats = p.slot_rows * (2 + D);
   float* part = p.partials + ((long long)row * gridDim.y + split) * slot_floats;
-  for (int i = tid; i < rows_here * (D / 2); i += kWarps * 32) {
-    const int r = i / (D / 2), d = 2 * (i - r * (D / 2));
-    float2 a = make_float2(0.f, 0.f);
+#pragma unroll 2
+  for (int i = tid; i < rows_here * (D / 4); i += kThreads) {
+    const int r = i / (D / 4), d = 4 * (i % (D / 4));
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = s_wt[r][w];
-      const float2 v = *reinterpret_cast<const float2*>(smem + (size_t)(w * stages) * STAGE_BYTES + (r * D + d) * 4);
+      const float4 v = *reinterpret_cast<const float4*>(smem + (size_t)(w * stages) * STAGE_BYTES + (r * AS + d) * 4);
       a.x = fmaf(f, v.x, a.x);
       a.y = fmaf(f, v.y, a.y);
+      a.z = fmaf(f, v.z, a.z);
+      a.w = fmaf(f, v.w, a.w);
     }
-    if (S == 1)
-      out_pair(r, d, a, s_norm[r]);
-    else
-      *reinterpret_cast<float2*>(part + 2 * p.slot_rows + r * D + d) = a;
+    if (S == 1) {
+      out_pair(r, d, make_float2(a.x, a.y), s_norm[r]);
+      out_pair(r, d + 2, make_float2(a.z, a.w), s_norm[r]);
+    } else {
+      float2* to = reinterpret_cast<float2*>(part + 2 * p.slot_rows + r * D + d);
+      to[0] = make_float2(a.x, a.y);
+      to[1] = make_float2(a.z, a.w);
+    }
   }
   if (S == 1) return;
   if (tid < rows_here) {

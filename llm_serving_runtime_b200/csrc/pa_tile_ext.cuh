@@ -173,20 +173,10 @@ __device__ __forceinline__ void init_rows(RowState& st, const DecodeParams& p, i
 
 // Query fragments of an 8-bit tile: k-step ks holds columns 16 ks + 4 quad, +1
 // (registers 0, 1) and +2, +3 (registers 2, 3), the order in which ldmatrix
-// hands out four neighbouring codes.  qinv: what takes the rows' own powers of
-// two back out of their dot products.
+// hands out four neighbouring codes.  Here they become fp16: each row times a power
+// of two of its own, which qinv takes back out of its dot products.
 template <typename T, int D>
-__device__ __forceinline__ void load_query_frags_8(uint32_t (&qa)[D / 16][4], const T* qp0, const T* qp1, int quad,
-                                                   int Dv, float (&qinv)[2]) {
-#pragma unroll
-  for (int ks = 0; ks < D / 16; ++ks) {
-    const int d = ks * 16 + 4 * quad;
-    const bool in = d < Dv;  // Dv is a multiple of 16
-    qa[ks][0] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d)) : 0u;
-    qa[ks][1] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d)) : 0u;
-    qa[ks][2] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d + 2)) : 0u;
-    qa[ks][3] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d + 2)) : 0u;
-  }
+__device__ __forceinline__ void scale_query_frags_8(uint32_t (&qa)[D / 16][4], float (&qinv)[2]) {
   qinv[0] = qinv[1] = 1.f;
   if constexpr (sizeof(T) == 2 && !kSplitProbabilities<T>::value) return;  // fp16 already
   float mx[2] = {0.f, 0.f};
@@ -211,6 +201,22 @@ __device__ __forceinline__ void load_query_frags_8(uint32_t (&qa)[D / 16][4], co
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       qa[ks][i] = pack2<__half>(lo_half<T>(qa[ks][i]) * mul[i & 1], hi_half<T>(qa[ks][i]) * mul[i & 1]);
+}
+
+// The same from the rows qp0 and qp1 (null: 0) in memory.
+template <typename T, int D>
+__device__ __forceinline__ void load_query_frags_8(uint32_t (&qa)[D / 16][4], const T* qp0, const T* qp1, int quad,
+                                                   int Dv, float (&qinv)[2]) {
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) {
+    const int d = ks * 16 + 4 * quad;
+    const bool in = d < Dv;  // Dv is a multiple of 16
+    qa[ks][0] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d)) : 0u;
+    qa[ks][1] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d)) : 0u;
+    qa[ks][2] = (qp0 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp0 + d + 2)) : 0u;
+    qa[ks][3] = (qp1 && in) ? __ldg(reinterpret_cast<const unsigned int*>(qp1 + d + 2)) : 0u;
+  }
+  scale_query_frags_8<T, D>(qa, qinv);
 }
 
 // c * tanh(x / c) in the log2 domain (cap, inv_cap = 1 / cap, both of it), with
