@@ -738,7 +738,9 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
   if (st != PA_OK) return st;
 
   if (ext) {
-    // as below: many query rows per KV head share K/V tiles, few split the work
+    // as below: many query rows per KV head share K/V tiles, few split the work (with
+    // 60 tiles for the bound, 300 tokens of one row took 34 us for 40, 500 of another
+    // 57 for 50: left at the plain kernels' one tile an SM)
     if (p.GQ >= 64 && (long long)p.B * p.Hkv * ((p.GQ + 127) / 128) >= info->num_sms) {
       if (sc == nullptr && rows16 && multiquery_policy() != kPolicyMma) {
         g_last_kernel = "pa::prefill_umma_kernel<scored>";
@@ -754,11 +756,11 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
     // CTAs of their own for each row, where every row has two SMs or more to be split
     // over, or where no row can be long: up to kDirectUnits units (a bound by the
     // table's width, or the window) one CTA ends before balance matters.  Measured
-    // against the stream-K kernel, us a call (8 KV heads a sequence): 1 x 32k 24 for
-    // 66, 4 of 256 to 8192 19 for 35, 8 29 for 32; 24 of 16 to 300 10.3 for 17.4, 96 of
-    // 1500 to 2048 76 for 82, 160 with a window of 1024 101 for 102.  One SM a long row is
-    // balanced only where rows are alike: 18 of 8000 to 8192 54 for 72, but 12 of 256 to
-    // 8192 46 for 33, 18 of 256 to 30,000 146 for 65.
+    // against the stream-K kernel, us a call (8 KV heads a sequence): 1 x 32k 20 for 66,
+    // 4 of 256 to 8192 13 for 35; 24 of 16 to 300 8.5 for 17.3, 96 of 1500 to 2048 70 for
+    // 82, 128 with a window of 1024 77 for 85.  Longer rows are balanced only where
+    // they are alike: 16 of 20,000 112 for 144, but 40 of 256 to 8192 99 for 53, 140 of
+    // them 168 for 142 (and split over clusters of up to 8 CTAs 68 for 53, 161 for 142).
     constexpr long long kDirectUnits = 130;
     const long long rows = (long long)p.B * p.Hkv * p.NMG;
     long long tokens = (long long)a->max_blocks * bs;

@@ -20,10 +20,13 @@
 // results do not depend on timing.  A call whose pages run out leaves the slots
 // that did not get all of theirs as they were and flags it.
 //
-// Bound: copies by memory (16-byte loads, four of a thread in flight; figures at
-// the launcher), the rest by latency.  The planning kernels are one CTA each: a
-// prefix sum over counts in tiles of 4096, the next tile's loads issued
-// before the current one is summed.
+// Bound: copies by memory (16-byte loads, four of a thread in flight), the rest by
+// latency.  48 pages of a 4-layer pool (25 MB moved) 6.7 us; 4096 pages compacted to
+// 2458 live ones (525 MB moved) 97 us, of it plan 6, tables 4, copies 83 (6.3 TB/s).  The
+// planning kernels are one CTA each: a prefix sum over counts in tiles of 4096, the
+// next tile's loads issued before the current one is summed.  64 beams replaced by
+// forks over 6000 pages: free 4, fork 8 + 6, reserve 8 us, chains of five to seven
+// dependent loads and barriers.
 #include <limits.h>
 
 #include "pa_common.cuh"

@@ -45,8 +45,12 @@
 // V row that is not finite would reach rows that do not see it through their zero
 // weights (0 * inf), and 128 rows share one MMA: chunks that some row sees only in
 // part are looked over, and a CTA that finds such a row computes its own rows anew
-// on CUDA cores, key by key.  4 x 1021 tokens of packed documents: 200 us on the
-// mma.sync kernel, figures of this one in the launcher's rule (pa_capi.cu).
+// on CUDA cores, key by key.  4 x 1021 tokens of packed documents of 700 (32/8 heads of
+// 128, 22.6 GFLOP of visible scores): 100 us, 199 on the mma.sync kernel.  Of a CTA's
+// 22 us 11 are its 6.8 chunks (1.6 us a chunk, as without scores) and 9 what it pays
+// once: key ranges 1.0, queries 2.5, first scores 1.0, output 2.7, the next CTA's start
+// 1.2.  Loading the queries before the key ranges took longer (101.5: the fences
+// of the start wait for them), two CTAs of 128 rows an SM too (109).
 #include <limits.h>
 #include <math.h>
 
