@@ -23,7 +23,7 @@
 // so a block of large scale and little weight cannot push the others' weights
 // out of fp16's range, and one exponential serves both sums.  w is rounded to
 // fp16 for the product (at most 2^-11 of each weight; normal down to 2^-28 of the
-// largest), the norm takes it unrounded.  Scales other than 0 are taken to be at
+// largest, nothing below 2^-39 of it), the norm takes it unrounded.  Scales other than 0 are taken to be at
 // least 2^-100 (the append writes no smaller ones).
 //
 // What a mask hides never reaches a row: hidden scores are -inf whatever K

@@ -43,7 +43,9 @@ def attend64(query, key_cache, value_cache, tables, lens, scale, *, key_scales=N
 
     * the output's own rounding, eps/2 of the value (none beyond fp32 arithmetic for fp32);
     * weights rounded before P.V: 2^-11 (fp16, and every 8-bit cache), 2^-16 (bf16
-      keeps a second part), of sum_j w_j |v_j|;
+      keeps a second part), of sum_j w_j |v_j|; 8-bit caches: the largest weighted
+      scale w_j vs_j is at 2^14 there, fp16's least step is 2^-24, so a weight far
+      below is off by at most 2^-25, 2^-39 of the largest, times its code;
     * scores: products of D terms summed in fp32 (tensor cores may truncate: 2^-23 a
       step), the cap (2^-21 of it), the exponent's argument and ex2 (2^-21): an
       error d of a score moves its weight by d, and weights enter twice (sum, norm);
@@ -99,7 +101,11 @@ def attend64(query, key_cache, value_cache, tables, lens, scale, *, key_scales=N
                 out[b, h, t] = w @ vt
                 n = int(on.sum())
                 slack = weight_eps + 2 * float(d[t][on].max()) + (n / 16 + 32) * 2.0**-23
-                bar[b, h, t] = (w @ vt.abs()) * slack + out[b, h, t].abs() * out_eps
+                if key_scales is not None:
+                    vs = value_scales.cpu().double()[tables[b, cols // bs], h // G][on]
+                    codes = value_cache.cpu().to(torch.float64)[tables[b, cols // bs], h // G, cols % bs][on].abs()
+                    bar[b, h, t] = 2.0**-39 * (w * vs).max() * codes.sum(0)
+                bar[b, h, t] += (w @ vt.abs()) * slack + out[b, h, t].abs() * out_eps
     # results below the type's normal range are rounded to its least step
     bar += 2.0**-24 if dt == torch.float16 else 1e-38
     return out, bar

@@ -397,3 +397,99 @@ def test_two_streams_with_workspaces_of_their_own():
     torch.cuda.synchronize()
     for w, outs in zip(want, got):
         assert all(torch.equal(w, o) for o in outs)
+
+
+KINDS = [BF, HF, FP, F8]
+
+
+def _case(cache, lens, q, Hq, Hkv, D, seed, bs=16):
+    """(query, kc, vc, tables, lens, scale keywords) with every row's blocks its own."""
+    g = torch.Generator().manual_seed(seed)
+    n = [(x + q + bs - 1) // bs for x in lens]
+    nb, M = sum(n) + 1, max(n)
+    perm = torch.randperm(nb, generator=g).int()
+    tables = torch.zeros(len(lens), M, dtype=torch.int32)
+    at = 0
+    for b, k in enumerate(n):
+        tables[b, :k] = perm[at: at + k]
+        at += k
+    dt = BF if cache == F8 else cache
+    query = torch.randn(len(lens), Hq, q, D, generator=g).to(dt).cuda()
+    kw = {}
+    if cache == F8:
+        pool = _random_pool(g, nb, 1, Hkv, bs, D)
+        kc, vc = pool.k_layer_view(0), pool.v_layer_view(0)
+        kw = {"key_scales": pool.k_layer_scales(0), "value_scales": pool.v_layer_scales(0)}
+    else:
+        kc, vc = (torch.randn(nb, Hkv, bs, D, generator=g).to(dt).cuda() for _ in range(2))
+    return query, kc, vc, tables, torch.tensor(lens, dtype=torch.int32), kw
+
+
+@pytest.mark.parametrize("q,B", [(1, 5), (5, 40), (40, 20)])
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 4.0])
+@pytest.mark.parametrize("cache", KINDS)
+def test_attention_scales_of_any_sign_and_size(cache, scale, q, B):
+    query, kc, vc, tables, lens, kw = _case(cache, [3 + 7 * (i % 9) for i in range(B)], q, 16, 8, 64, 11)
+    for mods in ((ScoreModifiers(window=20), ScoreModifiers(softcap=3.0)) if cache != F8 else
+                 (None, ScoreModifiers(softcap=3.0, window=20))):
+        out = paged_attention_decode(query, kc, vc, tables.cuda(), lens.cuda(), scale, score_modifiers=mods,
+                                     validate=True, **kw)
+        ref, bar = attend64(query, kc, vc, tables, lens, scale, softcap=mods.softcap if mods else 0.0,
+                            window=mods.window if mods else 0, **kw)
+        check(out, ref, bar)
+
+
+@pytest.mark.parametrize("q,B", [(1, 5), (1, 200), (40, 20)])
+def test_zero_scales(q, B):
+    """Blocks of zeros held under a scale of 0: a score of 0, a value of 0; rows of
+    nothing but such blocks too."""
+    query, kc, vc, tables, lens, kw = _case(F8, [30 + 5 * (i % 7) for i in range(B)], q, 16, 8, 64, 12)
+    kw["key_scales"][tables[0, 0].item()] = 0
+    kw["value_scales"][tables[1, 0].item()] = 0
+    for t in range((35 + q + 16) // 16):
+        kw["value_scales"][tables[2, t].item()] = 0
+        kw["key_scales"][tables[3, t].item()] = 0
+    for mods in (None, ScoreModifiers(window=25)):
+        out = paged_attention_decode(query, kc, vc, tables.cuda(), lens.cuda(), 0.125, score_modifiers=mods,
+                                     validate=True, **kw)
+        ref, bar = attend64(query, kc, vc, tables, lens, 0.125, window=mods.window if mods else 0, **kw)
+        check(out, ref, bar)
+
+
+@pytest.mark.parametrize("q,B", [(1, 3), (1, 200), (40, 20)])
+@pytest.mark.parametrize("cache", KINDS)
+def test_tables_too_short_for_the_lengths(cache, q, B):
+    """Flagged; the other rows are as they should be."""
+    query, kc, vc, tables, lens, kw = _case(cache, [20 + i % 5 for i in range(B)], q, 16, 8, 64, 13)
+    mods = None if cache == F8 else ScoreModifiers(softcap=9.0)
+    long = lens.clone()
+    long[1] = 10**6
+    args = (query, kc, vc, tables.cuda())
+    with pytest.raises(IndexError):
+        paged_attention_decode(*args, long.cuda(), 0.125, score_modifiers=mods, validate=True, **kw)
+    out = paged_attention_decode(*args, long.cuda(), 0.125, score_modifiers=mods, validate=False, **kw)
+    assert read_device_errors() == _lib.PA_DEVERR_TABLE_UNDERRUN
+    want = paged_attention_decode(*args, lens.cuda(), 0.125, score_modifiers=mods, validate=True, **kw)
+    keep = torch.arange(B) != 1
+    ref, bar = attend64(query[keep], kc, vc, tables[keep], lens[keep], 0.125, softcap=mods.softcap if mods else 0.0, **kw)
+    check(want[keep], ref, bar)
+    check(out[keep], ref, bar)
+
+
+def test_empty_calls():
+    for cache in KINDS:
+        query, kc, vc, tables, lens, kw = _case(cache, [5, 9], 1, 8, 2, 64, 14)
+        mods = ScoreModifiers(window=3, key_starts=_i32([]))
+        for _ in range(2):
+            out = paged_attention_decode(query[:0], kc, vc, tables[:0].cuda(), lens[:0].cuda(), 0.125,
+                                         score_modifiers=mods, **kw)
+            assert out.shape == (0, 8, 1, 64)
+        if cache == F8:
+            none = torch.zeros(0, 2, 1, 64, device="cuda")
+            kv_append(none, none, kc, vc, torch.zeros(0, dtype=torch.int64, device="cuda"), **kw)
+    pages = DevicePages(4, 16, 4, 4)
+    for _ in range(2):
+        pages.free(_i32([]))
+        pages.fork(_i32([]), _i32([]))
+        pages.reserve(_i32([]), _i32([]))
+    assert pages.read_errors() == 0 and read_device_errors() == 0
