@@ -666,29 +666,28 @@ def kv_append(
         args.position_offset = int(position_offset)
     args.batch, args.q_len, args.num_kv_heads, args.head_dim, args.block_size = B, q_len, Hkv, Dc, bs
     args.dtype = _DTYPE_CODE[key.dtype]
+    # an extended call's append reports where that call does
+    host = error_word if isinstance(error_word, _HostWord) else None
     if scales is not None and error_word is None:
         host = host_word(device)
-        if validate is None:
-            host.raise_landed()
-        args.error_flags = host.ptr
-        with _with_device(device):
-            _lib.check(_lib.load().pa_kv_append_8bit(ctypes.byref(args), ctypes.byref(scales), _stream_ptr(device)),
-                       "pa_kv_append_8bit")
-        host.finish(validate)
-        return
-    if error_word is None:
+    if error_word is None and host is None:
         error_word = decode_workspace(device)
-    args.error_flags = error_word.data_ptr()
+    args.error_flags = host.ptr if host is not None else error_word.data_ptr()
     deferred = validate is None and not _VALIDATE_DEFAULT and not _capturing()
     if deferred:
-        _raise_landed_errors(error_word)
+        if host is not None:
+            host.raise_landed()
+        else:
+            _raise_landed_errors(error_word)
     with _with_device(device):
         if scales is not None:
             _lib.check(_lib.load().pa_kv_append_8bit(ctypes.byref(args), ctypes.byref(scales), _stream_ptr(device)),
                        "pa_kv_append_8bit")
         else:
             _lib.check(_lib.load().pa_kv_append(ctypes.byref(args), _stream_ptr(device)), "pa_kv_append")
-    if deferred:
+    if host is not None:
+        host.finish(validate)
+    elif deferred:
         _copy_after_call(error_word, _stream_ptr(device))
     elif validate if validate is not None else _VALIDATE_DEFAULT:
         flags = read_device_errors(workspace=error_word)
@@ -832,7 +831,7 @@ def paged_attention_decode(
             key, value, key_cache, value_cache, slot_mapping,
             block_tables=block_tables, positions=context_lens,
             position_offset=-q_len if context_lens_include_new else 0,
-            error_word=None if host is not None and scales is not None else workspace, validate=False,
+            error_word=host if host is not None else workspace, validate=False,
             key_scales=key_scales, value_scales=value_scales,
         )
         appended = True
@@ -889,7 +888,8 @@ def paged_attention_decode(
                     paged_attention_decode(query[lo:hi], key_cache, value_cache, block_tables[lo:hi],
                                            context_lens[lo:hi], scale, out=out[lo:hi],
                                            context_lens_include_new=context_lens_include_new,
-                                           workspace=workspace, validate=False, key_scales=key_scales,
+                                           workspace=workspace if host is None else None, validate=False,
+                                           key_scales=key_scales,
                                            value_scales=value_scales,
                                            score_modifiers=None if score_modifiers is None
                                            else score_modifiers.rows(lo, hi))

@@ -493,3 +493,31 @@ def test_empty_calls():
         pages.fork(_i32([]), _i32([]))
         pages.reserve(_i32([]), _i32([]))
     assert pages.read_errors() == 0 and read_device_errors() == 0
+
+
+@pytest.mark.parametrize("cache", KINDS)
+def test_errors_of_every_part_of_a_call_are_reported(cache):
+    """The append of a changed-score call, and the halves of a batch beyond one launch."""
+    query, kc, vc, tables, lens, kw = _case(cache, [5, 9], 1, 8, 2, 64, 15)
+    kw["score_modifiers"] = ScoreModifiers(window=30)
+    rows = torch.zeros(2, 2, 1, 64, dtype=query.dtype, device="cuda")
+    args = (query, kc, vc, tables.cuda(), lens.cuda(), 0.125)
+    bad = dict(key=rows, value=rows, slot_mapping=torch.tensor([10**6, -1]).cuda())
+    with pytest.raises(IndexError, match="slot"):
+        paged_attention_decode(*args, validate=True, **bad, **kw)
+    for how in ({}, {"out": torch.empty_like(query)}, {"validate": False}):
+        paged_attention_decode(*args, **bad, **how, **kw)
+        torch.cuda.synchronize()
+        with pytest.raises(IndexError, match="slot"):
+            paged_attention_decode(*args, **kw)
+    B = 9000
+    many = torch.zeros(B, 1, dtype=torch.int32, device="cuda")
+    many[B - 1] = 10**6
+    big = (query[:1].expand(B, 8, 1, 64).contiguous(), kc, vc, many, torch.full((B,), 3, dtype=torch.int32).cuda(), 0.125)
+    with pytest.raises(IndexError, match="block"):
+        paged_attention_decode(*big, validate=True, **kw)
+    paged_attention_decode(*big, **kw)
+    torch.cuda.synchronize()
+    with pytest.raises(IndexError, match="block"):
+        paged_attention_decode(*big, **kw)
+    assert read_device_errors() == 0
