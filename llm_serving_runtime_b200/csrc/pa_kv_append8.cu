@@ -46,6 +46,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxBlock = 256;  // tokens of a block
 constexpr int kBatch = 8;       // pieces of 8 elements that a lane holds
+constexpr int kHeld = 4;        // and of codes that are rounded again
 
 // Eight neighbouring elements as they are in memory, and widened; kWide: loaded
 // 16 bytes at a time.
@@ -299,24 +300,33 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const float scale = fmaxf(held, needed_scale(amax));
-  const bool pow2 = (__float_as_uint(scale) & 0x7fffffu) == 0u;
-  const float inv = 1.f / scale;  // exact where scale is a power of two
-  for (int base = 0; base < items; base += kBatch * 32) {
-    if (items > kBatch * 32) load(base);
+  if ((__float_as_uint(scale) & 0x7fffffu) == 0u) {
+    const float inv = 1.f / scale;  // exact: a power of two
+    for (int base = 0; base < items; base += kBatch * 32) {
+      if (items > kBatch * 32) load(base);
 #pragma unroll
-    for (int n = 0; n < kBatch; ++n) {
-      const int i = base + n * 32 + lane;
-      if (i >= items) continue;
-      float v[8];
-      x[n].widen(v);
-      if (pow2) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], scale);
+      for (int n = 0; n < kBatch; ++n) {
+        const int i = base + n * 32 + lane;
+        if (i >= items) continue;
+        float v[8];
+        x[n].widen(v);
+        const int r = token_of(i);
+        *reinterpret_cast<uint2*>(dst + s_run[r].x * dst_t + (i - r * chunks) * 8) =
+            make_uint2(codes4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+                       codes4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv));
       }
+    }
+  } else {
+    // a scale that was found in the cache; short code (the kernel runs once, its fetch counts)
+#pragma unroll 1
+    for (int i = lane; i < items; i += 32) {
       const int r = token_of(i);
+      Piece<T> y;
+      y.template load<kWide>(src + s_run[r].y * src_t + (i - r * chunks) * 8);
+      float v[8];
+      y.widen(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = __fdiv_rn(v[j], scale);
       *reinterpret_cast<uint2*>(dst + s_run[r].x * dst_t + (i - r * chunks) * 8) =
           make_uint2(codes4(v[0], v[1], v[2], v[3]), codes4(v[4], v[5], v[6], v[7]));
     }
@@ -324,16 +334,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
   if (!fresh && scale != held) {
     // the block's other tokens to the new scale
     const float ratio = __fdiv_rn(held, scale);
-    for (int base = 0; base < bs * chunks; base += kBatch * 32) {
-      uint2 c[kBatch];
+    for (int base = 0; base < bs * chunks; base += kHeld * 32) {
+      uint2 c[kHeld];
 #pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
+      for (int n = 0; n < kHeld; ++n) {
         const int i = base + n * 32 + lane, o = token_of(i);
         if (i < bs * chunks && !((s_taken[o >> 5] >> (o & 31)) & 1u))
           c[n] = *reinterpret_cast<const uint2*>(dst + o * dst_t + (i - o * chunks) * 8);
       }
 #pragma unroll
-      for (int n = 0; n < kBatch; ++n) {
+      for (int n = 0; n < kHeld; ++n) {
         const int i = base + n * 32 + lane, o = token_of(i);
         if (i >= bs * chunks || ((s_taken[o >> 5] >> (o & 31)) & 1u)) continue;
         float2 f[4] = {two_values(c[n].x), two_values(c[n].x >> 16), two_values(c[n].y), two_values(c[n].y >> 16)};
