@@ -25,8 +25,8 @@
 // 2458 live ones (525 MB moved) 97 us, of it plan 6, tables 4, copies 83 (6.3 TB/s).  The
 // planning kernels are one CTA each: a prefix sum over counts in tiles of 4096, the
 // next tile's loads issued before the current one is summed.  64 beams replaced by
-// forks over 6000 pages: free 4, fork 8 + 6, reserve 8 us, chains of five to seven
-// dependent loads and barriers.
+// forks over 6000 pages: free 4, fork 8 + 6, reserve 8 us with cold caches, some 14 us
+// in a row, mostly launches (marks and lists in shared memory saved 0.2).
 #include <limits.h>
 
 #include "pa_common.cuh"

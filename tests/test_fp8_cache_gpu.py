@@ -152,6 +152,31 @@ def test_long_padding_between_a_blocks_tokens():
     c.append(rows.to(BF), rows.to(BF), slots, q=q)
 
 
+@pytest.mark.parametrize("H", [1, 5])
+@pytest.mark.parametrize("clash", [False, True])
+def test_many_runs_among_neighbouring_tokens(H, clash):
+    """Slots in any order: runs of one to three tokens, padding between them, two rows;
+    with a block that the row, or the other row, comes back to."""
+    g = _gen(62)
+    bs, q = 16, 75
+    blocks = torch.randperm(200, generator=g).tolist()
+    slots = torch.full((2, q), -1, dtype=torch.int64)
+    for b in range(2):
+        t = 0
+        while t < q:
+            blk = blocks.pop()
+            for o in torch.randperm(bs, generator=g)[: 1 + t % 3].tolist():
+                if t < q and t % 7 != 5:
+                    slots[b, t] = blk * bs + o
+                t += 1
+    if clash:
+        slots[0, 60] = slots[0, 2] // bs * bs + 9
+        slots[1, 30] = slots[0, 20]
+    c = Append(200, H, bs, 32, 62)
+    k, v = _rows(2, H, q, 32, g, BF), _rows(2, H, q, 32, g, BF)
+    c.append(k, v, slots.reshape(-1), q=q, flags=_lib.PA_DEVERR_BLOCK_CONFLICT if clash else 0)
+
+
 def test_a_slot_given_twice_takes_the_last_token():
     g = _gen(6)
     c = Append(4, 2, 16, 64, 6)
