@@ -1,12 +1,11 @@
-// pa_decode_direct.cu — pa_decode_ext for few rows: a row (sequence, KV head,
-// group of 16 query rows) gets CTAs of its own.
+// pa_decode_direct.cu — pa_decode_ext for few rows, or rows that cannot be long: a
+// row (sequence, KV head, group of 16 query rows) gets CTAs of its own.
 //
 // The stream-K kernel (pa_decode_kernel.cuh) balances any batch, but a warp that
 // crosses rows pays for each start and end, a warp's least share is several units,
-// and a long row's many pieces are merged by one warp.  With no more rows than
-// CTAs fit the GPU none of that is needed: CTA (row, s) takes the s-th of S equal
-// ranges of the row's units, its warps an equal part of it each (their own ring
-// of TMA tiles, as there), and merges their states in shared memory; the last CTA
+// and a long row's many pieces are merged by one warp.  None of that is needed here:
+// CTA (row, s) takes the s-th of S equal ranges of the row's units, its warps an equal
+// part of it each (their own ring of TMA tiles, as there), and merges their states in shared memory; the last CTA
 // of a row to finish merges the S partial states, all threads together, with the
 // log-sum-exp rule, in the order of the ranges.  S is at most the launch's second
 // dimension and leaves every CTA chunk_units units or more (known on the device
@@ -16,8 +15,8 @@
 // Bound: issue and latency of a unit's chain (products, maxima, exponentials; 170
 // registers leave 12 warps an SM), then what a row pays once.  96 x 4 tokens of 16
 // to 2048 cached ones, 8 KV heads (768 rows, 90 MB of codes) 38 us at 1.7 instructions
-// a clock; of a CTA's 12 us some 5 are lengths, table, queries, first tile and the
-// merge.  128 rows with a window of 1024 (16-bit, 441 MB) 77 us, 5.7 TB/s; one row of
+// a clock; a CTA pays 3 us for lengths, table, first tile and merge, and its queries
+// and output.  128 rows with a window of 1024 (16-bit, 441 MB) 77 us, 5.7 TB/s; one row of
 // 32k 20 us, 3.3 TB/s.
 #include "pa_common.cuh"
 #include "pa_internal.h"
