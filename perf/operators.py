@@ -241,7 +241,7 @@ def prepare(c, seed):
     st["prefix"] = torch.full((B,), c["prefix"], dtype=torch.int32, device=dev) if c["prefix"] else None
     st["slopes"] = (torch.exp2(-8.0 * torch.arange(1, c["Hq"] + 1, device=dev, dtype=torch.float32) / c["Hq"])
                     if c["alibi"] else None)
-    if own and (c["cache"] == "same" or c["softcap"] or c["window"] or c["alibi"] or c["document"] or c["prefix"]):
+    if own and (c["softcap"] or c["window"] or c["alibi"] or c["document"] or c["prefix"]):
         from llm_serving_runtime_b200 import ScoreModifiers
 
         st["mods"] = ScoreModifiers(softcap=c["softcap"], window=c["window"], alibi_slopes=st["slopes"],
