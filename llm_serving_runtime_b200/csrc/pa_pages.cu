@@ -102,13 +102,16 @@ __device__ int collect_free(const int32_t* refs, int n, int want, int32_t* list,
 }
 
 // Marks the first argument that names each slot: afterwards mark[slot] is its
-// index.  Arguments outside [0, slots) are passed over.  The whole block calls it.
-__device__ void mark_first(const int32_t* arg, int n, int slots, int32_t* mark) {
+// index.  Arguments outside [0, slots) are passed over, and so are those whose
+// partner (null: none) is negative: such a pair is padding and claims nothing.  The
+// whole block calls it.
+__device__ void mark_first(const int32_t* arg, const int32_t* partner, int n, int slots, int32_t* mark) {
+  auto names = [&](int i) { return arg[i] >= 0 && arg[i] < slots && (partner == nullptr || partner[i] >= 0); };
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (arg[i] >= 0 && arg[i] < slots) mark[arg[i]] = INT_MAX;
+    if (names(i)) mark[arg[i]] = INT_MAX;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += blockDim.x)
-    if (arg[i] >= 0 && arg[i] < slots) atomicMin(&mark[arg[i]], i);
+    if (names(i)) atomicMin(&mark[arg[i]], i);
   __syncthreads();
 }
 
@@ -238,7 +241,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Pag
   int32_t* fresh = mark + t.num_seqs;
   int32_t* len = fresh + t.num_seqs;
   int32_t* list = len + t.num_seqs;
-  mark_first(children, n, t.num_seqs, mark);
+  mark_first(children, parents, n, t.num_seqs, mark);
   int want = 0;
   for (int base = 0; base < n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_reserve_kernel(const PageT
   int32_t* mark = t.scratch;
   int32_t* rank = mark + t.num_seqs;
   int32_t* list = rank + 2 * t.num_seqs;
-  mark_first(slots, n, t.num_seqs, mark);
+  mark_first(slots, nullptr, n, t.num_seqs, mark);
   long long want = 0;  // pages asked for; at most n * max_blocks
   for (int base = 0; base < n; base += kPlanThreads) {
     const int i = base + threadIdx.x;
