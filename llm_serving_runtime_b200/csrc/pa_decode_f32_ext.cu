@@ -120,14 +120,23 @@ __global__ void __launch_bounds__(f32_warps(DPL * 32) * 32) decode_f32_ext_kerne
     // lane t < 16: block and offset of token t
     const int tok = u * kTile + (lane & 15);
     long long ko = -1, vo = 0;
+    bool zero = false;  // of a block outside the pool: zeros, as TMA fills them for the other types
     if (tok >= lo && tok < hi) {
       const int lb = tok / p.bs, off = tok - lb * p.bs;
       const int phys = __ldg(&p.block_tables[(long long)b * p.bt_stride + lb]);
       if (phys < 0 || phys >= p.num_blocks) {
         raise_flag(p.status, PA_DEVERR_BLOCK_ID_RANGE);
+        zero = true;
       } else {
         ko = phys * p.k_sblk + h * p.k_sh + off * p.k_st;
         vo = phys * p.v_sblk + h * p.v_sh + off * p.v_st;
+      }
+    }
+    for (uint32_t left = __ballot_sync(0xffffffffu, zero) & 0xffffu; left != 0u; left &= left - 1) {
+      const int t = __ffs(left) - 1;
+      for (int c = lane; c < D; c += 32) {
+        s_k[buf * kTile * PITCH + t * PITCH + c] = 0.f;
+        s_v[buf * kTile * D + t * D + c] = 0.f;
       }
     }
     constexpr int PER = D / kVec;  // copies of a row

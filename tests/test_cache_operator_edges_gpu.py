@@ -1,4 +1,5 @@
-"""Edges of the operators over a paged cache: padding pairs among forks."""
+"""Edges of the operators over a paged cache: padding pairs among forks, block ids outside
+the pool."""
 
 from __future__ import annotations
 
@@ -6,10 +7,11 @@ import numpy as np
 import pytest
 import torch
 
-from _ops64 import Pages
-from llm_serving_runtime_b200 import DevicePages
+from _ops64 import F8, Pages
+from llm_serving_runtime_b200 import DevicePages, ScoreModifiers, paged_attention_decode, read_device_errors
 
 pytestmark = pytest.mark.gpu
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
 
 
 def _i32(x):
@@ -53,3 +55,56 @@ def test_forks_among_padding_pairs(seed):
         children = rng.integers(full, S, n)
         _step(pages, table, "fork", parents.tolist(), children.tolist())
         _step(pages, table, "free", rng.permutation(np.arange(full, S))[: (S - full) // 2].tolist())
+
+
+def _attend_case(cache, lens, q, Hq, Hkv, D, bs, seed):
+    """(query, kc, vc, tables, lens, scale keywords); the pool's last block holds zeros
+    (of scale 0), and no table names it."""
+    g = torch.Generator().manual_seed(seed)
+    n = [(x + q + bs - 1) // bs for x in lens]
+    nb = sum(n) + 1
+    tables = torch.zeros(len(lens), max(n), dtype=torch.int32)
+    at = 0
+    for b, k in enumerate(n):
+        tables[b, :k] = torch.arange(at, at + k)
+        at += k
+    dt = BF if cache == F8 else cache
+    query = torch.randn(len(lens), Hq, q, D, generator=g).to(dt).cuda()
+    kc, vc = ((torch.randn(nb, Hkv, bs, D, generator=g) * 4).to(cache) for _ in range(2))
+    kc.view(torch.uint8)[-1] = vc.view(torch.uint8)[-1] = 0
+    kw = {}
+    if cache == F8:
+        for name in ("key_scales", "value_scales"):
+            s = torch.rand(nb, Hkv, generator=g) + 0.25
+            s[-1] = 0
+            kw[name] = s.cuda()
+    return query, kc.cuda(), vc.cuda(), tables, _i32(lens), kw
+
+
+@pytest.mark.parametrize("q,B", [(1, 6), (1, 20), (3, 40), (40, 20), (40, 40)])
+@pytest.mark.parametrize("cache,D", [(FP, 32), (FP, 33), (FP, 64), (FP, 128), (BF, 64), (HF, 128), (F8, 64)])
+def test_a_bad_block_counts_as_zeros(cache, D, q, B):
+    """A block id outside the pool is flagged and read as zeros, never as what the shared
+    memory of the GPU still holds: the same bits as a block of zeros, call after call."""
+    lens = [70, 16, 5, 300] + [90 + 7 * i for i in range(B - 4)]
+    query, kc, vc, tables, lens, kw = _attend_case(cache, lens, q, 8, 4, D, 16, 31)
+    nb = kc.shape[0]
+    where = [(0, 0), (0, 2), (1, 0), (3, 1), (3, 7), (3, 18), (5, 3)]
+    zeros = tables.clone()
+    for b, i in where:
+        zeros[b, i] = nb - 1
+    mods = ScoreModifiers(softcap=20.0)
+    want = paged_attention_decode(query, kc, vc, zeros.cuda(), lens, 0.2, score_modifiers=mods, validate=True, **kw)
+    assert bool(want.isfinite().all())
+    for bad in (-1, nb, nb + 1000):
+        wrong = tables.clone()
+        for b, i in where:
+            wrong[b, i] = bad
+        wrong = wrong.cuda()
+        for _ in range(3):
+            # fills shared memory with other numbers
+            paged_attention_decode(query, kc * 3 if cache != F8 else kc, vc, tables.cuda(), lens, 0.2,
+                                   score_modifiers=mods, **kw)
+            out = paged_attention_decode(query, kc, vc, wrong, lens, 0.2, score_modifiers=mods, validate=False, **kw)
+            assert read_device_errors() & 0x1
+            assert torch.equal(out, want)
