@@ -85,7 +85,9 @@ typedef struct pa_cache_view {
  *   slot = block_tables[b, p / bs] * bs + p % bs,
  *          p = positions[b] + position_offset + t                      (otherwise)
  * and lands in cache[slot / bs, h, slot % bs, :].  A negative slot_mapping entry
- * marks a padding token and is skipped. */
+ * marks a padding token and is skipped, and so is a row whose position is 0 where
+ * position_offset is -q_len: its length counts the new tokens, so it has none (an
+ * empty slot of a table of sequences).  Other negative p are flagged. */
 typedef struct pa_kv_append_args {
   const void* key;
   int64_t key_stride_b, key_stride_h, key_stride_t;

@@ -172,6 +172,15 @@ struct AppendParams {
   uint32_t* error_flags;
 };
 
+// A row whose position counts this call's tokens and is 0 (an empty slot of a table of
+// sequences): it has no tokens, which is no error.
+#ifdef __CUDACC__
+__host__ __device__
+#endif
+inline bool empty_row(const AppendParams& p, long long position) {
+  return position == 0 && p.position_offset == -p.q_len;
+}
+
 // Scales of an 8-bit cache that an append writes (strides in elements).
 struct ScaleParams {
   float* k_scales;

@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const AppendParams p) {
                                   : (long long)static_cast<const int32_t*>(p.positions)[b];
       const long long pos = start + p.position_offset + t;
       if (pos < 0) {
-        if (reporter) raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
+        if (reporter && !empty_row(p, start)) raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
         continue;
       }
       const long long lb = pos / p.bs;

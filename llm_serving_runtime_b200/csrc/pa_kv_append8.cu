@@ -198,7 +198,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 2)
     if constexpr (!kSlots) {
       if (tid < (int)blockIdx.x) other = block_of_run(tid);  // in flight beside this run's own
       const long long pos0 = first_position(p, b);
-      if (pos0 < 0 && k == 0 && tid == 0 && blockIdx.y == 0) raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
+      if (pos0 < 0 && k == 0 && tid == 0 && blockIdx.y == 0 && !empty_row(p, pos0 - p.position_offset))
+        raise_flag(p.error_flags, PA_DEVERR_SLOT_RANGE);
       const long long lb = ((pos0 < 0 ? 0 : pos0) >> bs_log2) + k;
       const long long t0 = max(0LL, (lb << bs_log2) - pos0), t1 = min((long long)p.q_len, ((lb + 1) << bs_log2) - pos0);
       if (t0 >= t1) return;

@@ -10,7 +10,8 @@
 * ``block_tables`` int32 [B, max_blocks]: physical block of each logical block
 * ``context_lens`` int32 [B]: tokens already cached BEFORE this step's q_len new
   tokens (pass ``context_lens_include_new=True`` for the reference's seq_lens,
-  which include them, runtime/phase2/paged_attention_triton.py:50)
+  which include them, runtime/phase2/paged_attention_triton.py:50; a row of length 0
+  then has no tokens: nothing is appended for it and its output is zero)
 * ``scale``        softmax scale (usually head_dim ** -0.5)
 * ``slot_mapping`` int64 [B * q_len] or None: cache slot (block * bs + offset) of
   each new token; -1 skips a padding token.  When None and ``key``/``value``
@@ -598,7 +599,9 @@ def kv_append(
     otherwise to block_tables[b, p // bs] at offset p % bs with
     p = positions[b] + position_offset + t.  Bit-exact.  Invalid slots or block
     ids are skipped and flagged; the next call on the same error word raises
-    IndexError (``validate=True``: this call, synchronously).
+    IndexError (``validate=True``: this call, synchronously).  A row at position 0
+    under a position_offset of -q_len is empty (its length counts the new tokens) and
+    is skipped without an error, like a slot of -1.
 
     A cache of ``torch.float8_e4m3fn`` takes ``key_scales`` / ``value_scales``
     (float32 [num_blocks, Hkv], any strides) and rows of fp32, fp16 or bf16: the

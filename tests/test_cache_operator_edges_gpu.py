@@ -1,5 +1,5 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
-the pool."""
+the pool, empty slots."""
 
 from __future__ import annotations
 
@@ -8,7 +8,14 @@ import pytest
 import torch
 
 from _ops64 import F8, Pages
-from llm_serving_runtime_b200 import DevicePages, ScoreModifiers, paged_attention_decode, read_device_errors
+from llm_serving_runtime_b200 import (
+    DevicePages,
+    ScoreModifiers,
+    kv_append,
+    paged_attention_decode,
+    read_device_errors,
+)
+from llm_serving_runtime_b200.kv_block_pool import Fp8KVBlockPool
 
 pytestmark = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -108,3 +115,77 @@ def test_a_bad_block_counts_as_zeros(cache, D, q, B):
             out = paged_attention_decode(query, kc, vc, wrong, lens, 0.2, score_modifiers=mods, validate=False, **kw)
             assert read_device_errors() & 0x1
             assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("q", [1, 3])
+@pytest.mark.parametrize("cache", [BF, HF, FP, F8])
+def test_a_loop_over_slots_some_of_which_are_empty(cache, q):
+    """The whole table of a DevicePages goes into the call: a slot of length 0 has no new
+    tokens, its rows are zero, nothing is written for it and nothing reported."""
+    g = torch.Generator().manual_seed(5)
+    P, bs, S, M, Hq, Hkv, D = 40, 16, 6, 8, 8, 2, 64
+    dt = BF if cache == F8 else cache
+    pages = DevicePages(P, bs, S, M)
+    live = [1, 4]
+    pages.reserve(_i32(live), _i32([40, 15]), validate=True)
+    kw = {"score_modifiers": ScoreModifiers(softcap=30.0)}
+    if cache == F8:
+        pool = Fp8KVBlockPool(P, 1, Hkv, bs, D)
+        kc, vc = pool.k_layer_view(0), pool.v_layer_view(0)
+        kw.update(key_scales=pool.k_layer_scales(0), value_scales=pool.v_layer_scales(0))
+    else:
+        kc, vc = (torch.randn(P, Hkv, bs, D, generator=g).to(cache).cuda() for _ in range(2))
+    forms = [kw] if cache == F8 else [kw, {}]  # plain attention too
+    for step in range(4):
+        if step == 2:
+            pages.free(_i32([4]), validate=True)
+            live = [1]
+        pages.reserve(_i32(live), _i32([q] * len(live)), validate=True)
+        query = torch.randn(S, Hq, q, D, generator=g).to(dt).cuda()
+        key, value = (torch.randn(S, Hkv, q, D, generator=g).to(dt).cuda() for _ in range(2))
+        rows = torch.tensor(live).cuda()
+        for form in forms:
+            state = [t.clone() for t in (kc, vc, *(form[s] for s in ("key_scales", "value_scales") if s in form))]
+            outs, caches = [], []
+            for validate in (True, None):
+                for t, s in zip((kc, vc, form.get("key_scales"), form.get("value_scales")), state):
+                    t.copy_(s)
+                outs.append(paged_attention_decode(query, kc, vc, pages.block_tables, pages.seq_lens, 0.125, key=key,
+                                                   value=value, context_lens_include_new=True, validate=validate,
+                                                   **form))
+                caches.append([t.float() for t in (kc, vc)])
+            assert read_device_errors() == 0
+            for t, s in zip((kc, vc, form.get("key_scales"), form.get("value_scales")), state):
+                t.copy_(s)
+            want = paged_attention_decode(query[rows], kc, vc, pages.block_tables[rows], pages.seq_lens[rows], 0.125,
+                                          key=key[rows], value=value[rows], context_lens_include_new=True,
+                                          validate=True, **form)
+            for out, cache_after in zip(outs, caches):
+                # plain 16-bit attention splits its work by the batch: both sides round their
+                # weights (2^-11 at most) and their outputs
+                bar = 0.0 if form or cache == FP else float(torch.finfo(dt).eps * want.abs().max()
+                                                            + 2.0**-10 * max(vc.abs().max(), value.abs().max()))
+                assert float((out[rows] - want).abs().max()) <= bar
+                assert sum(int(x) for x in out.abs().sum((1, 2, 3)) != 0) == len(live)
+                for a, t in zip(cache_after, (kc, vc)):
+                    assert torch.equal(a, t.float())
+
+
+@pytest.mark.parametrize("cache", [BF, F8])
+def test_other_tokens_before_the_start_are_still_reported(cache):
+    """Only a whole row of length 0 is empty: a negative position, or a length that is less
+    than its new tokens, stays an error."""
+    P, bs, Hkv, D = 6, 16, 2, 64
+    kc, vc = (torch.zeros(P, Hkv, bs, D, device="cuda").to(cache) for _ in range(2))
+    kw = {n: torch.zeros(P, Hkv, device="cuda") for n in ("key_scales", "value_scales")} if cache == F8 else {}
+    rows = torch.ones(2, Hkv, 2, D, dtype=BF, device="cuda")
+    tables = _i32([[1, 2], [3, 4]])
+
+    def append(positions, offset):
+        kv_append(rows, rows, kc, vc, block_tables=tables, positions=_i32(positions), position_offset=offset,
+                  validate=True, **kw)
+
+    append([0, 5], -2)  # length 0, and a row whose two tokens are its last
+    for positions, offset in (([1, 5], -2), ([0, 5], -1), ([-2, 5], 0), ([-1, 5], -2)):
+        with pytest.raises(IndexError, match="slot"):
+            append(positions, offset)
