@@ -423,6 +423,14 @@ PA_API int pa_workspace_init(void* workspace, size_t workspace_bytes, void* stre
  * (paged_kv_kernel.py:118-119, :167-170, :221-222). */
 PA_API int pa_read_device_errors(void* device_word, uint32_t* host_flags, int32_t clear, void* stream);
 
+/* Takes the bits of an error word that other streams may report into meanwhile
+ * (pa_decode_ext's or pa_pages_*' in pinned host memory, say): *taken = *word and
+ * *word = 0 in one exchange on the device, behind the work on `stream`, so that no
+ * bit is lost.  Both are words of device or pinned host memory; the caller waits
+ * for `stream` before it reads *taken.  No counterpart in the reference, which
+ * checks on the host. */
+PA_API int pa_take_error_word(uint32_t* word, uint32_t* taken, void* stream);
+
 /* Text for the last failure on this host thread ("" when none). */
 PA_API const char* pa_last_error(void);
 

@@ -59,6 +59,7 @@ EXPORTED_SYMBOLS = (
     "pa_decode_workspace_bytes",
     "pa_workspace_init",
     "pa_read_device_errors",
+    "pa_take_error_word",
     "pa_last_error",
     "pa_last_kernel",
     "pa_version",
@@ -269,6 +270,8 @@ def load() -> ctypes.CDLL:
         lib.pa_pages_reserve.argtypes = [tables, _vp, _vp, _i32, _vp]
         lib.pa_pages_compact.restype = ctypes.c_int
         lib.pa_pages_compact.argtypes = [tables, views, _i32, _vp, _vp]
+        lib.pa_take_error_word.restype = ctypes.c_int
+        lib.pa_take_error_word.argtypes = [_vp, _vp, _vp]
         lib.pa_decode_workspace_bytes.restype = _sz
         lib.pa_decode_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32, _i32]
         lib.pa_workspace_init.restype = ctypes.c_int

@@ -279,6 +279,9 @@ namespace pa {
 
 int set_last_error(int status, const char* msg) { return fail(status, "%s", msg); }
 
+// The kernels OR their bits into a word with atomics, so taking them has to be one too.
+__global__ void take_word_kernel(uint32_t* word, uint32_t* taken) { *taken = atomicExch(word, 0u); }
+
 size_t ws_counter_bytes(int nw_total) { return round_up((size_t)nw_total * 4); }
 
 size_t ws_partial_bytes(int nw_total, int slot_rows, int D) {
@@ -333,6 +336,15 @@ int pa_read_device_errors(void* device_word, uint32_t* host_flags, int32_t clear
   }
   e = cudaStreamSynchronize(s);
   if (e != cudaSuccess) return cuda_fail(e, "cudaStreamSynchronize");
+  return PA_OK;
+}
+
+int pa_take_error_word(uint32_t* word, uint32_t* taken, void* stream) {
+  g_last_error[0] = 0;
+  if (word == nullptr || taken == nullptr) return fail(PA_ERR_INVALID_ARGUMENT, "null pointer");
+  pa::take_word_kernel<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(word, taken);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "take_error_word launch");
   return PA_OK;
 }
 

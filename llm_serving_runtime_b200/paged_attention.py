@@ -188,11 +188,11 @@ def read_device_errors(device: torch.device | None = None, *, clear: bool = True
         device = device or torch.device("cuda", torch.cuda.current_device())
         workspace = decode_workspace(device)
         word = _host_words.get(workspace.device.index)
-        if word is not None:
+        if word is not None and clear:
+            host = word.take()
+        elif word is not None:
             torch.cuda.current_stream(word.device).synchronize()
             host = int(word.word.value)
-            if clear:
-                word.word.value = 0
     if clear:
         with _checks_lock:
             c = _checks.get((workspace.device.index, workspace.data_ptr()))
@@ -308,9 +308,11 @@ class _HostWord:
     """A device error word in pinned host memory, for the kernels of the extended
     operators (8-bit caches, score modifiers, pages): a kernel's atomic OR reaches it
     directly, so looking for the errors of earlier calls is one host read, with
-    no copy queued behind each call."""
+    no copy queued behind each call.  The host only reads it: kernels of any stream may
+    report at any time, so the bits are taken by an exchange on the device, into the
+    word behind it."""
 
-    __slots__ = ("ptr", "word", "device")
+    __slots__ = ("ptr", "word", "taken", "device")
 
     # Words come out of slabs that stay: a kernel or captured graph may still report
     # into the word of an object that is gone.
@@ -322,21 +324,26 @@ class _HostWord:
         with _HostWord._lock:
             if _HostWord._left == 0:
                 _HostWord._slabs.append(torch.zeros(1024, dtype=torch.int32, pin_memory=True))
-                _HostWord._left = 1024
+                _HostWord._left = 512
             _HostWord._left -= 1
-            self.ptr = _HostWord._slabs[-1].data_ptr() + 4 * _HostWord._left
+            self.ptr = _HostWord._slabs[-1].data_ptr() + 8 * _HostWord._left
         self.word = ctypes.c_uint32.from_address(self.ptr)
+        self.taken = ctypes.c_uint32.from_address(self.ptr + 4)
         self.device = device
 
     def take(self) -> int:
         """The bits so far, cleared, once the work on the current stream is done."""
-        torch.cuda.current_stream(self.device).synchronize()
-        flags, self.word.value = self.word.value, 0
-        return int(flags)
+        with _take_lock, _with_device(self.device):
+            _lib.check(_lib.load().pa_take_error_word(self.ptr, self.ptr + 4, _stream_ptr(self.device)),
+                       "pa_take_error_word")
+            torch.cuda.current_stream(self.device).synchronize()
+            return int(self.taken.value)
 
     def raise_landed(self) -> None:
         if self.word.value and not _capturing():
-            raise device_error(self.take())
+            flags = self.take()
+            if flags:  # else another thread has taken them
+                raise device_error(flags)
 
     def finish(self, validate: bool | None) -> None:
         """End of a call: the check that ``validate`` asks for."""
@@ -346,6 +353,7 @@ class _HostWord:
                 raise device_error(flags)
 
 
+_take_lock = threading.Lock()  # two takers of a word share the place that its bits go to
 _host_words: dict[int, _HostWord] = {}
 
 

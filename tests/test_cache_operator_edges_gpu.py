@@ -1,5 +1,5 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
-the pool, empty slots."""
+the pool, empty slots, error words read while other streams report."""
 
 from __future__ import annotations
 
@@ -11,7 +11,9 @@ from _ops64 import F8, Pages
 from llm_serving_runtime_b200 import (
     DevicePages,
     ScoreModifiers,
+    copy_pages,
     kv_append,
+    paged_attention,
     paged_attention_decode,
     read_device_errors,
 )
@@ -189,3 +191,97 @@ def test_other_tokens_before_the_start_are_still_reported(cache):
     for positions, offset in (([1, 5], -2), ([0, 5], -1), ([-2, 5], 0), ([-1, 5], -2)):
         with pytest.raises(IndexError, match="slot"):
             append(positions, offset)
+
+
+class _OtherStream:
+    """An error word seen by a host whose every look is followed at once by a report of a
+    kernel on another stream (here a new bit is set in the same memory)."""
+
+    def __init__(self, word):
+        self.word, self.reported, self.bits = word, 0, [0x100, 0x40, 0x20, 0x10]
+
+    @property
+    def value(self):
+        seen = self.word.value
+        self.reported |= self.bits[0]
+        self.word.value = seen | self.bits.pop(0)
+        return seen
+
+    @value.setter
+    def value(self, new):
+        self.word.value = new
+
+
+def test_no_report_is_lost_between_a_look_and_the_clearing(monkeypatch):
+    pages = DevicePages(8, 4, 4, 4)
+    word = pages._word
+    real = word.word
+    pages.reserve(_i32([9]), _i32([1]), validate=False)  # a slot outside the table: 0x80
+    torch.cuda.synchronize()
+    assert real.value == 0x80
+    other = _OtherStream(real)
+    monkeypatch.setattr(word, "word", other)
+    seen = word.take() if word.word.value else 0  # as the next call looks and then clears
+    monkeypatch.setattr(word, "word", real)
+    assert seen | word.take() == 0x80 | other.reported
+    assert word.take() == 0 and pages.read_errors() == 0
+
+
+def test_reading_the_devices_errors_loses_no_report(monkeypatch):
+    c = torch.zeros(8, 4, device="cuda")
+    copy_pages([c], _i32([1]), _i32([2]), validate=True)
+    word = paged_attention._host_words[0]
+    assert read_device_errors() == 0
+    real = word.word
+    copy_pages([c], _i32([99]), _i32([2]), validate=False)
+    torch.cuda.synchronize()
+    other = _OtherStream(real)
+    monkeypatch.setattr(word, "word", other)
+    seen = read_device_errors()
+    monkeypatch.setattr(word, "word", real)
+    assert seen & 0x1
+    assert seen | read_device_errors() == 0x1 | other.reported
+    assert word.take() == 0
+
+
+def test_an_error_that_another_thread_took_does_not_raise_again(monkeypatch):
+    c = torch.zeros(8, 4, device="cuda")
+    copy_pages([c], _i32([1]), _i32([2]), validate=True)
+    word = paged_attention._host_words[0]
+    real = word.word
+
+    class Taken:  # the look sees a bit, and another thread takes it before this one can
+        @property
+        def value(self):
+            return 0x1
+
+        @value.setter
+        def value(self, new):
+            real.value = new
+
+    monkeypatch.setattr(word, "word", Taken())
+    try:
+        word.raise_landed()
+    finally:
+        monkeypatch.setattr(word, "word", real)
+
+
+def test_errors_reported_while_others_are_read():
+    """Two streams report, one after each reading of the other's: every report raises
+    somewhere, and none twice."""
+    c = torch.zeros(8, 4, device="cuda")
+    copy_pages([c], _i32([1]), _i32([2]), validate=True)
+    word = paged_attention._host_words[0]
+    bad = [(_i32([99]), _i32([2])), (_i32([1, 1]), _i32([3, 3]))]
+    streams = [torch.cuda.Stream() for _ in bad]
+    torch.cuda.synchronize()
+    for _ in range(50):
+        seen = 0
+        for s, (src, dst) in zip(streams, bad):
+            with torch.cuda.stream(s):
+                copy_pages([c], src, dst, validate=False)
+                seen |= word.take()
+        torch.cuda.synchronize()
+        seen |= word.take()
+        assert seen == 0x41
+    assert word.take() == 0
