@@ -313,7 +313,8 @@ typedef struct pa_score_modifiers {
 
 /* pa_decode over an 8-bit cache (scales != NULL: args->dtype is the type of query
  * and out, fp16 or bf16; head_dim a multiple of 16) and / or with changed scores
- * (modifiers != NULL; any dtype).  Same workspace as pa_decode.  error_flags: a word
+ * (modifiers != NULL; any dtype).  A workspace as pa_decode's, of
+ * pa_decode_ext_workspace_bytes().  error_flags: a word
  * (device, or pinned host memory that the host reads itself) that receives the
  * PA_DEVERR_* bits instead of the workspace's first; may be NULL. */
 PA_API int pa_decode_ext(const pa_decode_args* args, const pa_cache_scales* scales,
@@ -411,6 +412,10 @@ PA_API int pa_decode_static_workspace(const pa_decode_args* args, void* stream);
  * never aliased to scratch. */
 PA_API size_t pa_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                  int32_t q_len, int32_t head_dim, int32_t dtype, int32_t device);
+
+/* The same for pa_decode_ext: more than pa_decode's for fp32 caches, else as much. */
+PA_API size_t pa_decode_ext_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                     int32_t q_len, int32_t head_dim, int32_t dtype, int32_t device);
 
 /* Zero a workspace (its merge counters and status word) on `stream`.  Needed
  * once after allocation; pa_decode leaves the counters at zero after each call.

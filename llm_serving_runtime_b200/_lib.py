@@ -57,6 +57,7 @@ EXPORTED_SYMBOLS = (
     "pa_pages_reserve",
     "pa_pages_compact",
     "pa_decode_workspace_bytes",
+    "pa_decode_ext_workspace_bytes",
     "pa_workspace_init",
     "pa_read_device_errors",
     "pa_take_error_word",
@@ -272,8 +273,9 @@ def load() -> ctypes.CDLL:
         lib.pa_pages_compact.argtypes = [tables, views, _i32, _vp, _vp]
         lib.pa_take_error_word.restype = ctypes.c_int
         lib.pa_take_error_word.argtypes = [_vp, _vp, _vp]
-        lib.pa_decode_workspace_bytes.restype = _sz
-        lib.pa_decode_workspace_bytes.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32, _i32]
+        for fn in (lib.pa_decode_workspace_bytes, lib.pa_decode_ext_workspace_bytes):
+            fn.restype = _sz
+            fn.argtypes = [_i32, _i32, _i32, _i32, _i32, _i32, _i32]
         lib.pa_workspace_init.restype = ctypes.c_int
         lib.pa_workspace_init.argtypes = [_vp, _sz, _vp]
         lib.pa_read_device_errors.restype = ctypes.c_int

@@ -290,6 +290,10 @@ size_t ws_partial_bytes(int nw_total, int slot_rows, int D) {
 
 }  // namespace pa
 
+static size_t f32_ext_workspace_bytes(int num_sms) {
+  return pa::kWsFixedBytes + pa::ws_counter_bytes(num_sms * pa::kDecodeWarps) + pa::f32_ext_partial_bytes(num_sms);
+}
+
 extern "C" {
 
 const char* pa_last_error(void) { return g_last_error; }
@@ -298,20 +302,29 @@ const char* pa_last_kernel(void) { return g_last_kernel; }
 
 int32_t pa_version(void) { return 1 * 10000 + 0 * 100 + 0; }
 
-size_t pa_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
-                                 int32_t q_len, int32_t head_dim, int32_t dtype, int32_t device) {
+static size_t decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t q_len,
+                                     int32_t head_dim, int32_t dtype, int32_t device, bool ext) {
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || q_len <= 0 || head_dim <= 0 ||
       num_q_heads % num_kv_heads != 0)
     return 0;
   DeviceInfo* info = nullptr;
   if (device_info(device, &info) != PA_OK) return 0;
   const DecodeShape s = decode_shape(num_q_heads, num_kv_heads, q_len);
-  if (dtype == PA_DTYPE_FLOAT32)  // what pa_decode_ext needs; pa_decode takes the header alone
-    return pa::kWsFixedBytes + pa::ws_counter_bytes(info->num_sms * pa::kDecodeWarps) +
-           pa::f32_ext_partial_bytes(info->num_sms);
+  if (dtype == PA_DTYPE_FLOAT32)  // plain decode does not split its rows
+    return ext ? f32_ext_workspace_bytes(info->num_sms) : pa::kWsHeaderBytes;
   const int DP = padded_head_dim(head_dim, dtype);
   if (DP == 0) return pa::kWsHeaderBytes;  // not served: pa_decode itself reports it
   return workspace_bytes_impl(s.slot_rows, DP, info->num_sms * pa::kDecodeWarps);
+}
+
+size_t pa_decode_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                 int32_t q_len, int32_t head_dim, int32_t dtype, int32_t device) {
+  return decode_workspace_bytes(batch, num_q_heads, num_kv_heads, q_len, head_dim, dtype, device, false);
+}
+
+size_t pa_decode_ext_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                     int32_t q_len, int32_t head_dim, int32_t dtype, int32_t device) {
+  return decode_workspace_bytes(batch, num_q_heads, num_kv_heads, q_len, head_dim, dtype, device, true);
 }
 
 int pa_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
@@ -653,7 +666,7 @@ static int decode_impl(const pa_decode_args* a, const pa_prefix_groups* grp, con
       return fail(PA_ERR_UNSUPPORTED, "cache base must be 4-byte aligned");
     if (sm != nullptr) {
       const int nw = info->num_sms * pa::kDecodeWarps;
-      const size_t need = pa::kWsFixedBytes + pa::ws_counter_bytes(nw) + pa::f32_ext_partial_bytes(info->num_sms);
+      const size_t need = f32_ext_workspace_bytes(info->num_sms);
       if (a->workspace_bytes < need)
         return fail(PA_ERR_WORKSPACE, "workspace too small: %zu bytes given, %zu needed", a->workspace_bytes, need);
       char* ws = static_cast<char*>(a->workspace);

@@ -224,7 +224,7 @@ PyObject* py_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
   }
   if (!eight && !scored) return none();
   const int include_new = PyObject_IsTrue(o[10]);
-  const size_t need = pa_decode_workspace_bytes(B, Hq, Hkv, q, D, code, dev.index());
+  const size_t need = pa_decode_ext_workspace_bytes(B, Hq, Hkv, q, D, code, dev.index());
   if (need == 0 || static_cast<size_t>(ws->numel()) < need || !on(*ws, dev)) return none();
   const at::Tensor *key = tensor(o[7]), *value = tensor(o[8]), *slots = tensor(o[6]);
   if ((o[7] != Py_None && !key) || (o[8] != Py_None && !value) || (o[6] != Py_None && !slots) ||

@@ -575,13 +575,14 @@ _ws_bytes_cache: dict[tuple, int] = {}
 _BATCH_LIMIT_TEXT = "too large for the decode kernel's shared memory"
 
 
-def _workspace_bytes(B: int, Hq: int, Hkv: int, q_len: int, D: int, dcode: int, dev_index: int) -> int:
-    key = (B, Hq, Hkv, q_len, D, dcode, dev_index)
+def _workspace_bytes(B: int, Hq: int, Hkv: int, q_len: int, D: int, dcode: int, dev_index: int, ext: bool) -> int:
+    key = (B, Hq, Hkv, q_len, D, dcode, dev_index, ext)
     n = _ws_bytes_cache.get(key)
     if n is None:
-        n = _lib.load().pa_decode_workspace_bytes(B, Hq, Hkv, q_len, D, dcode, dev_index)
+        name = "pa_decode_ext_workspace_bytes" if ext else "pa_decode_workspace_bytes"
+        n = getattr(_lib.load(), name)(B, Hq, Hkv, q_len, D, dcode, dev_index)
         if n == 0:
-            raise RuntimeError(f"pa_decode_workspace_bytes failed: {_lib.last_error()}")
+            raise RuntimeError(f"{name} failed: {_lib.last_error()}")
         _ws_bytes_cache[key] = n
     return n
 
@@ -822,7 +823,8 @@ def paged_attention_decode(
             raise ValueError("prefix_groups must describe this batch on the cache's device")
         need = _cascade_workspace_bytes(B, Hq, Hkv, q_len, D, dcode, device.index, prefix_groups)
     else:
-        need = _workspace_bytes(B, Hq, Hkv, q_len, D, dcode, device.index)
+        need = _workspace_bytes(B, Hq, Hkv, q_len, D, dcode, device.index,
+                                scales is not None or modifiers is not None)
     # The extended kernels report into the host word, unless the caller brings a
     # workspace to hold the errors of its own calls.
     host = host_word(device) if workspace is None and (scales is not None or modifiers is not None) else None

@@ -1,5 +1,5 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
-the pool, empty slots, error words read while other streams report."""
+the pool, empty slots, error words read while other streams report, workspaces."""
 
 from __future__ import annotations
 
@@ -11,6 +11,7 @@ from _ops64 import F8, Pages
 from llm_serving_runtime_b200 import (
     DevicePages,
     ScoreModifiers,
+    _lib,
     copy_pages,
     kv_append,
     paged_attention,
@@ -285,3 +286,50 @@ def test_errors_reported_while_others_are_read():
         seen |= word.take()
         assert seen == 0x41
     assert word.take() == 0
+
+
+@pytest.fixture
+def fresh_workspaces(monkeypatch):
+    """No workspace yet, as in a new process."""
+    for name, value in (("_workspaces", {}), ("_outgrown", [])):
+        monkeypatch.setattr(paged_attention, name, value)
+    yield paged_attention._workspaces
+    torch.cuda.synchronize()
+
+
+def _fp32_case(B=3):
+    g = torch.Generator().manual_seed(6)
+    kc, vc = (torch.randn(20, 2, 16, 64, generator=g).cuda() for _ in range(2))
+    query = torch.randn(B, 4, 1, 64, generator=g).cuda()
+    return query, kc, vc, torch.randint(0, 20, (B, 4), generator=g).int().cuda(), _i32([50, 3, 17][:B]), 0.125
+
+
+def test_plain_fp32_decode_asks_for_no_more_than_its_header(fresh_workspaces):
+    need = _lib.load().pa_decode_workspace_bytes(3, 4, 2, 1, 64, _lib.PA_DTYPE_FLOAT32, 0)
+    assert need == 256
+    args = _fp32_case()
+    paged_attention.decode_workspace(torch.device("cuda", 0))  # what any earlier call leaves
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # no eager call of this kind before
+        out = paged_attention_decode(*args)
+    graph.replay()
+    torch.cuda.synchronize()
+    ws = fresh_workspaces[0]
+    assert ws.numel() == 256
+    got = out.clone()
+    assert torch.equal(got, paged_attention_decode(*args, validate=True))
+    assert fresh_workspaces[0] is ws
+    # changed scores bring their own need
+    capped = paged_attention_decode(*args, score_modifiers=ScoreModifiers(softcap=1e4), validate=True)
+    assert fresh_workspaces[0].numel() > 256
+    assert float((capped - got).abs().max()) < 1e-3
+    for _ in range(2):  # the short way finds a workspace that fits
+        assert torch.equal(capped, paged_attention_decode(*args, score_modifiers=ScoreModifiers(softcap=1e4)))
+
+
+def test_a_workspace_of_the_plain_size_is_refused_for_changed_fp32_scores():
+    args = _fp32_case()
+    with pytest.raises(RuntimeError, match="workspace too small"):
+        paged_attention_decode(*args, score_modifiers=ScoreModifiers(window=3),
+                               workspace=torch.zeros(256, dtype=torch.uint8, device="cuda"))
