@@ -11,6 +11,7 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -64,6 +65,8 @@ bool tables_ok(const at::Tensor& t, int64_t B, c10::Device dev) {
 }
 
 bool is_current(c10::Device dev) { return c10::cuda::current_device() == dev.index(); }
+
+bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
 
 void* stream_of(c10::Device dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 
@@ -153,7 +156,8 @@ PyObject* py_append8(PyObject*, PyObject* const* o, Py_ssize_t n) {
 
 // decode(query, key_cache, value_cache, tables, lens, scale, slots, key, value, out, include_new, key_scales,
 //        value_scales, modifiers, workspace, word, weights, n_weights) -> out | None
-// modifiers: None or (softcap, window, alibi_slopes, key_starts, prefix_lens)
+// modifiers: None or (softcap, window, alibi_slopes, key_starts, prefix_lens).  A call that is being captured
+// goes the long way, which notes that a graph holds the workspace.
 PyObject* py_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
   if (n != 18) return none();
   const at::Tensor *pq = tensor(o[0]), *pk = tensor(o[1]), *pv = tensor(o[2]), *pt = tensor(o[3]), *pl = tensor(o[4]);
@@ -169,7 +173,7 @@ PyObject* py_decode(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const int64_t Hkv = kc.size(1);
   const int code = dtype_code(query.scalar_type());
   if (B <= 0 || q <= 0 || code < 0 || D != kc.size(3) || !on(query, dev) || query.stride(3) != 1 || Hkv <= 0 ||
-      Hq % Hkv != 0 || !tables_ok(tables, B, dev) || !int32_vector(lens, B, dev) || !is_current(dev))
+      Hq % Hkv != 0 || !tables_ok(tables, B, dev) || !int32_vector(lens, B, dev) || !is_current(dev) || capturing())
     return none();
   const double scale = PyFloat_AsDouble(o[5]);
   if (scale == -1.0 && PyErr_Occurred()) {

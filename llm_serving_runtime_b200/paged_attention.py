@@ -142,7 +142,9 @@ _host = _Host()
 # One workspace per device: status word + merge counters + partial slots.
 _ws_lock = threading.Lock()
 _workspaces: dict[int, torch.Tensor] = {}
-# Workspaces that a larger one replaced: captured graphs may still write to them.
+# Devices whose workspace a captured graph writes to, and the workspaces of such graphs
+# that a larger one replaced.
+_captured: set[int] = set()
 _outgrown: list[torch.Tensor] = []
 
 
@@ -157,22 +159,31 @@ def decode_workspace(device: torch.device, nbytes: int = 256) -> torch.Tensor:
 
     Growing allocates, which a CUDA-graph capture forbids: size it with one
     eager call before capture.  Calls that overlap on the GPU (different streams)
-    must not share a workspace — pass ``workspace=`` explicitly there.
+    must not share a workspace — pass ``workspace=`` explicitly there.  A workspace
+    that was asked for during a capture is kept when a larger one replaces it, for
+    the graph's sake.
     """
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    capturing = torch.cuda.is_current_stream_capturing()
     with _ws_lock:
         ws = _workspaces.get(idx)
         if ws is None or ws.numel() < nbytes:
-            if torch.cuda.is_current_stream_capturing():
+            if capturing:
                 raise RuntimeError(
                     "paged decode workspace must be sized before CUDA-graph capture: "
                     "run the same call once eagerly first"
                 )
-            if ws is not None:
+            if ws is not None and idx in _captured:
                 _outgrown.append(ws)
+                _captured.discard(idx)
                 nbytes = max(int(nbytes), 2 * ws.numel())  # what is kept stays below what is used
+            elif ws is not None:
+                # its last call is ordered before this one's, whichever stream that was on
+                ws.record_stream(torch.cuda.current_stream(ws.device))
             ws = torch.zeros(max(int(nbytes), 256), dtype=torch.uint8, device=torch.device("cuda", idx))
             _workspaces[idx] = ws
+        if capturing:
+            _captured.add(idx)
         return ws
 
 

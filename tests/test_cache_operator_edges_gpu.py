@@ -291,7 +291,7 @@ def test_errors_reported_while_others_are_read():
 @pytest.fixture
 def fresh_workspaces(monkeypatch):
     """No workspace yet, as in a new process."""
-    for name, value in (("_workspaces", {}), ("_outgrown", [])):
+    for name, value in (("_workspaces", {}), ("_outgrown", []), ("_captured", set())):
         monkeypatch.setattr(paged_attention, name, value)
     yield paged_attention._workspaces
     torch.cuda.synchronize()
@@ -333,3 +333,44 @@ def test_a_workspace_of_the_plain_size_is_refused_for_changed_fp32_scores():
     with pytest.raises(RuntimeError, match="workspace too small"):
         paged_attention_decode(*args, score_modifiers=ScoreModifiers(window=3),
                                workspace=torch.zeros(256, dtype=torch.uint8, device="cuda"))
+
+
+def test_an_outgrown_workspace_is_kept_for_captured_graphs_alone(fresh_workspaces):
+    dev = torch.device("cuda", 0)
+    first = paged_attention.decode_workspace(dev, 1000)
+    second = paged_attention.decode_workspace(dev, 5000)
+    third = paged_attention.decode_workspace(dev, 6000)
+    assert (first.numel(), second.numel(), third.numel()) == (1000, 5000, 6000)
+    assert not paged_attention._outgrown
+    assert paged_attention.decode_workspace(dev, 100) is third
+    graph, args = torch.cuda.CUDAGraph(), _fp32_case()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = paged_attention_decode(*args)
+    fourth = paged_attention.decode_workspace(dev, 7000)
+    assert [w.data_ptr() for w in paged_attention._outgrown] == [third.data_ptr()]
+    assert fourth.numel() >= 12000  # what is kept stays below what is used
+    fifth = paged_attention.decode_workspace(dev, fourth.numel() + 1)
+    assert len(paged_attention._outgrown) == 1 and fifth.numel() == fourth.numel() + 1
+    graph.replay()
+    assert torch.equal(out, paged_attention_decode(*args, validate=True))
+
+
+@pytest.mark.parametrize("short", [True, False])
+def test_a_graph_of_an_extended_call_keeps_its_workspace(fresh_workspaces, monkeypatch, short):
+    """Captured in one extension call or through the checks: growing the workspace later
+    takes nothing from the graph."""
+    if not short:
+        monkeypatch.setattr(paged_attention, "_VALIDATE_DEFAULT", True)
+    args, mods = _fp32_case(), ScoreModifiers(softcap=3.0)
+    for _ in range(2):
+        want = paged_attention_decode(*args, score_modifiers=mods)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged_attention_decode(*args, score_modifiers=mods)
+    ws = fresh_workspaces[0]
+    paged_attention.decode_workspace(ws.device, 3 * ws.numel())
+    assert [w.data_ptr() for w in paged_attention._outgrown] == [ws.data_ptr()]
+    graph.replay()
+    assert torch.equal(out, want)
