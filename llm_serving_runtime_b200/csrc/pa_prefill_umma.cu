@@ -44,9 +44,12 @@
 // (a cap costs two more instructions of the exponential's unit a score).  A
 // V row that is not finite would reach rows that do not see it through their zero
 // weights (0 * inf), and 128 rows share one MMA: chunks that some row sees only in
-// part are looked over, and a CTA that finds such a row computes its own rows anew
-// on CUDA cores, key by key.  4 x 1021 tokens of packed documents of 700 (32/8 heads of
-// 128, 22.6 GFLOP of visible scores): 100 us, 199 on the mma.sync kernel.  Of a CTA's
+// part are looked over, such V rows zeroed for the products, and what they give
+// the rows that see them added on CUDA cores at the end (add_odd_values): 8 x 512
+// tokens on 32,768 cached ones 5.66 ms with and without one infinite value among the
+// new tokens; where rows of two documents alternate, so that all chunks are looked over
+// again, 7.8 ms without, 8.7 with one, 8.9 with 64 and 19.5 with 4096.  4 x 1021 tokens
+// of packed documents of 700 (32/8 heads of 128, 22.6 GFLOP of visible scores): 100 us, 199 on the mma.sync kernel.  Of a CTA's
 // 22 us 11 are its 6.8 chunks (1.6 us a chunk, as without scores) and 9 what it pays
 // once: key ranges 1.0, queries 2.5, first scores 1.0, output 2.7, the next CTA's start
 // 1.2.  Loading the queries before the key ranges took longer (101.5: the fences
@@ -174,46 +177,112 @@ __device__ __forceinline__ void split_bf16_pair(float p0, float p1, uint32_t& hi
   lo = __byte_perm(__float_as_uint(r0), __float_as_uint(r1), 0x7632);
 }
 
-// A CTA's rows once more, key by key, a row a warp at a time: the rare case that
-// a V row some row must not see is not finite.  Query row qr of KV head h of
-// sequence b; lanes span the columns.
-template <typename T>
-__device__ __forceinline__ void attend_row_plain(const DecodeParams& p, int b, int h, int L, int qr, int lane) {
-  const int t = qr / p.G, g = qr - t * p.G;
-  const T* qrow = static_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)(h * p.G + g) * p.q_sh +
-                  (long long)t * p.q_st;
-  T* orow = static_cast<T*>(p.out) + (long long)b * p.o_sb + (long long)(h * p.G + g) * p.o_sh + (long long)t * p.o_st;
-  const KeyRange kr = row_keys<true>(p, b, L, t);
-  const float slope = p.alibi_slopes != nullptr ? p.alibi_slopes[h * p.G + g] * 1.4426950408889634f : 0.f;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+// Adds to a warp's rows of O (at t_o in tensor memory) what V rows that are not finite
+// give them, and stores the rows that got something: in chunks that some row of the CTA
+// sees only in part such V rows were zeroed for the products, and here each is found
+// again, its weights worked out on CUDA cores and added for the rows that see it, in the
+// order of the keys.  on: the thread's row exists, and is not NaN already (its sum is, when
+// a key that it sees is).  lo .. hi: keys that some row of the CTA sees from kv_lo, the
+// first chunk's start, on; [full_lo, full_hi): keys that all rows see.
+template <typename T, int D>
+__device__ __forceinline__ void add_odd_values(const DecodeParams& p, uint32_t t_o, const T* qrow, T* orow, int b,
+                                               int h, int pos, KeyRange kr, float slope, bool on, float m_ref,
+                                               float inv, int kv_lo, int lo, int hi, int full_lo, int full_hi,
+                                               int lane) {
+  const float nbase = m_ref == -INFINITY ? 0.f : -m_ref;
+  const int from = __reduce_min_sync(0xffffffffu, on ? kr.first : INT_MAX);
+  const int to = __reduce_max_sync(0xffffffffu, on ? kr.end : 0);
+  if (from >= to) return;
+  const T* kc = static_cast<const T*>(p.k_cache) + h * p.k_sh;
+  const T* vc = static_cast<const T*>(p.v_cache) + h * p.v_sh;
+  bool changed = false;
+#pragma unroll 1
+  for (int c0 = kv_lo + (max(from, kv_lo) - kv_lo) / kChunk * kChunk; c0 < to; c0 += kChunk) {
+    if (c0 >= full_lo && c0 + kChunk <= full_hi) continue;
+#pragma unroll 1
+    for (int k0 = c0; k0 < c0 + kChunk; k0 += 32) {
+      int phys = -1;  // lane: key k0 + lane
+      bool odd = false;
+      if (k0 + lane >= lo && k0 + lane < hi) {
+        phys = p.block_tables[(long long)b * p.bt_stride + (k0 + lane) / p.bs];
+        if (phys >= 0 && phys < p.num_blocks) {
+          const T* vrow = vc + phys * p.v_sblk + ((k0 + lane) % p.bs) * p.v_st;
+          for (int d = 0; d < p.Dv; d += 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(vrow + d);
+            odd |= not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w);
+          }
+        }
+      }
+#pragma unroll 1
+      for (uint32_t left = __ballot_sync(0xffffffffu, odd); left != 0u; left &= left - 1) {
+        const int at = __ffs(left) - 1, j = k0 + at;
+        const long long blk = __shfl_sync(0xffffffffu, phys, at);
+        const bool sees = on && j >= kr.first && j < kr.end;
+        if (!__any_sync(0xffffffffu, sees)) continue;
+        float w = 0.f;
+        if (sees) {
+          const T* krow = kc + blk * p.k_sblk + (j % p.bs) * p.k_st;
+          float x = 0.f;
+#pragma unroll 1
+          for (int d = 0; d < p.Dv; d += 8) {
+            const uint4 a = *reinterpret_cast<const uint4*>(qrow + d), k = *reinterpret_cast<const uint4*>(krow + d);
+            x = fmaf(lo_half<T>(a.x), lo_half<T>(k.x), fmaf(hi_half<T>(a.x), hi_half<T>(k.x), x));
+            x = fmaf(lo_half<T>(a.y), lo_half<T>(k.y), fmaf(hi_half<T>(a.y), hi_half<T>(k.y), x));
+            x = fmaf(lo_half<T>(a.z), lo_half<T>(k.z), fmaf(hi_half<T>(a.z), hi_half<T>(k.z), x));
+            x = fmaf(lo_half<T>(a.w), lo_half<T>(k.w), fmaf(hi_half<T>(a.w), hi_half<T>(k.w), x));
+          }
+          x *= p.scale_log2;
+          if (p.softcap_log2 > 0.f)
+            x = p.softcap <= kDirectCap ? softcap_direct(x, p.softcap_log2, p.inv_softcap_log2)
+                                        : softcap_log2(x, p.softcap_log2, p.inv_softcap_log2);
+          x = fmaf(-slope, fabsf((float)(pos - j)), x);
+          w = ex2(x + nbase);
+          changed = true;
+        }
+        const T* vrow = vc + blk * p.v_sblk + (j % p.bs) * p.v_st;
+#pragma unroll 1
+        for (int col = 0; col < D; col += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld32(t_o + col, o);
+          tmem_wait_ld();
 #pragma unroll
-  for (int k = 0; k < 4; ++k) q[k] = lane + 32 * k < p.Dv ? (float)qrow[lane + 32 * k] : 0.f;
-  for (int j = kr.first; j < kr.end; ++j) {
-    const int phys = p.block_tables[(long long)b * p.bt_stride + j / p.bs];
-    if (phys < 0 || phys >= p.num_blocks) continue;  // flagged by the producer
-    const T* krow = static_cast<const T*>(p.k_cache) + phys * p.k_sblk + h * p.k_sh + (j % p.bs) * p.k_st;
-    const T* vrow = static_cast<const T*>(p.v_cache) + phys * p.v_sblk + h * p.v_sh + (j % p.bs) * p.v_st;
-    float x = 0.f;
+          for (int i = 0; i < 32; i += 8) {
+            if (!sees || col + i >= p.Dv) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(vrow + col + i);
+            const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 32 * k < p.Dv) x = fmaf(q[k], (float)krow[lane + 32 * k], x);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) x += __shfl_xor_sync(0xffffffffu, x, s);
-    x *= p.scale_log2;
-    if (p.softcap_log2 > 0.f) x = softcap_log2(x, p.softcap_log2, p.inv_softcap_log2);
-    x = fmaf(-slope, fabsf((float)(L - p.q_len + t - j)), x);
-    const float mn = fmaxf(m, x), base = mn == -INFINITY ? 0.f : mn;
-    const float a = ex2(m - base), w = ex2(x - base);
-    l = fmaf(l, a, w);
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (lane + 32 * k < p.Dv) o[k] = fmaf(w, (float)vrow[lane + 32 * k], o[k] * a);
-    m = mn;
+            for (int e = 0; e < 4; ++e) {
+              o[i + 2 * e] = __float_as_uint(fmaf(w, lo_half<T>(vw[e]), __uint_as_float(o[i + 2 * e])));
+              o[i + 2 * e + 1] = __float_as_uint(fmaf(w, hi_half<T>(vw[e]), __uint_as_float(o[i + 2 * e + 1])));
+            }
+          }
+          __syncwarp();
+          tmem_st32(t_o + col, o);
+        }
+        tmem_wait_st();
+      }
+    }
   }
-  const float inv = row_norm<T>(l, kr.first < kr.end);
+  if (!__any_sync(0xffffffffu, changed)) return;
+#pragma unroll 1
+  for (int col = 0; col < D; col += 32) {
+    uint32_t o[32];
+    __syncwarp();
+    tmem_ld32(t_o + col, o);
+    tmem_wait_ld();
+    if (!changed) continue;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 32 * k < p.Dv) orow[lane + 32 * k] = from_float<T>(o[k] * inv);
+    for (int i = 0; i < 32; i += 8) {
+      if (col + i >= p.Dv) break;
+      uint4 v;
+      v.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+      v.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+      v.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+      v.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+      *reinterpret_cast<uint4*>(orow + col + i) = v;
+    }
+  }
 }
 
 // Byte offset of 16-byte chunk `c` of row `r` in a 128-byte-swizzled region.
@@ -253,7 +322,7 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(q_ready + 1);
   __shared__ int s_last;
   // Changed scores: keys that some / every row of the CTA sees, and whether a V row
-  // that is not finite turned up among keys some row does not see.
+  // that is not finite turned up in a chunk that some row does not see whole.
   __shared__ int s_lo, s_hi, s_full_lo, s_full_hi, s_odd;
 
   const int tid = threadIdx.x;
@@ -753,7 +822,8 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
         // (The chunk's own barrier has completed; waiting on it here makes the
         // copied bytes visible to this thread.)
         if (t == 0 && (tok0 < s_full_lo || tok0 + kChunk > s_full_hi)) {
-          if (!mbar_test_then_wait(smem_addr(&kv_full[j % S]), (uint32_t)((j / S) & 1))) {
+          const bool landed = mbar_test_then_wait(smem_addr(&kv_full[j % S]), (uint32_t)((j / S) & 1));
+          if (!__all_sync(0xffffffffu, landed)) {
             ok = false;
             break;
           }
@@ -761,15 +831,23 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
           const int row = r >> 1, tok = tok0 + row;
           const bool seen = tok >= s_lo && tok < kv_end;
           bool odd = false;
+          auto piece = [&](int hf, int c) -> uint4* {
+            return reinterpret_cast<uint4*>(vbase + hf * HALF_BYTES + row * 128 + (r & 1) * 64 + c * 16);
+          };
 #pragma unroll
           for (int hf = 0; hf < HALVES; ++hf)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(vbase + hf * HALF_BYTES + row * 128 + (r & 1) * 64 + c * 16);
-              const uint4 v = *at;
+              const uint4 v = *piece(hf, c);
               odd |= not_finite2<T>(v.x) | not_finite2<T>(v.y) | not_finite2<T>(v.z) | not_finite2<T>(v.w);
-              if (!seen) *at = make_uint4(0u, 0u, 0u, 0u);
             }
+          odd |= __shfl_xor_sync(0xffffffffu, (int)odd, 1) != 0;  // in the other half
+          if (!seen || odd) {
+#pragma unroll
+            for (int hf = 0; hf < HALVES; ++hf)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) *piece(hf, c) = make_uint4(0u, 0u, 0u, 0u);
+          }
           if (odd && seen) s_odd = 1;
           fence_proxy_async_smem();
         }
@@ -978,10 +1056,12 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       }
       if constexpr (kScored) {
         asm volatile("bar.sync 1, 256;" ::: "memory");  // the eight softmax warps
-        if (*reinterpret_cast<volatile int*>(&s_odd) != 0) {
-          const int L = min(max(p.context_lens[b_kv] + p.len_offset, 0), cap);
-          const int first = row0 + warp * 32, last = min(first + 32, rows_total);
-          for (int i = first; i < last; ++i) attend_row_plain<T>(p, b_kv, h, L, i, lane);
+        if (tile_on && *reinterpret_cast<volatile int*>(&s_odd) != 0 && __all_sync(0xffffffffu, ok)) {
+          const T* qrow = static_cast<const T*>(p.q) + (long long)b * p.q_sb + (long long)(h * p.G + g) * p.q_sh +
+                          (long long)tq * p.q_st;
+          add_odd_values<T, D>(p, t_o, qrow, orow, b, h, lim, kr, slope,
+                               row_ok && l == l && kr.first < kr.end, m_ref, inv, kv_lo, s_lo, kv_end,
+                               s_full_lo, s_full_hi, lane);
         }
       }
     }

@@ -1,5 +1,6 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
-the pool, empty slots, error words read while other streams report, workspaces."""
+the pool, empty slots, error words read while other streams report, workspaces,
+values that are not finite."""
 
 from __future__ import annotations
 
@@ -7,7 +8,7 @@ import numpy as np
 import pytest
 import torch
 
-from _ops64 import F8, Pages
+from _ops64 import F8, Pages, attend64, check
 from llm_serving_runtime_b200 import (
     DevicePages,
     ScoreModifiers,
@@ -374,3 +375,92 @@ def test_a_graph_of_an_extended_call_keeps_its_workspace(fresh_workspaces, monke
     assert [w.data_ptr() for w in paged_attention._outgrown] == [ws.data_ptr()]
     graph.replay()
     assert torch.equal(out, want)
+
+
+def _chunk_case(dtype, B, q, L, Hkv, G, D, bs, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = (L + q + bs - 1) // bs
+    nb = B * n
+    tables = torch.randperm(nb, generator=g).int().reshape(B, n)
+    kc, vc = (torch.randn(nb, Hkv, bs, D, generator=g).to(dtype).cuda() for _ in range(2))
+    query = torch.randn(B, Hkv * G, q, D, generator=g).to(dtype).cuda()
+    return query, kc, vc, tables, torch.full((B,), L, dtype=torch.int32)
+
+
+def _put(cache, tables, bs, b, pos, col, value):
+    cache[int(tables[b, pos // bs]), :, pos % bs, col] = value
+
+
+@pytest.mark.parametrize("dtype,D,bs", [(BF, 64, 16), (BF, 128, 8), (HF, 128, 64), (HF, 72, 16)])
+@pytest.mark.parametrize("kind", ["causal", "window", "documents", "prefix"])
+def test_values_that_are_not_finite_reach_the_rows_that_see_them(dtype, D, bs, kind):
+    """Prefill chunks on the tcgen05 kernel: infinities and NaN among values that some of a
+    tile's rows see and others do not, from one of them to every key of a sequence.  They
+    stand in one column each, so the others show that nothing else changes."""
+    B, q, L, Hkv, G = 19, 40, 100, 8, 2
+    query, kc, vc, tables, lens = _chunk_case(dtype, B, q, L, Hkv, G, D, bs, 41)
+    rng = np.random.default_rng(3)
+    some = [float("inf"), -float("inf"), float("nan")]
+    new = np.arange(L, L + q)
+    seen_in_part = {"causal": new, "window": np.concatenate([np.arange(L - 50, L - 10), new]),
+                    "documents": np.arange(L + q), "prefix": np.arange(L + 8, L + q)}[kind]
+    for b in range(B):
+        n = [0, 1, 2, 7, 40][b % 5]
+        if b == 4:
+            where = seen_in_part
+        else:
+            where = rng.permutation(seen_in_part)[:n]
+        for pos in where:
+            _put(vc, tables, bs, b, int(pos), int(rng.integers(0, D)), some[int(rng.integers(0, 3))])
+    for pos in (L + 3, L + 20):  # a key of its own that is not finite: its rows are NaN
+        _put(kc, tables, bs, 7, pos, 1, float("nan"))
+        _put(vc, tables, bs, 7, pos, 2, float("inf"))
+    args = {"softcap": 20.0}
+    if kind == "window":
+        args["window"] = 50
+    elif kind == "documents":
+        pos = torch.arange(L, L + q)[None].repeat(B, 1)
+        args["key_starts"] = (pos // 9 * 9 - (pos % 9 == 0) * 60).clamp_min(0).int().cuda()
+    elif kind == "prefix":
+        args["prefix_lens"] = torch.full((B,), L + 8, dtype=torch.int32, device="cuda")
+    mods = ScoreModifiers(alibi_slopes=torch.linspace(0, 0.2, Hkv * G).cuda(), **args)
+    out = paged_attention_decode(query, kc, vc, tables.cuda(), lens.cuda(), 0.1, score_modifiers=mods, validate=True)
+    assert _lib.last_kernel() == "pa::prefill_umma_kernel<scored>"
+    ref, bar = attend64(query, kc, vc, tables, lens, 0.1, alibi_slopes=mods.alibi_slopes, **args)
+    assert bool(torch.isnan(ref).any()) and bool(torch.isinf(ref).any())
+    o = out.double().cpu()
+    assert torch.equal(torch.isinf(o) * o.sign().nan_to_num(), torch.isinf(ref) * ref.sign().nan_to_num())
+    assert torch.equal(torch.isnan(o), torch.isnan(ref))
+    fine = torch.isfinite(ref)
+    check(o.where(fine, 0.0), ref.where(fine, 0.0), bar.where(fine, 0.0))
+    for _ in range(3):
+        again = paged_attention_decode(query, kc, vc, tables.cuda(), lens.cuda(), 0.1, score_modifiers=mods)
+        assert torch.equal(out.view(torch.int16), again.view(torch.int16))
+
+
+def test_one_value_that_is_not_finite_costs_little():
+    """A call over long cached contexts takes about as long with an infinite value among
+    its new tokens as without (a hundred times as long when the rows of its tile are
+    worked out anew)."""
+    B, q, L, bs = 8, 256, 8192, 16
+    n = (L + q + bs - 1) // bs
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kc, vc = (torch.randn(B * n, 8, bs, 128, generator=g, device="cuda").to(BF) for _ in range(2))
+    query = torch.randn(B, 32, q, 128, generator=g, device="cuda").to(BF)
+    tables = torch.arange(B * n, dtype=torch.int32, device="cuda").reshape(B, n)
+    lens, mods = _i32([L] * B), ScoreModifiers(softcap=50.0)
+
+    def best():
+        took = []
+        for _ in range(5):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            paged_attention_decode(query, kc, vc, tables, lens, 0.09, score_modifiers=mods)
+            b.record()
+            b.synchronize()
+            took.append(a.elapsed_time(b))
+        return min(took)
+
+    clean = best()
+    vc[int(tables[0, (L + 100) // bs]), :, (L + 100) % bs, 3] = float("inf")
+    assert best() < 5 * clean
