@@ -889,8 +889,9 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       // Both are free once this tile's last P.V has completed: its commit
       // tracks every MMA issued before it, and tile 1's last P.V is the last
       // MMA.  Without a clean finish (a wait ran out, copies may still be in
-      // flight) the rows go out one per thread.
-      const bool staged = tile_on && __all_sync(0xffffffffu, ok) && __any_sync(0xffffffffu, row_ok);
+      // flight), or without chunks (nothing waited for the other warps' query
+      // rows, which lie in the same space), the rows go out one per thread.
+      const bool staged = n_chunks > 0 && tile_on && __all_sync(0xffffffffu, ok) && __any_sync(0xffffffffu, row_ok);
       if (staged) {
         constexpr int CHF = D / 4;  // 16-byte pieces per fp32 row
         uint8_t* sw = (t == 0 ? s_q : s_kv) + (warp & 3) * (32 * D * 4);
@@ -990,9 +991,10 @@ __global__ void __launch_bounds__(umma_threads(kPrefix), 1)
       float inv = (ok && l > 0.f) ? 1.f / l : 0.f;
       if constexpr (kScored) inv = ok ? row_norm<T>(l, kr.first < kr.end) : 0.f;
       // As in the prefix epilogue: the warp's rows go out through shared
-      // memory (this tile's Q tile, free once its last P.V has completed),
+      // memory (this tile's Q tile, free once its last P.V has completed; without
+      // chunks other warps may still be writing their query rows into it),
       // whole rows per store instruction.
-      const bool staged = tile_on && __all_sync(0xffffffffu, ok) && __any_sync(0xffffffffu, row_ok);
+      const bool staged = n_chunks > 0 && tile_on && __all_sync(0xffffffffu, ok) && __any_sync(0xffffffffu, row_ok);
       if (staged) {
         constexpr int CHB = D / 8;  // 16-byte pieces per output row
         uint8_t* sw = s_q + t * QT_BYTES + (warp & 3) * (32 * D * 2);

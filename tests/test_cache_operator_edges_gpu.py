@@ -1,6 +1,6 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
 the pool, empty slots, error words read while other streams report, workspaces,
-values that are not finite."""
+values that are not finite, rows without keys."""
 
 from __future__ import annotations
 
@@ -464,3 +464,30 @@ def test_one_value_that_is_not_finite_costs_little():
     clean = best()
     vc[int(tables[0, (L + 100) // bs]), :, (L + 100) % bs, 3] = float("inf")
     assert best() < 5 * clean
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 72, 128])
+@pytest.mark.parametrize("scored", [True, False])
+def test_rows_without_keys_are_zero_on_the_multi_query_kernel(scored, D, dtype):
+    """Sequences of length 0 and tokens before a sequence's start, whole tiles of them: zeros,
+    not what a tile's queries left where its rows are stored from."""
+    B, q, Hkv, G, bs = 40, 64, 4, 8, 16
+    g = torch.Generator().manual_seed(43)
+    nb = 200
+    kc, vc = (torch.randn(nb, Hkv, bs, D, generator=g).to(dtype).cuda() for _ in range(2))
+    tables = torch.randint(0, nb, (B, 8), generator=g).int().cuda()
+    query = torch.randn(B, Hkv * G, q, D, generator=g).to(dtype).cuda()
+    lens = torch.tensor([[0, 20, -3, 64, 100, 1, 33, 0][b % 8] for b in range(B)])
+    kw = {"score_modifiers": ScoreModifiers(softcap=30.0)} if scored else {}
+    want = None
+    for _ in range(20):
+        out = paged_attention_decode(query, kc, vc, tables, _i32(lens.tolist()), 0.1, context_lens_include_new=True,
+                                     validate=True, **kw)
+        assert _lib.last_kernel() == "pa::prefill_umma_kernel" + ("<scored>" if scored else "")
+        for b, n in enumerate(lens.tolist()):
+            empty = q - min(max(n, 0), q)  # tokens before the start
+            assert not bool(out[b, :, :empty].any()), b
+            assert n <= 0 or bool((out[b, :, empty:] != 0).any())
+        want = out if want is None else want
+        assert torch.equal(out, want)
