@@ -23,8 +23,11 @@
 // so a block of large scale and little weight cannot push the others' weights
 // out of fp16's range, and one exponential serves both sums.  w is rounded to
 // fp16 for the product (at most 2^-11 of each weight; normal down to 2^-28 of the
-// largest, nothing below 2^-39 of it), the norm takes it unrounded.  Scales other than 0 are taken to be at
-// least 2^-100 (the append writes no smaller ones).
+// largest, nothing below 2^-39 of it), the norm takes it unrounded.  The norm's fp32 range
+// holds as long as the V scales of a row's blocks lie within 2^100 of one another.  Scales
+// up to 2^-100, the least that the append writes (a block of zeros), would not beside
+// values above 3e10: such blocks' values count as 0 (they are below 4e-28), and their
+// weights go into the norm by way of a scale of 2^-40.
 //
 // What a mask hides never reaches a row: hidden scores are -inf whatever K
 // holds, and in units where rows see different keys (or none), V rows that are not
@@ -547,11 +550,11 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
   // ---- online softmax, weighted by the V scales ----
   // (a comparison that NaN fails keeps a NaN scale's NaN)
   float lvs[4], ivs[4];
-  constexpr float kLeast = 7.8886090522101181e-31f;  // 2^-100
+  constexpr float kZeros = 7.8886090522101181e-31f;  // 2^-100
 #pragma unroll
   for (int n = 0; n < 4; ++n) {
-    lvs[n] = vs[n] < kLeast ? -100.f : lg2(vs[n]);
-    ivs[n] = (vs[n] < kLeast ? 1.2676506002282294e30f : rcp_approx(vs[n])) * 6.103515625e-05f;  // 2^-14 / vs
+    lvs[n] = vs[n] <= kZeros ? -40.f : lg2(vs[n]);
+    ivs[n] = (vs[n] <= kZeros ? 1.099511627776e12f : rcp_approx(vs[n])) * 6.103515625e-05f;  // 2^-14 / vs
   }
   float alpha[2], w[2][8];
 #pragma unroll
@@ -613,8 +616,9 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
         const bool second = c & 1, g1 = t & 8, g2 = t & 16;
         const float p0 = second ? w[r][1] : w[r][0], p1 = second ? w[r][3] : w[r][2];
         const float p2 = second ? w[r][5] : w[r][4], p3 = second ? w[r][7] : w[r][6];
-        const float wt = __shfl_sync(0xffffffffu, g2 ? (g1 ? p3 : p2) : (g1 ? p1 : p0), src);
+        float wt = __shfl_sync(0xffffffffu, g2 ? (g1 ? p3 : p2) : (g1 ? p1 : p0), src);
         if (tok_base + t < st.first[r] || tok_base + t >= st.end[r]) continue;
+        if ((g2 ? (g1 ? vs[3] : vs[2]) : (g1 ? vs[1] : vs[0])) <= kZeros) wt = 0.f;
 #pragma unroll
         for (int nd = 0; nd < NDT; ++nd)
 #pragma unroll
@@ -648,10 +652,10 @@ __device__ __forceinline__ void attend_unit_8(uint32_t kbase, uint32_t vbase, co
     pa[h][2] = pack2<__half>(w[0][4 * h + 2], w[0][4 * h + 3]);
     pa[h][3] = pack2<__half>(w[1][4 * h + 2], w[1][4 * h + 3]);
   }
-  if (fminf(fminf(vs[0], vs[1]), fminf(vs[2], vs[3])) == 0.f) {  // a zero scale: values of 0
+  if (fminf(fminf(vs[0], vs[1]), fminf(vs[2], vs[3])) <= kZeros) {  // blocks of zeros
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      if (vs[n] == 0.f) pa[n >> 1][2 * (n & 1)] = pa[n >> 1][2 * (n & 1) + 1] = 0u;
+      if (vs[n] <= kZeros) pa[n >> 1][2 * (n & 1)] = pa[n >> 1][2 * (n & 1) + 1] = 0u;
   }
   const uint32_t vat = tile_chunk_addr<e4m3_t, D>(vbase, v_row_8(lane & 15), lane >> 4);
   auto pv = [&](auto masked) {

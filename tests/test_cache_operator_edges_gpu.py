@@ -1,6 +1,6 @@
 """Edges of the operators over a paged cache: padding pairs among forks, block ids outside
 the pool, empty slots, error words read while other streams report, workspaces,
-values that are not finite, rows without keys."""
+values that are not finite, rows without keys, blocks of zeros."""
 
 from __future__ import annotations
 
@@ -491,3 +491,42 @@ def test_rows_without_keys_are_zero_on_the_multi_query_kernel(scored, D, dtype):
             assert n <= 0 or bool((out[b, :, empty:] != 0).any())
         want = out if want is None else want
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("B,q,L,M,kernel", [(2, 1, 300, 20, "pa::decode_direct_kernel<few>"),
+                                            (1, 5, 5000, 400, "pa::decode_direct_kernel<few>"),
+                                            (40, 1, 300, 20, "pa::decode_direct_kernel<many>"),
+                                            (40, 1, 300, 300, "pa::decode_mma_kernel<ext>"),
+                                            (20, 40, 200, 20, "pa::prefill_mma_kernel<ext>")])
+@pytest.mark.parametrize("scored", [True, False])
+def test_blocks_of_zeros_beside_huge_values(scored, B, q, L, M, kernel):
+    """A block of zeros (a scale of 0, or the append's least, 2^-100) has its weight in the
+    norm beside blocks of any scale up to 2^60, in whichever order they come."""
+    Hkv, G, D, bs = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(44)
+    per = (L + q + bs - 1) // bs
+    nb = B * per
+    tables = torch.zeros(B, M, dtype=torch.int32)
+    tables[:, :per] = torch.arange(nb).reshape(B, per)
+    kc, vc = ((torch.randn(nb, Hkv, bs, D, generator=g) * 100).clamp(-448, 448).to(F8) for _ in range(2))
+    ks = torch.exp2(torch.randint(-9, -6, (nb, Hkv), generator=g).float())
+    vs = torch.exp2(torch.randint(-9, -6, (nb, Hkv), generator=g).float())
+    kind = torch.randint(0, 6, (nb, Hkv), generator=g)
+    vs[kind == 1] = 0
+    vs[kind == 2] = 2.0**-100
+    vs[kind == 3] = 2.0 ** float([32, 45, 60][B % 3])
+    vs[:per:2] = 0  # a row of whole zeros up to its end
+    vs[per - 1] = 2.0**33
+    kind[1::7] = 2  # its codes are 0 as well
+    vs[1::7] = 2.0**-100
+    vc.view(torch.uint8)[1::7] = 0
+    query = torch.randn(B, Hkv * G, q, D, generator=g).to(BF).cuda()
+    lens = torch.full((B,), L, dtype=torch.int32)
+    state = [t.cuda() for t in (kc, vc)]
+    kw = {"key_scales": ks.cuda(), "value_scales": vs.cuda()}
+    mods = {"softcap": 20.0} if scored else {}
+    out = paged_attention_decode(query, *state, tables.cuda(), lens.cuda(), 0.05, validate=True,
+                                 score_modifiers=ScoreModifiers(**mods) if scored else None, **kw)
+    assert _lib.last_kernel() == kernel
+    ref, bar = attend64(query, *state, tables, lens, 0.05, **kw, **mods)
+    check(out, ref, bar)
