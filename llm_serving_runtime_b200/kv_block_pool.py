@@ -79,13 +79,13 @@ def write_tokens_batch_into(
         if touch is not None:
             logical = (first[:, None] + torch.arange(span + 1, device=device)[None, :]).clamp_max(logical_last[:, None])
             touch(torch.gather(block_tables.to(torch.int64), 1, logical).reshape(-1))
-    scales = {}
-    if pool.k_layer_view(layer_idx).dtype == CACHE_8BIT:
+    key_cache, scales = pool.k_layer_view(layer_idx), {}
+    if key_cache.dtype == CACHE_8BIT:
         scales = {"key_scales": pool.k_layer_scales(layer_idx), "value_scales": pool.v_layer_scales(layer_idx)}
     kv_append(
         key_states,
         value_states,
-        pool.k_layer_view(layer_idx),
+        key_cache,
         pool.v_layer_view(layer_idx),
         None,
         block_tables=block_tables,

@@ -19,7 +19,7 @@ from llm_serving_runtime_b200 import (
     paged_attention_decode,
     read_device_errors,
 )
-from llm_serving_runtime_b200.kv_block_pool import Fp8KVBlockPool
+from llm_serving_runtime_b200.kv_block_pool import Fp8KVBlockPool, write_tokens_batch_into
 
 pytestmark = pytest.mark.gpu
 BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
@@ -530,3 +530,22 @@ def test_blocks_of_zeros_beside_huge_values(scored, B, q, L, M, kernel):
     assert _lib.last_kernel() == kernel
     ref, bar = attend64(query, *state, tables, lens, 0.05, **kw, **mods)
     check(out, ref, bar)
+
+
+def test_a_batched_write_takes_each_view_of_the_pool_once():
+    class Counting:
+        def __init__(self, pool):
+            self.pool, self.taken = pool, []
+
+        def __getattr__(self, name):
+            if name.startswith(("k_layer", "v_layer")):
+                self.taken.append(name)
+            return getattr(self.pool, name)
+
+    pool = Counting(Fp8KVBlockPool(4, 2, 2, 16, 64))
+    rows = torch.ones(1, 2, 3, 64, dtype=BF, device="cuda")
+    write_tokens_batch_into(pool, 1, torch.tensor([[2, 3]]), torch.tensor([15]), rows, rows)
+    assert sorted(pool.taken) == ["k_layer_scales", "k_layer_view", "v_layer_scales", "v_layer_view"]
+    torch.cuda.synchronize()
+    got = pool.pool.k.float() * pool.pool.k_scales[..., None, None]
+    assert got[2, 1, :, 15].eq(1).all() and got[3, 1, :, :2].eq(1).all() and int(got.count_nonzero()) == 2 * 3 * 64
