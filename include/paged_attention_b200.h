@@ -289,8 +289,9 @@ typedef struct pa_cache_scales {
  * (scale = need; what else it held is void); otherwise scale = max(held, need), and
  * where that grows the block's other codes are rounded again to it.  Rounding is
  * to nearest even, infinities saturate, NaN stays NaN.  All tokens of a call for
- * one block must be one row's, without a token of another block between them
- * (PA_DEVERR_BLOCK_CONFLICT else); of a slot given twice the last one counts. */
+ * one block must be one row's, without a token of another block between them and,
+ * through tables, through one entry of the row's table (PA_DEVERR_BLOCK_CONFLICT
+ * else); of a slot given twice the last one counts. */
 PA_API int pa_kv_append_8bit(const pa_kv_append_args* args, const pa_cache_scales* scales, void* stream);
 
 /* ---- changed scores --------------------------------------------------------

@@ -387,7 +387,8 @@ static int append_impl(const pa_kv_append_args* a, const pa_cache_scales* sc, vo
       return fail(PA_ERR_INVALID_ARGUMENT, "key_scales and value_scales must be given");
     st = check_cache_8bit(*a, a->block_size, a->head_dim);
     if (st != PA_OK) return st;
-    // one CTA for each block a row can touch, or each slot
+    // through tables a CTA for each block that a row can touch; through slots the kernel
+    // counts tokens (b * q_len + t) in 32 bits
     const long long runs = a->slot_mapping != nullptr ? a->q_len
                                                       : ((long long)a->q_len + a->block_size - 2) / a->block_size + 1;
     if (runs * a->batch > (1LL << 30))

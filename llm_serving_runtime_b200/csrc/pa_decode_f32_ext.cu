@@ -365,7 +365,12 @@ __global__ void __launch_bounds__(f32_warps(DPL * 32) * 32) decode_f32_ext_kerne
 
 namespace {
 
-// Row groups times splits of a launch: two CTAs an SM, as far as splits go.
+// Row groups times splits of a launch: two CTAs an SM, as far as splits go.  Both fit
+// into the shared memory at a head width of 32; from 64 on an SM holds one (132 to 134
+// KB), and a launch that uses all its splits runs in two rounds.  With one an SM
+// single rows are faster (us, 8 heads: 4000 tokens, 128 wide, 29 for 40; 8000, 64 wide,
+// 20 for 26; 32,000, 128 wide, 117 for 131), several are not (4 of 8000, 128 wide, 128 for
+// 120; 2 of 20,000 with 4 tokens, 64 wide, 156 for 149).
 constexpr int kCtasPerSm = 2;
 
 int f32_rows(const DecodeParams& p) { return p.GQ <= 4 ? 4 : 8; }

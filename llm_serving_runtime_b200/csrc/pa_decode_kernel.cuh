@@ -379,8 +379,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 1)
   // in its equal share of the total cost C.
   constexpr int kRowCostUnits = cascade ? kRowCostUnitsCascade : kRowCostUnitsPlain;
   const long long C = W + (long long)kRowCostUnits * s_rpref[B];
-  // (half of it with changed scores or 8 bits, whose units take longer: measured 15
-  // to 27 us for 22 rows of a 44-token window with shares of 2 to 8 units)
+  // (a quarter of the least share with changed scores or 8 bits, whose units take longer:
+  // measured 15 to 27 us for 22 rows of a 44-token window with shares of 2 to 8 units)
   constexpr int kMinUnits = kExt ? kMinUnitsPerWarp / 4 : kMinUnitsPerWarp;
   long long nw_eff = (C + kMinUnits - 1) / kMinUnits;
   if (nw_eff > p.nw_total) nw_eff = p.nw_total;

@@ -23,7 +23,7 @@ constexpr int kPrefillStages = 6;
 // member table check (11 warps keep the 168-register budget that 10 have).
 constexpr int umma_threads(bool prefix) { return (prefix ? 11 : 10) * 32; }
 // Minimum number of 16-token units a warp's share of the flat work list holds
-// before the kernel stops splitting the work further.
+// before the kernel stops splitting the work further (pa_decode_ext: a quarter of it).
 constexpr int kMinUnitsPerWarp = 8;
 // Cost of a row's start and end in the decode kernel's stream-K split, in
 // units: warps whose slices hold many short rows get fewer units.  Under the

@@ -49,11 +49,12 @@
 // tokens on 32,768 cached ones 5.66 ms with and without one infinite value among the
 // new tokens; where rows of two documents alternate, so that all chunks are looked over
 // again, 7.8 ms without, 8.7 with one, 8.9 with 64 and 19.5 with 4096.  4 x 1021 tokens
-// of packed documents of 700 (32/8 heads of 128, 22.6 GFLOP of visible scores): 100 us, 199 on the mma.sync kernel.  Of a CTA's
-// 22 us 11 are its 6.8 chunks (1.6 us a chunk, as without scores) and 9 what it pays
-// once: key ranges 1.0, queries 2.5, first scores 1.0, output 2.7, the next CTA's start
-// 1.2.  Loading the queries before the key ranges took longer (101.5: the fences
-// of the start wait for them), two CTAs of 128 rows an SM too (109).
+// of packed documents of 700 (32/8 heads of 128, 22.6 GFLOP of visible scores): 100 us,
+// 199 on the mma.sync kernel.  Of a CTA's 22 us 11 are its 6.8 chunks (1.6 us a chunk,
+// as without scores) and 9 what it pays once: key ranges 1.0, queries 2.5, first scores
+// 1.0, output 2.7, the next CTA's start 1.2.  Loading the queries before the key ranges
+// took longer (101.5: the fences of the start wait for them), two CTAs of 128 rows an SM
+// too (109).
 #include <limits.h>
 #include <math.h>
 

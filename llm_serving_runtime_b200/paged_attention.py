@@ -40,7 +40,10 @@ runtime/phase2/paged_kv_kernel.py:118-119, :221-222) once the copy shows a bit
 — no host synchronisation on the normal path.  ``validate=True`` (or
 ``PA_B200_VALIDATE=1``) checks synchronously at the end of the call instead;
 ``validate=False`` skips the check.  Calls under CUDA-graph capture are not
-checked (``read_device_errors`` reads the word after a replay).
+checked (``read_device_errors`` reads the word after a replay).  Calls with 8-bit
+caches or changed scores that are given no workspace, and ``copy_pages``, share one
+word a device in pinned host memory: the next such call raises, whichever stream
+or thread it is on.
 """
 
 from __future__ import annotations
@@ -629,7 +632,9 @@ def kv_append(
     2^e (e >= -100) with its largest finite magnitude at most 448 * 2^e; writing
     offset 0 starts the block anew, any other write only raises the scale, and the
     block's other codes are then rounded again.  The tokens of a block must come
-    from one row of the call (another row's are left out and flagged).
+    from one row of the call, and from one place in it: another row's, those of a row
+    that comes back to a block after another one, and those of a second entry of a
+    row's table that names the block are left out and flagged.
     head_dim is a multiple of 16, block_size a power of two in [8, 256].
     """
     if key_scales is not None and error_word is None and validate is None and not _VALIDATE_DEFAULT:
