@@ -11,6 +11,7 @@ import torch
 from _ops64 import F8, Pages, attend64, check
 from llm_serving_runtime_b200 import (
     DevicePages,
+    PrefixGroups,
     ScoreModifiers,
     _lib,
     copy_pages,
@@ -549,3 +550,35 @@ def test_a_batched_write_takes_each_view_of_the_pool_once():
     torch.cuda.synchronize()
     got = pool.pool.k.float() * pool.pool.k_scales[..., None, None]
     assert got[2, 1, :, 15].eq(1).all() and got[3, 1, :, :2].eq(1).all() and int(got.count_nonzero()) == 2 * 3 * 64
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_empty_parts_of_a_prefix_take_nothing_from_the_queries(D):
+    """A short shared prefix beside a long one, whose splits it leaves empty: an infinite query
+    of one member does not reach the others of its tile."""
+    Hkv, G, bs, q = 8, 4, 16, 1
+    g = torch.Generator().manual_seed(45)
+    prefixes, sizes = [64, 4096], [5, 2]
+    rows = [list(range(5)), [5, 6]]
+    lens = [70, 64, 90, 75, 200, 4100, 4096]
+    M = (max(lens) + q + bs - 1) // bs
+    tables, at = torch.zeros(7, M, dtype=torch.int32), 0
+    for prefix, members in zip(prefixes, rows):
+        shared = torch.arange(at, at + prefix // bs)
+        at += prefix // bs
+        for r in members:
+            tables[r, : prefix // bs] = shared
+            n = (lens[r] + q + bs - 1) // bs - prefix // bs
+            tables[r, prefix // bs: prefix // bs + n] = torch.arange(at, at + n)
+            at += n
+    kc, vc = (torch.randn(at, Hkv, bs, D, generator=g).to(BF).cuda() for _ in range(2))
+    query = torch.randn(sum(sizes), Hkv * G, q, D, generator=g).to(BF).cuda()
+    groups = PrefixGroups.from_members(rows, prefixes, 7, "cuda")
+    args = (kc, vc, tables.cuda(), _i32(lens), D**-0.5)
+    want = paged_attention_decode(query, *args, prefix_groups=groups, validate=True)
+    assert bool(want.isfinite().all())
+    query[2] = float("inf")
+    others = torch.tensor([0, 1, 3, 4, 5, 6]).cuda()
+    for _ in range(20):
+        out = paged_attention_decode(query, *args, prefix_groups=groups, validate=True)
+        assert torch.equal(out[others], want[others])
